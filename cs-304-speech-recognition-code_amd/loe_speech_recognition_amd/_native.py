@@ -22,7 +22,9 @@ HOP = 160
 N_FFT = 320
 MIN_FRAMES = 9          # the width-9 delta filter needs 9 frames (librosa raises below that)
 KERNEL_IDS = {"frame_index": 0, "mel_power": 1, "mfcc_finish": 2, "emission": 3, "viterbi": 4, "stats": 5,
-              "separation": 6}
+              "separation": 6, "top": 7, "sample": 8, "distill": 9}
+MAX_CLASSES = 1 << 24   # classes of a row of scores (LSR_MAX_CLASSES)
+MAX_TOP = 256           # listed classes per row (LSR_MAX_TOP)
 
 _PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.normpath(os.path.join(_PKG_DIR, "..", "lib", "liblsr_hip.so"))
@@ -92,6 +94,10 @@ def _declare(lib) -> None:
         "lsr_separation_scan": (c_int, [P, P, c_int, P, P, c_int, c_int64, c_int, c_double, c_double, c_int, c_int,
                                         P, P, P, P, P, P]),
         "lsr_gather_segments": (c_int, [P, P, c_int, P, P, c_int, c_int64, P]),
+        "lsr_top_scores": (c_int, [P, P, c_int, c_int64, c_int64, c_int64, c_int, c_double, P, P, P]),
+        "lsr_sample_scores": (c_int, [P, P, c_int, c_int64, c_int64, c_int64, P, c_double, c_int, c_double, c_double,
+                                      P, P, P, P, P, P]),
+        "lsr_distill_scores": (c_int, [P, P, c_int, c_int64, c_int64, c_int64, P, P, c_int, P, c_double, P, P, P]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(lib, name)          # AttributeError here = the .so does not export a declared symbol
@@ -111,7 +117,7 @@ EXPORTED_SYMBOLS = [
     "lsr_comm_destroy", "lsr_allgather_labels", "lsr_allreduce_stats", "lsr_label_record_bytes",
     "lsr_host_pack_label_records", "lsr_host_unpack_label_records", "lsr_pack_label_records", "lsr_unpack_label_records",
     "lsr_labels_from_paths", "lsr_ll_stride", "lsr_decode_chain_batch_wide", "lsr_chain_emission_mode",
-    "lsr_model_slot",
+    "lsr_model_slot", "lsr_top_scores", "lsr_sample_scores", "lsr_distill_scores",
 ]
 
 
@@ -206,7 +212,8 @@ class Engine:
         if rc != 0 or not ctx.value:
             raise NativeError(f"lsr_ctx_create({device}) failed with code {rc}")
         self.ctx = ctx
-        self._check(self.lib.lsr_set_stream(self.ctx, c_void_p(torch.cuda.current_stream(self.device).cuda_stream)))
+        self._stream = torch.cuda.current_stream(self.device)
+        self._check(self.lib.lsr_set_stream(self.ctx, c_void_p(self._stream.cuda_stream)))
         self._model_token = None
         self._graph_token = None
         self._rotated = {}               # token -> triangularised whitening matrices (at most 8 kept)
@@ -245,6 +252,29 @@ class Engine:
         if stream is None:
             stream = self.torch.cuda.current_stream(self.device)
         self._check(self.lib.lsr_set_stream(self.ctx, c_void_p(stream.cuda_stream)))
+        self._stream = stream
+
+    def on_current_stream(self, fn, *args) -> None:
+        """``fn(ctx, *args)`` on torch's current stream, after the work already queued on the engine's stream (the two are
+        usually one).  For entry points that use no workspace of the context.  While the current stream is captured the
+        engine's earlier work is not waited for: a capture starts from finished work."""
+        cuda = self.torch.cuda
+        before = cuda.current_device()
+        stream = cuda.current_stream(self.device)
+        try:
+            if stream == self._stream:
+                self._check(fn(self.ctx, *args))
+                return
+            if not cuda.is_current_stream_capturing():
+                stream.wait_stream(self._stream)
+            self._check(self.lib.lsr_set_stream(self.ctx, c_void_p(stream.cuda_stream)))
+            try:
+                self._check(fn(self.ctx, *args))
+            finally:
+                self._check(self.lib.lsr_set_stream(self.ctx, c_void_p(self._stream.cuda_stream)))
+        finally:
+            if before != self.device_index:              # the library makes its own device the current one
+                cuda.set_device(before)
 
     @staticmethod
     def _ptr(t) -> c_void_p:

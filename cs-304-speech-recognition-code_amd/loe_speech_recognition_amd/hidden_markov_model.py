@@ -20,6 +20,7 @@ import scipy.linalg
 from . import _native
 from .distributed import all_reduce_stats
 from .model_boundary import ModelBoundary
+from .scores import sample_scores, top_scores
 from .signal import Signal, SortedSignals
 from .transition_probability import LogTransitionProbabilities, TransitionProbabilities
 
@@ -707,6 +708,25 @@ class HiddenMarkovModelInference:
         if (cnt > label_cap).any():
             return self.predict_batch(eng.mfcc(ab), label_cap=label_cap)
         return _native.records_to_strings(labels.cpu().numpy(), cnt, names)
+
+    def state_scores_device(self, signals):
+        """(FeatureBatch, device tensor float32 [total frames, states]): the emission score of every state for every
+        frame (the columns of the emission matrix that hold states; a view, its row stride is larger)."""
+        eng = self._bind()
+        fb = signals if isinstance(signals, _native.FeatureBatch) else eng.feature_batch(signals)
+        return fb, eng.emission(fb)[:fb.total_frames, :len(self._multivariate_normals)]
+
+    def state_targets(self, signals, k: int, temperature: float = 1.0):
+        """(FeatureBatch, values, index, rest): the ``k`` best states of every frame as targets for a student that is
+        trained with ``distill_scores`` (same temperature there); device tensors as ``top_scores`` returns them."""
+        fb, scores = self.state_scores_device(signals)
+        return (fb, *top_scores(scores, k, temperature=temperature, want_rest=True))
+
+    def sample_states(self, signals, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+        """(FeatureBatch, index int32 [total frames], logprob): a state per frame drawn from the emission scores with one
+        uniform number per frame (device tensor float32); settings as in ``sample_scores``."""
+        fb, scores = self.state_scores_device(signals)
+        return (fb, *sample_scores(scores, uniform, temperature, top_k, top_p, min_p))
 
     def _viterbi(self, observation_sequence: np.ndarray) -> Tuple[np.float32, np.ndarray]:
         return self.viterbi_batch([observation_sequence])[0]

@@ -7,12 +7,13 @@ from __future__ import annotations
 
 import os
 from dataclasses import dataclass, field
-from typing import List
+from typing import List, Optional, Tuple
 
 import numpy as np
 
 from . import _native
 from .hidden_markov_model import HiddenMarkovModel, stack_gaussians
+from .scores import sample_scores, top_scores
 from .ti_digits import TI_DIGITS_LABELS
 
 
@@ -76,6 +77,26 @@ class ModelCollection:
 
     def predict(self, signal: np.ndarray) -> str:
         return self.predict_batch([signal])[0]
+
+    def nbest_batch(self, signals, n: int) -> List[List[Tuple[str, np.float32]]]:
+        """The ``n`` best (label, score) pairs of every utterance, best first, models with equal scores in the order of
+        the collection: the head of the sorted list of which ``predict`` returns the first label (model_collection.py:26-28).
+        A model that cannot score an utterance (-inf) is left out."""
+        values, index, _ = top_scores(self.scores_device(signals), n)
+        names = [str(m) for m in self._models]
+        return [[(names[i], v) for i, v in zip(row_i, row_v) if i >= 0]
+                for row_i, row_v in zip(index.cpu().numpy().tolist(), values.cpu().numpy())]
+
+    def sample_batch(self, signals, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0) -> List[Optional[str]]:
+        """A label per utterance drawn in proportion to ``exp(score / temperature)`` among the models that the cuts leave
+        (see ``sample_scores``), with the uniform numbers given - for instance pseudo-labels that keep the recogniser's
+        doubt.  Scores are log-likelihoods of whole utterances; a temperature of the order of the utterances' frames makes
+        them comparable per frame.  None where no model can score the utterance."""
+        scores = self.scores_device(signals)
+        uniform = _native.get_engine().to_device(np.asarray(uniform, dtype=np.float32))
+        index, _ = sample_scores(scores, uniform, temperature, top_k, top_p, min_p)
+        names = [str(m) for m in self._models]
+        return [names[i] if i >= 0 else None for i in index.cpu().numpy().tolist()]
 
     @classmethod
     def load_from_files(cls, folder_path: str):

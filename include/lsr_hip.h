@@ -63,7 +63,10 @@ typedef struct lsr_ctx lsr_ctx;
 #define LSR_K_VITERBI 4
 #define LSR_K_STATS 5
 #define LSR_K_SEPARATION 6
-#define LSR_K_COUNT 7
+#define LSR_K_TOP 7
+#define LSR_K_SAMPLE 8
+#define LSR_K_DISTILL 9
+#define LSR_K_COUNT 10
 
 /* ---- context ---------------------------------------------------------------------------- */
 int lsr_ctx_create(int device, lsr_ctx** out);
@@ -359,6 +362,61 @@ int lsr_pack_label_records(lsr_ctx* ctx, const uint8_t* labels_d, const int32_t*
                            int label_cap, int64_t shard_cap, uint8_t* records_d);
 int lsr_unpack_label_records(lsr_ctx* ctx, const uint8_t* records_d, int world, int64_t n_total, int label_cap,
                              uint8_t* labels_out_d, int32_t* n_labels_out_d);
+
+/* ---- rows of log scores --------------------------------------------------------------------- */
+/* What a model answers with is a matrix of log scores, a row per frame, clip or token and a column per class: emission
+ * scores (lsr_emission_batch), the last-frame scores of a collection (lsr_decode_chain_batch), the output of a student
+ * that is trained on them.  The reference only takes the arg-max of such rows (model_collection.py:26-28); the three
+ * entry points below take the n best, draw from a row, and train a student on the n best of a teacher.
+ *
+ * scores_d: n_rows rows of n_classes (1..LSR_MAX_CLASSES) elements of `dtype`, classes adjacent, row_stride elements
+ * from row to row (any value >= 0; 0 gives every row the same scores).  Order of a row: score descending, equal scores
+ * (-0 and +0 are equal) by ascending class; a score of -infinity or NaN is absent from lsr_top_scores and
+ * lsr_sample_scores.  n_rows = 0 is valid and does nothing.  The calls only enqueue kernels: no allocation, no copy and no
+ * memset, so they can be captured into a graph, and calls on different streams share nothing.  Results do not depend on
+ * the launch: the same inputs give the same bits. */
+#define LSR_F32 0
+#define LSR_F16 1
+#define LSR_BF16 2
+#define LSR_MAX_CLASSES (1 << 24)
+#define LSR_MAX_TOP 256
+
+/* The first k (1..min(n_classes, LSR_MAX_TOP)) entries of every row: values_d float32[n_rows][k], index_d
+ * int32[n_rows][k]; a row with fewer entries is filled with -infinity / -1.  rest_d float32[n_rows] (may be NULL): log of
+ * the sum of e^((x - x_best) / temperature) over the other entries of the row, -infinity if there are none - the log
+ * weight of "any other class" relative to the row's best. */
+int lsr_top_scores(lsr_ctx* ctx, const void* scores_d, int dtype, int64_t n_rows, int64_t n_classes, int64_t row_stride,
+                   int k, double temperature, float* values_d, int32_t* index_d, float* rest_d);
+
+/* One class per row from a uniform number uniform_d[n_rows] in [0, 1) (values outside are clamped).  With weights
+ * w = e^((x - x_best) / temperature) the row keeps, of its order, the shorter of: the first top_k entries (<= 0: all); of
+ * those the shortest head that holds top_p of their weight (>= 1: all, <= 0: the first); the entries with
+ * x >= x_best + temperature ln(min_p) (<= 0: all, values above 1 count as 1).  index_d[n_rows] is the first class, in
+ * ascending class order, at which the running weight of the kept classes exceeds uniform * their total, logprob_d[n_rows]
+ * the log of its share of the total.  temperature <= 0 (or NaN in temperature_d): the row's first entry, log share 0.  A
+ * row without entries: -1, -infinity.  If the row holds +infinity only those entries have weight.  Each setting is one
+ * number for all rows or, where its pointer is not NULL, float32 / int32[n_rows].  Weights are computed in 64 bits and
+ * summed as whole multiples of 2^-52 (up to 1 024 classes) ... 2^-38 (2^24 classes) of the best one's. */
+int lsr_sample_scores(lsr_ctx* ctx, const void* scores_d, int dtype, int64_t n_rows, int64_t n_classes, int64_t row_stride,
+                      const float* uniform_d, double temperature, int top_k, double top_p, double min_p,
+                      const float* temperature_d, const int32_t* top_k_d, const float* top_p_d, const float* min_p_d,
+                      int32_t* index_d, float* logprob_d);
+
+/* Loss of a student's scores against a teacher's top scores, and its gradient.  Teacher rows: top_values_d
+ * float32[n_rows][k] with classes top_index_d int32[n_rows][k] (k in 1..LSR_MAX_TOP) and, if rest_d is not NULL, the log
+ * weight of all other classes relative to the best value, as lsr_top_scores gives them; an entry whose class lies outside
+ * 0..n_classes - 1 or whose value is -infinity or NaN is absent, a class that is given twice counts with both.  With
+ * p = softmax of the teacher's entries / temperature (with the rest as one more outcome), q = softmax(scores /
+ * temperature) and q_rest the student's weight on the classes that are not listed
+ *   loss_d[r]    = w temperature^2 [ sum p (ln p - ln q) + p_rest (ln p_rest - ln q_rest) ]        (w = row_weight_d[r], NULL: 1)
+ *   grad_d[r][i] = d loss_d[r] / d scores[r][i] = w temperature [ q_i - p_i - (i not listed) p_rest q_i / q_rest ]
+ * grad_d (elements of `dtype`, rows of n_classes back to back, must not overlap the scores; may be NULL) is the gradient of
+ * the sum of the losses.  Loss and gradient are exactly 0 for a row whose weight is 0, whose teacher has no entry or whose
+ * scores are all -infinity, and NaN for any other row with a NaN or +infinity among its scores.  k = 1 with temperature 1
+ * and no rest is the cross entropy with a class label. */
+int lsr_distill_scores(lsr_ctx* ctx, const void* scores_d, int dtype, int64_t n_rows, int64_t n_classes, int64_t row_stride,
+                       const float* top_values_d, const int32_t* top_index_d, int k, const float* rest_d, double temperature,
+                       const float* row_weight_d, float* loss_d, void* grad_d);
 
 /* ---- silence stripping ------------------------------------------------------------------- */
 /* Replaces the per-clip scan of SignalSeparation._remove_empty / .detect_speech
