@@ -124,6 +124,145 @@ __global__ __launch_bounds__(LSR_ROW_THREADS) void lsr_distill_kernel(
     }
 }
 
+// Short rows (at most LSR_QUAD_CLASSES classes), a quad per row.  The teacher's weights are added up per class in LDS, in
+// the place of the quad's own row (no other wavefront touches it), and read back into registers beside the scores.
+// With z = (x - m) / T, y = (t - best) / T, S the sum of the teacher's weights e^y and of e^rest:
+//   KL = 1/S sum_j e^{y_j} (y_j - z_j) + ln Z - ln S + p_R (rest - ln q_R - ln Z),
+// one logarithm instruction sequence for Z, S and the rest together, a lane each.
+template <int DT, int E, bool REST, bool GRAD>
+__global__ __launch_bounds__(LSR_ROW_THREADS) void lsr_distill_quad_kernel(
+    const typename row_type<DT>::type* __restrict__ scores, int64_t n_rows, int n_classes, int64_t row_stride,
+    const float* __restrict__ values, const int32_t* __restrict__ index, int k, const float* __restrict__ rest,
+    double temperature, const float* __restrict__ weight, float* __restrict__ loss,
+    typename row_type<DT>::type* __restrict__ grad) {
+    // 16 floats of padding: the runs that 16 lanes read at once, four rows', lie in different banks
+    __shared__ float listed[LSR_QUAD_ROWS][4 * E + 16];
+    const int q = threadIdx.x & 3, slot = threadIdx.x >> 2;
+    const int64_t row = (int64_t)blockIdx.x * LSR_QUAD_ROWS + slot;
+    const bool live = row < n_rows;
+    const int64_t r = live ? row : n_rows - 1;            // every lane takes part in the exchanges
+    const auto* mine = scores + r * row_stride;
+    float x[E];
+    quad_load<DT, E>(mine, n_classes, (n_rows - 1 - r) * row_stride + n_classes, q, x);
+    float4* own = (float4*)&listed[slot][q * 4];
+#pragma unroll
+    for (int g = 0; g < E / 4; ++g) own[g * 4] = make_float4(0, 0, 0, 0);
+    row_wave_fence();
+    const double inv_t = 1.0 / temperature, unit = inv_t * ROW_LOG2E;
+    float m = -INFINITY;
+    int nan = 0;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        nan |= !(x[i] < INFINITY);
+        m = row_max(m, x[i]);
+    }
+    m = quad_max(m);
+    nan = quad_max(nan);
+    float best = -INFINITY;
+    for (int j = q; j < k; j += 4) {
+        const int c = index[r * k + j];
+        const float v = values[r * k + j];
+        if (c >= 0 && c < n_classes && v > best) best = v;
+    }
+    best = quad_max(best);
+    const double w = weight ? (double)weight[r] : 1.0;
+    const bool used = w != 0 && best > -INFINITY && (m > -INFINITY || nan);
+    double sum = 0, cross = 0;
+    for (int j = q; j < k; j += 4) {
+        const int c = index[r * k + j];
+        const float v = values[r * k + j];
+        if (c < 0 || c >= n_classes || !(v > -INFINITY)) continue;
+        const double y = v == best ? 0.0 : ((double)v - best) * unit, z = ((double)(float)mine[c] - m) * unit;
+        const double p = row_exp2(y);
+        sum += p;
+        if (p > 0) cross += p * (y - z);
+        // at least the smallest normal number: what is in the list is what is not 0
+        atomicAdd(&listed[slot][c], fmaxf((float)p, 1.17549435e-38f));
+    }
+    row_wave_fence();
+    sum = quad_sum(sum);
+    cross = quad_sum(cross) * (1.0 / ROW_LOG2E);
+    float p[E];
+#pragma unroll
+    for (int g = 0; g < E / 4; ++g) {
+        const float4 f = own[g * 4];
+        p[4 * g] = f.x;
+        p[4 * g + 1] = f.y;
+        p[4 * g + 2] = f.z;
+        p[4 * g + 3] = f.w;
+    }
+    // sums of e^z relative to m for what is listed and relative to m_r for the others (relative to m for all without rest)
+    float m_r = m;
+    if (REST) {
+        m_r = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < E; ++i)
+            if (!(p[i] > 0)) m_r = row_max(m_r, x[i]);
+        m_r = quad_max(m_r);
+    }
+    const float unit_f = (float)unit, from = m_r > -INFINITY ? m_r : 0.0f;
+    float z_l = 0, z_r = 0;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        const bool in = REST && p[i] > 0;
+        x[i] = __builtin_amdgcn_exp2f((x[i] - (in ? m : from)) * unit_f);
+        if (in)
+            z_l += x[i];
+        else
+            z_r += x[i];
+    }
+    z_l = quad_sum(z_l);
+    z_r = quad_sum(z_r);
+    const double shift = REST && z_r > 0 ? row_exp2(((double)m_r - m) * unit) : 1.0;
+    const double z = REST ? z_l + shift * z_r : z_r;
+    double p_r = 0, rest_log = 0;
+    if (REST) {
+        rest_log = (double)rest[r];
+        p_r = exp(rest_log);
+        sum += p_r;
+    }
+    const double ln = log(q == 0 ? z : q == 1 ? sum : (double)z_r);
+    const double ln_z = quad_move<0x00>(ln), ln_s = quad_move<0x55>(ln), ln_r = quad_move<0xAA>(ln);
+    if (live && q == 0) {
+        double l = cross / sum + ln_z - ln_s;
+        if (REST && p_r > 0) l += p_r / sum * (z_r > 0 ? rest_log - ln_r - ((double)m_r - m) * inv_t : INFINITY);
+        loss[r] = used ? (nan ? NAN : (float)(w * temperature * temperature * l)) : 0.0f;
+    }
+    if (!GRAD || !live) return;
+    const double scale = w * temperature;
+    const float c_l = (float)(scale / z), c_p = (float)(scale / sum);
+    const float c_r = REST ? (z_r > 0 ? (float)(scale * (shift / z - p_r / sum / z_r)) : 0.0f) : c_l;
+#pragma unroll
+    for (int g = 0; g < E / 4; ++g) {
+        float d[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int i = 4 * g + j;
+            d[j] = (REST && p[i] > 0 ? c_l : c_r) * x[i] - c_p * p[i];
+            d[j] = used ? (nan ? NAN : d[j]) : 0.0f;
+        }
+        quad_store(grad + r * n_classes, n_classes, g, q, d);
+    }
+}
+
+template <int DT, int E>
+static void lsr_distill_quad(hipStream_t stream, const void* scores_d, int64_t n_rows, int n_classes, int64_t row_stride,
+                             const float* values_d, const int32_t* index_d, int k, const float* rest_d, double temperature,
+                             const float* weight_d, float* loss_d, void* grad_d) {
+    const auto* scores = (const typename row_type<DT>::type*)scores_d;
+    auto* grad = (typename row_type<DT>::type*)grad_d;
+    const dim3 grid((unsigned)((n_rows + LSR_QUAD_ROWS - 1) / LSR_QUAD_ROWS));
+#define LAUNCH(REST, GRAD)                                                                                                   \
+    hipLaunchKernelGGL((lsr_distill_quad_kernel<DT, E, REST, GRAD>), grid, dim3(LSR_ROW_THREADS), 0, stream, scores, n_rows,   \
+                       n_classes, row_stride, values_d, index_d, k, rest_d, temperature, weight_d, loss_d, grad)
+    if (rest_d) {
+        if (grad_d) LAUNCH(true, true); else LAUNCH(true, false);
+    } else {
+        if (grad_d) LAUNCH(false, true); else LAUNCH(false, false);
+    }
+#undef LAUNCH
+}
+
 extern "C" int lsr_distill_scores(lsr_ctx* ctx, const void* scores_d, int dtype, int64_t n_rows, int64_t n_classes,
                                   int64_t row_stride, const float* top_values_d, const int32_t* top_index_d, int k,
                                   const float* rest_d, double temperature, const float* row_weight_d, float* loss_d,
@@ -142,6 +281,15 @@ extern "C" int lsr_distill_scores(lsr_ctx* ctx, const void* scores_d, int dtype,
     LSR_HIP_CHECK(ctx, hipSetDevice(ctx->device));
     const dim3 grid((unsigned)(n_rows < 65536 ? n_rows : 65536));
     lsr_prof_begin(ctx, LSR_K_DISTILL);
+    if (n_classes <= LSR_QUAD_CLASSES) {
+        LSR_DTYPE_SWITCH(dtype, LSR_QUAD_SWITCH(n_classes, lsr_distill_quad<DT, E>(ctx->stream, scores_d, n_rows, (int)n_classes,
+                                                                                   row_stride, top_values_d, top_index_d, k,
+                                                                                   rest_d, temperature, row_weight_d, loss_d,
+                                                                                   grad_d)));
+        lsr_prof_end(ctx);
+        LSR_LAUNCH_CHECK(ctx, "lsr_distill_quad_kernel");
+        return LSR_OK;
+    }
     if (dtype == LSR_F32)
         hipLaunchKernelGGL(lsr_distill_kernel<ROW_F32>, grid, dim3(LSR_ROW_THREADS), 0, ctx->stream, (const float*)scores_d,
                            n_rows, (int)n_classes, row_stride, top_values_d, top_index_d, k, rest_d, temperature, row_weight_d,

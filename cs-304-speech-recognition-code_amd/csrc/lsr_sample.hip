@@ -148,6 +148,146 @@ __global__ __launch_bounds__(LSR_ROW_THREADS) void lsr_sample_kernel(const typen
     }
 }
 
+// Short rows (at most LSR_QUAD_CLASSES classes), a quad per row.  ORDER: some row is cut by its order, so the entries are
+// sorted; the sorted weights give the threshold, which the registers in class order are then compared with.  The sums are
+// 64-bit floating ones in a fixed order.
+template <int DT, int E, bool ORDER>
+__global__ __launch_bounds__(LSR_ROW_THREADS) void lsr_sample_quad_kernel(const typename row_type<DT>::type* __restrict__ scores,
+                                                                          int64_t n_rows, int n_classes, int64_t row_stride,
+                                                                          const float* __restrict__ uniform, sample_args a,
+                                                                          int32_t* __restrict__ index,
+                                                                          float* __restrict__ logprob) {
+    const int q = threadIdx.x & 3;
+    const int64_t row = (int64_t)blockIdx.x * LSR_QUAD_ROWS + (threadIdx.x >> 2);
+    const bool live = row < n_rows;
+    const int64_t r = live ? row : n_rows - 1;            // every lane takes part in the exchanges
+    float x[E];
+    quad_load<DT, E>(scores + r * row_stride, n_classes, (n_rows - 1 - r) * row_stride + n_classes, q, x);
+    const double t = a.temperature_d ? (double)a.temperature_d[r] : a.temperature;
+    const double min_p = a.min_p_d ? (double)a.min_p_d[r] : a.min_p;
+    float best = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        x[i] = x[i] > -INFINITY ? x[i] : -INFINITY;       // NaN is absent
+        best = row_max(best, x[i]);
+    }
+    best = quad_max(best);
+    const bool none = best == -INFINITY;
+    if (__any(best == INFINITY)) {                        // only the infinite ones have weight
+#pragma unroll
+        for (int i = 0; i < E; ++i)
+            if (best == INFINITY) x[i] = x[i] == INFINITY ? 0.0f : -INFINITY;
+        if (best == INFINITY) best = 0.0f;
+    }
+    const double unit = ROW_LOG2E / t;
+    float last = -INFINITY;                               // the last entry that is kept
+    int last_class = n_classes;
+    if (ORDER) {
+        const double top_p = a.top_p_d ? (double)a.top_p_d[r] : a.top_p;
+        const int cut = a.top_k_d ? a.top_k_d[r] : a.top_k;
+        const int top_k = cut > 0 ? cut : 4 * E;
+        double e[E], w[E];
+#pragma unroll
+        for (int i = 0; i < E; ++i) e[i] = quad_entry(row_key(x[i]), quad_class(i, q));
+        quad_sort<E>(e, q);
+        double sum = 0, least = 3.9;
+#pragma unroll
+        for (int i = 0; i < E; ++i) w[i] = 0;
+        if (__any(top_p < 1)) {
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                const uint32_t key = quad_entry_key(e[i]);
+                w[i] = key && q * E + i < top_k ? row_exp2(((double)row_value(key) - best) * unit) : 0.0;
+                sum += w[i];
+            }
+        }
+        const double target = top_p < 1 ? top_p * quad_sum(sum) : INFINITY;
+        double run = quad_before(sum, q);
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            const int place = q * E + i;
+            // a place is kept while the weight ahead of it is short of the target
+            if (place < top_k && (place == 0 || run < target) && quad_entry_key(e[i])) least = row_min(least, e[i]);
+            run += w[i];
+        }
+        least = quad_min(least);
+        if (!none) {
+            last = row_value(quad_entry_key(least));
+            last_class = quad_entry_class(least);
+        }
+    }
+    if (min_p > 0) {
+        const double low = (double)best + t * log(min_p < 1.0 ? min_p : 1.0);
+        float f = (float)low;
+        if ((double)f < low) f = nextafterf(f, INFINITY);
+        if (f > last) {
+            last = f;
+            last_class = n_classes;
+        }
+    }
+    double w[E], total = 0;
+    const bool greedy = !(t > 0);
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        const bool kept = x[i] > last || (x[i] == last && quad_class(i, q) <= last_class);
+        w[i] = kept && x[i] > -INFINITY ? row_exp2(((double)x[i] - best) * unit) : 0.0;
+    }
+    double lane[E / 4];
+#pragma unroll
+    for (int g = 0; g < E / 4; ++g) {
+        lane[g] = (w[4 * g] + w[4 * g + 1]) + (w[4 * g + 2] + w[4 * g + 3]);
+        total += quad_sum(lane[g]);
+    }
+    const double goal = (double)uniform[r] * total;
+    double base = 0;
+    int at = 1 << 30, end = -1;
+#pragma unroll
+    for (int g = 0; g < E / 4; ++g) {
+        double run = base + quad_before(lane[g], q);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            run += w[4 * g + j];
+            if (w[4 * g + j] > 0) {
+                end = quad_class(4 * g + j, q);
+                if (run > goal) at = min(at, end);
+            }
+        }
+        base += quad_sum(lane[g]);
+    }
+    at = quad_min(at);
+    end = quad_max(end);
+    if (at >= n_classes) at = end;                        // a uniform number of 1 or more
+    if (__any(greedy)) {
+        int first = 1 << 30;
+#pragma unroll
+        for (int i = 0; i < E; ++i)
+            if (x[i] == best) first = min(first, quad_class(i, q));
+        first = quad_min(first);
+        if (greedy) at = first;
+    }
+    if (!live || q) return;
+    index[r] = none ? -1 : at;
+    float share = -INFINITY;
+    if (!none && !greedy) {
+        const float v = (float)scores[r * row_stride + at];
+        share = (float)((isinf(v) ? 0.0 : ((double)v - best) / t) - log(total));
+    }
+    logprob[r] = !none && greedy ? 0.0f : share;
+}
+
+template <int DT, int E>
+static void lsr_sample_quad(hipStream_t stream, const void* scores_d, int64_t n_rows, int n_classes, int64_t row_stride,
+                            const float* uniform_d, const sample_args& a, bool order, int32_t* index_d, float* logprob_d) {
+    const auto* scores = (const typename row_type<DT>::type*)scores_d;
+    const dim3 grid((unsigned)((n_rows + LSR_QUAD_ROWS - 1) / LSR_QUAD_ROWS));
+    if (order)
+        hipLaunchKernelGGL((lsr_sample_quad_kernel<DT, E, true>), grid, dim3(LSR_ROW_THREADS), 0, stream, scores, n_rows,
+                           n_classes, row_stride, uniform_d, a, index_d, logprob_d);
+    else
+        hipLaunchKernelGGL((lsr_sample_quad_kernel<DT, E, false>), grid, dim3(LSR_ROW_THREADS), 0, stream, scores, n_rows,
+                           n_classes, row_stride, uniform_d, a, index_d, logprob_d);
+}
+
 extern "C" int lsr_sample_scores(lsr_ctx* ctx, const void* scores_d, int dtype, int64_t n_rows, int64_t n_classes,
                                  int64_t row_stride, const float* uniform_d, double temperature, int top_k, double top_p,
                                  double min_p, const float* temperature_d, const int32_t* top_k_d, const float* top_p_d,
@@ -167,7 +307,16 @@ extern "C" int lsr_sample_scores(lsr_ctx* ctx, const void* scores_d, int dtype, 
     sample_args a = {temperature, top_p,  min_p, top_k, temperature_d, top_p_d, min_p_d, top_k_d, ldexp(1.0, 52 - shift),
                      ldexp(1.0, -shift)};
     const dim3 grid((unsigned)(n_rows < 65536 ? n_rows : 65536));
+    const bool order = top_k_d || top_p_d || (top_k > 0 && top_k < n_classes) || top_p < 1;
     lsr_prof_begin(ctx, LSR_K_SAMPLE);
+    if (n_classes <= LSR_QUAD_CLASSES) {
+        LSR_DTYPE_SWITCH(dtype, LSR_QUAD_SWITCH(n_classes, lsr_sample_quad<DT, E>(ctx->stream, scores_d, n_rows, (int)n_classes,
+                                                                                  row_stride, uniform_d, a, order, index_d,
+                                                                                  logprob_d)));
+        lsr_prof_end(ctx);
+        LSR_LAUNCH_CHECK(ctx, "lsr_sample_quad_kernel");
+        return LSR_OK;
+    }
     if (dtype == LSR_F32)
         hipLaunchKernelGGL(lsr_sample_kernel<ROW_F32>, grid, dim3(LSR_ROW_THREADS), 0, ctx->stream, (const float*)scores_d,
                            n_rows, (int)n_classes, row_stride, uniform_d, a, index_d, logprob_d);

@@ -116,6 +116,84 @@ __global__ __launch_bounds__(LSR_ROW_THREADS) void lsr_top_kernel(const typename
     }
 }
 
+// Short rows (at most LSR_QUAD_CLASSES classes), a quad per row: the entries are sorted by a network over the quad's
+// registers; for k <= E only the first E places are merged, which drops half of every exchange between lanes.
+template <int DT, int E, bool HEAD, bool REST>
+__global__ __launch_bounds__(LSR_ROW_THREADS) void lsr_top_quad_kernel(const typename row_type<DT>::type* __restrict__ scores,
+                                                                       int64_t n_rows, int n_classes, int64_t row_stride, int k,
+                                                                       float inv_t, float* __restrict__ values,
+                                                                       int32_t* __restrict__ index, float* __restrict__ rest) {
+    const int q = threadIdx.x & 3;
+    const int64_t row = (int64_t)blockIdx.x * LSR_QUAD_ROWS + (threadIdx.x >> 2);
+    const bool live = row < n_rows;
+    const int64_t r = live ? row : n_rows - 1;            // every lane takes part in the exchanges
+    float x[E];
+    quad_load<DT, E>(scores + r * row_stride, n_classes, (n_rows - 1 - r) * row_stride + n_classes, q, x);
+    double e[E];
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        x[i] = x[i] > -INFINITY ? x[i] : -INFINITY;      // NaN is absent
+        e[i] = quad_entry(row_key(x[i]), quad_class(i, q));
+    }
+    if (HEAD)
+        quad_sort_head<E>(e);
+    else
+        quad_sort<E>(e, q);
+    double least = 3.9;                                   // entry at place k - 1
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        const int place = HEAD ? i : q * E + i;
+        if (REST) least = place == k - 1 ? e[i] : least;
+        // with HEAD all lanes hold the same places: lane q writes the places that are q modulo 4
+        if (live && place < k && (!HEAD || (place & 3) == q)) {
+            const uint32_t key = quad_entry_key(e[i]);
+            values[r * k + place] = key ? row_value(key) : -INFINITY;
+            index[r * k + place] = key ? quad_entry_class(e[i]) : -1;
+        }
+    }
+    if (!REST) return;
+    if (!HEAD) least = quad_min(least);
+    // the best entry is at place 0
+    const double top = HEAD ? e[0] : quad_move<0x00>(e[0]);
+    const uint32_t best_key = quad_entry_key(top);
+    const float best = best_key ? row_value(best_key) : 0.0f;
+    // relative to the highest score of the rest: relative to the row's best it could underflow to nothing
+    const uint32_t last_key = quad_entry_key(least);
+    const float last = last_key ? row_value(last_key) : -INFINITY;
+    const int last_class = quad_entry_class(least);
+    float high = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        const bool beyond = x[i] < last || (x[i] == last && quad_class(i, q) > last_class);
+        x[i] = beyond ? x[i] : -INFINITY;
+        high = row_max(high, x[i]);
+    }
+    high = quad_max(high);
+    float sum = 0.0f;
+    const float unit = inv_t * 1.44269504f;
+#pragma unroll
+    for (int i = 0; i < E; ++i) sum += x[i] == high ? 1.0f : __builtin_amdgcn_exp2f((x[i] - high) * unit);
+    sum = quad_sum(sum);
+    if (live && q == 0)
+        rest[r] = high > -INFINITY ? (high == best ? 0.0f : (high - best) * inv_t) + logf(sum) : -INFINITY;
+}
+
+template <int DT, int E>
+static void lsr_top_quad(hipStream_t stream, const void* scores_d, int64_t n_rows, int n_classes, int64_t row_stride, int k,
+                         float inv_t, float* values_d, int32_t* index_d, float* rest_d) {
+    const auto* scores = (const typename row_type<DT>::type*)scores_d;
+    const dim3 grid((unsigned)((n_rows + LSR_QUAD_ROWS - 1) / LSR_QUAD_ROWS));
+#define LAUNCH(HEAD, REST)                                                                                                   \
+    hipLaunchKernelGGL((lsr_top_quad_kernel<DT, E, HEAD, REST>), grid, dim3(LSR_ROW_THREADS), 0, stream, scores, n_rows,       \
+                       n_classes, row_stride, k, inv_t, values_d, index_d, rest_d)
+    if (k <= E) {
+        if (rest_d) LAUNCH(true, true); else LAUNCH(true, false);
+    } else {
+        if (rest_d) LAUNCH(false, true); else LAUNCH(false, false);
+    }
+#undef LAUNCH
+}
+
 extern "C" int lsr_top_scores(lsr_ctx* ctx, const void* scores_d, int dtype, int64_t n_rows, int64_t n_classes,
                               int64_t row_stride, int k, double temperature, float* values_d, int32_t* index_d,
                               float* rest_d) {
@@ -131,6 +209,13 @@ extern "C" int lsr_top_scores(lsr_ctx* ctx, const void* scores_d, int dtype, int
     const dim3 grid((unsigned)(n_rows < 65536 ? n_rows : 65536));
     const float inv_t = (float)(1.0 / temperature);
     lsr_prof_begin(ctx, LSR_K_TOP);
+    if (n_classes <= LSR_QUAD_CLASSES) {
+        LSR_DTYPE_SWITCH(dtype, LSR_QUAD_SWITCH(n_classes, lsr_top_quad<DT, E>(ctx->stream, scores_d, n_rows, (int)n_classes,
+                                                                               row_stride, k, inv_t, values_d, index_d, rest_d)));
+        lsr_prof_end(ctx);
+        LSR_LAUNCH_CHECK(ctx, "lsr_top_quad_kernel");
+        return LSR_OK;
+    }
     if (dtype == LSR_F32)
         hipLaunchKernelGGL(lsr_top_kernel<ROW_F32>, grid, dim3(LSR_ROW_THREADS), 0, ctx->stream, (const float*)scores_d,
                            n_rows, (int)n_classes, row_stride, k, inv_t, values_d, index_d, rest_d);
