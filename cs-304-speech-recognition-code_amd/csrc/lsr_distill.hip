@@ -11,116 +11,176 @@
 
 #include "lsr_rows.h"
 
-template <int DT>
-__global__ __launch_bounds__(LSR_ROW_THREADS) void lsr_distill_kernel(
-    const typename row_type<DT>::type* __restrict__ scores, int64_t n_rows, int n_classes, int64_t row_stride,
+// Long rows, a team of W wavefronts per row (lsr_rows.h).  Wavefront 0 handles the list while the row is on its way; the
+// listed classes are marked in a bit map, and where there is an outcome for the rest they are blanked in the registers, so
+// that maximum, sum and gradient run over the others alone.  The gradient of the listed classes is written over afterwards.
+template <int DT, int W, int N, bool REST, bool GRAD>
+__global__ __launch_bounds__(64 * W) void lsr_distill_team_kernel(
+    const typename row_type<DT>::type* __restrict__ scores, int n_classes, int64_t row_stride,
     const float* __restrict__ values, const int32_t* __restrict__ index, int k, const float* __restrict__ rest,
     double temperature, const float* __restrict__ weight, float* __restrict__ loss,
     typename row_type<DT>::type* __restrict__ grad) {
     using T = typename row_type<DT>::type;
-    __shared__ int cls[LSR_MAX_TOP];
-    __shared__ float teacher[LSR_MAX_TOP];                // the teacher's values, then probabilities
+    using Row = team_row<DT, W, N>;
+    constexpr int THREADS = 64 * W, RUN = Row::RUN, MAP = W == 1 ? 1024 : W == 4 ? 16384 : 131072;   // bits of the map
+    __shared__ uint32_t map[MAP / 32];
+    __shared__ int cls[LSR_MAX_TOP];                      // listed classes, -1 for absent entries
+    __shared__ float teacher[LSR_MAX_TOP];                // values, then weights relative to the best
     __shared__ float student[LSR_MAX_TOP];                // scores of the listed classes
-    __shared__ bool first[LSR_MAX_TOP];                   // the class was not listed before
-    __shared__ float part[LSR_ROW_THREADS / 64];
-    __shared__ double row[8];
+    __shared__ bool first[LSR_MAX_TOP];                   // the class has not been listed before
+    __shared__ float part_f[W];
+    __shared__ double part_d[W], constant[5];
+    __shared__ int again, state;
     const int tid = threadIdx.x;
-    const double inv_t = 1.0 / temperature;
-    for (int64_t r = blockIdx.x; r < n_rows; r += gridDim.x) {
-        const T* x = scores + r * row_stride;
-        T* g = grad ? grad + r * n_classes : nullptr;
-        const double w = weight ? (double)weight[r] : 1.0;
-        __syncthreads();
-        if (tid < k) {
-            const int c = index[r * k + tid];
-            const float v = values[r * k + tid];
-            const bool there = c >= 0 && c < n_classes && v > -INFINITY;
-            cls[tid] = there ? c : -1;
-            teacher[tid] = there ? v : -INFINITY;
-            student[tid] = there ? (float)x[c] : -INFINITY;
-        }
-        __syncthreads();
-        if (tid < k) {
-            bool f = cls[tid] >= 0;
-            for (int j = 0; j < tid; ++j) f &= cls[j] != cls[tid];
-            first[tid] = f;
-        }
-        // highest score and sum of the classes that are not listed (all of them when there is no bucket for the others)
-        auto listed = [&](int c) {
-            bool f = false;
-            for (int j = 0; j < k; ++j) f |= cls[j] == c;
-            return f;
-        };
-        float high = -INFINITY;
-        bool nan = false;
-        for (int c = tid; c < n_classes; c += LSR_ROW_THREADS) {
-            const float v = (float)x[c];
-            nan |= !(v < INFINITY);                        // +infinity makes the softmax undefined as well
-            if (v > high && !listed(c)) high = v;
-        }
-        for (int d = 32; d; d >>= 1) high = fmaxf(high, __shfl_xor(high, d));
-        if ((tid & 63) == 0) part[tid >> 6] = high;
-        nan = __syncthreads_or(nan);
-        high = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
-        __syncthreads();
-        float sum = 0.0f;
-        if (high > -INFINITY)
-            for (int c = tid; c < n_classes; c += LSR_ROW_THREADS)
-                if (!listed(c)) sum += expf(((float)x[c] - high) * (float)inv_t);
-        sum = row_wave_sum(sum);
-        if ((tid & 63) == 0) part[tid >> 6] = sum;
-        __syncthreads();
-        if (tid == 0) {                                   // the few numbers of a row, in 64 bits
-            const double z_r = (double)part[0] + part[1] + part[2] + part[3], m_r = (double)high * inv_t;
-            double best = -INFINITY, m = z_r > 0 ? m_r : -INFINITY, p_sum = 0, p_r = 0;
-            for (int j = 0; j < k; ++j) {
-                best = fmax(best, (double)teacher[j]);
-                m = fmax(m, (double)student[j] * inv_t);
-            }
-            const bool used = w != 0 && best > -INFINITY && (m > -INFINITY || nan);
-            double z = z_r > 0 ? z_r * exp(m_r - m) : 0;
-            for (int j = 0; j < k; ++j) {
-                const double p = cls[j] < 0 ? 0 : teacher[j] == best ? 1 : exp((teacher[j] - best) * inv_t);
-                p_sum += p;
-                teacher[j] = (float)p;
-                if (first[j]) z += exp(student[j] * inv_t - m);
-            }
-            if (rest) {
-                p_r = exp((double)rest[r]);
-                p_sum += p_r;
-                p_r /= p_sum;
-            }
-            double l = 0;
-            for (int j = 0; j < k; ++j) {
-                const double p = teacher[j] / p_sum;
-                teacher[j] = (float)p;
-                if (p > 0) l += p * (log(p) - (student[j] * inv_t - m - log(z)));
-            }
-            if (p_r > 0) l += p_r * (log(p_r) - (z_r > 0 ? log(z_r) + m_r - m - log(z) : -INFINITY));
-            row[0] = used;
-            row[1] = w * temperature;
-            row[2] = m;
-            row[3] = 1 / z;
-            row[4] = z_r > 0 ? w * temperature * (exp(m_r - m) / z - p_r / z_r) : 0;   // the row constant outside L
-            loss[r] = used ? (nan ? NAN : (float)(w * temperature * temperature * l)) : 0.0f;
-        }
-        __syncthreads();
-        if (!g) continue;
-        const bool used = row[0] != 0;
-        const float scale = (float)row[4];
-        for (int c = tid; c < n_classes; c += LSR_ROW_THREADS)
-            if (!used)
-                g[c] = (T)0.0f;
-            else if (nan)
-                g[c] = (T)NAN;
-            else if (!listed(c))
-                g[c] = (T)(high > -INFINITY ? scale * expf(((float)x[c] - high) * (float)inv_t) : 0.0f);
-        if (used && !nan && tid < k && first[tid]) {
-            double p = 0;
+    const int64_t r = blockIdx.x;
+    const T* mine = scores + r * row_stride;
+    Row row;
+    row.open(mine, n_classes);
+    for (int i = tid; i < MAP / 32; i += THREADS) map[i] = 0;
+    if (tid == 0) again = 0;
+    team_sync<W>();
+    for (int j = tid; j < k; j += THREADS) {
+        const int c = index[r * k + j];
+        const float v = values[r * k + j];
+        const bool there = c >= 0 && c < n_classes && v > -INFINITY;
+        cls[j] = there ? c : -1;
+        teacher[j] = there ? v : -INFINITY;
+        student[j] = there ? (float)mine[c] : -INFINITY;
+        first[j] = there;
+        if (there && (atomicOr(&map[(c & (MAP - 1)) >> 5], 1u << (c & 31)) >> (c & 31) & 1)) again = 1;
+    }
+    team_sync<W>();
+    if (again)                                            // a class, or in very long rows two that share a bit, came again
+        for (int j = tid; j < k; j += THREADS)
+            for (int i = 0; i < j; ++i)
+                if (cls[i] == cls[j]) first[j] = false;
+    // the runs of the row without the listed classes
+    auto blank = [&](int step, uint4& u) {
+        const int c = Row::first_class(step);
+        uint32_t b = map[(c & (MAP - 1)) >> 5] >> (c & 31) & ((1u << RUN) - 1);
+        if (b == 0) return;
+        if (n_classes > MAP) {                            // the bit may be another class's
+            uint32_t sure = 0;
             for (int j = 0; j < k; ++j)
-                if (cls[j] == cls[tid]) p += teacher[j];
-            g[cls[tid]] = (T)(float)(row[1] * (exp(student[tid] * inv_t - row[2]) * row[3] - p));
+                if (cls[j] >= c && cls[j] < c + RUN) sure |= 1u << (cls[j] - c);
+            b &= sure;
         }
+        uint32_t w[4] = {u.x, u.y, u.z, u.w};
+        const uint32_t none = Row::nothing().x;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (DT == ROW_F32)
+                w[i] = b >> i & 1 ? none : w[i];
+            else {
+                const uint32_t m = (b >> (2 * i) & 1 ? 0xffffu : 0u) | (b >> (2 * i) & 2 ? 0xffff0000u : 0u);
+                w[i] = (w[i] & ~m) | (none & m);
+            }
+        }
+        u = make_uint4(w[0], w[1], w[2], w[3]);
+    };
+    if (REST && N) {
+#pragma unroll
+        for (int i = 0; i < (N ? N : 1); ++i) blank(i, row.kept[i]);
+    }
+    auto each = [&](auto f) {
+        row.next_pass();
+        row.template each_run<4>([&](int step, uint4 u) {
+            if (REST && !N) blank(step, u);
+            float v[RUN];
+            Row::decode(u, v);
+            f(v, Row::first_class(step));
+        });
+    };
+    float high = -INFINITY;
+    each([&](const float(&v)[RUN], int) {
+#pragma unroll
+        for (int j = 0; j < RUN; ++j) high = row_max(high, v[j]);
+    });
+    const float m_r = team_max<W>(high, part_f);
+    const double inv_t = 1.0 / temperature, unit = inv_t * ROW_LOG2E;
+    const float unit_f = (float)unit, from = m_r > -INFINITY ? m_r : 0.0f;
+    float part = 0;
+    each([&](const float(&v)[RUN], int) {
+#pragma unroll
+        for (int j = 0; j < RUN; ++j) part += __builtin_amdgcn_exp2f((v[j] - from) * unit_f);
+    });
+    const double z_r = team_sum<W>((double)part, part_d);
+
+    if (tid < 64) {                                       // the list, in 64 bits
+        const double w = weight ? (double)weight[r] : 1.0;
+        float best = -INFINITY, m = m_r;
+        for (int j = tid; j < k; j += 64) {
+            best = row_max(best, teacher[j]);
+            if (REST) m = row_max(m, student[j]);
+        }
+        best = wave_max(best);
+        if (REST) m = wave_max(m);
+        double sum = 0, cross = 0, z_l = 0;
+        for (int j = tid; j < k; j += 64) {
+            if (cls[j] < 0) continue;
+            const double y = teacher[j] == best ? 0.0 : ((double)teacher[j] - best) * unit, z = ((double)student[j] - m) * unit;
+            const double p = row_exp2(y);
+            sum += p;
+            if (p > 0) cross += p * (y - z);
+            if (REST && first[j]) z_l += student[j] < INFINITY ? row_exp2(z) : NAN;
+            teacher[j] = (float)p;
+        }
+        sum = wave_sum(sum);
+        cross = wave_sum(cross) * (1.0 / ROW_LOG2E);
+        z_l = wave_sum(z_l);
+        // NaN or +infinity among the scores: their exponentials, and with them the sum, are NaN
+        const double shift = REST ? (z_r > 0 ? row_exp2(((double)m_r - m) * unit) : 0.0) : 1.0, z = z_l + (REST && z_r == 0 ? 0.0 : shift * z_r);
+        const bool nan = z != z || z_r != z_r, used = w != 0 && best > -INFINITY && (m > -INFINITY || nan);
+        double rest_log = 0, p_r = 0;
+        if (REST) {
+            rest_log = (double)rest[r];
+            p_r = row_exp2(rest_log * ROW_LOG2E);
+            sum += p_r;
+        }
+        const double ln = row_log(tid == 0 ? z : tid == 1 ? sum : z_r);
+        const double ln_z = __shfl(ln, 0), ln_s = __shfl(ln, 1), ln_r = __shfl(ln, 2);
+        if (tid == 0) {
+            double l = cross / sum + ln_z - ln_s;
+            if (REST && p_r > 0) l += p_r / sum * (z_r > 0 ? rest_log - ln_r - ((double)m_r - m) * inv_t : INFINITY);
+            loss[r] = used ? (nan ? NAN : (float)(w * temperature * temperature * l)) : 0.0f;
+            const double scale = w * temperature;
+            state = used ? (nan ? 2 : 1) : 0;
+            constant[0] = REST ? (z_r > 0 ? scale * (shift / z - p_r / sum / z_r) : 0.0) : scale / z;   // others
+            constant[1] = scale / z;                      // listed: student's part,
+            constant[2] = scale / sum;                    // teacher's part
+            constant[3] = (double)m;
+        }
+    }
+    if (!GRAD) return;
+    team_sync<W>();
+    T* g = grad + r * n_classes;
+    const int how = state;
+    const float scale = (float)constant[0];
+    each([&](const float(&v)[RUN], int c) {
+        struct __attribute__((packed, aligned(sizeof(T)))) { T e[RUN]; } out;
+#pragma unroll
+        for (int j = 0; j < RUN; ++j) {
+            const float d = scale * __builtin_amdgcn_exp2f((v[j] - from) * unit_f);
+            out.e[j] = (T)(how == 1 ? d : how ? NAN : 0.0f);
+        }
+        if (c + RUN <= n_classes) {
+            *(decltype(out)*)(g + c) = out;
+        } else {
+#pragma unroll
+            for (int j = 0; j < RUN; ++j)
+                if (c + j < n_classes) g[c + j] = out.e[j];
+        }
+    });
+    if (how != 1) return;
+    team_sync<W>();                                       // the listed classes are written after the pass over the row
+    for (int j = tid; j < k; j += THREADS) {
+        if (!first[j]) continue;
+        float p = teacher[j];
+        if (again) {
+            p = 0;
+            for (int i = 0; i < k; ++i) p += cls[i] == cls[j] ? teacher[i] : 0.0f;
+        }
+        g[cls[j]] = (T)(float)(constant[1] * row_exp2(((double)student[j] - constant[3]) * unit) - constant[2] * p);
     }
 }
 
@@ -218,10 +278,10 @@ __global__ __launch_bounds__(LSR_ROW_THREADS) void lsr_distill_quad_kernel(
     double p_r = 0, rest_log = 0;
     if (REST) {
         rest_log = (double)rest[r];
-        p_r = exp(rest_log);
+        p_r = row_exp2(rest_log * ROW_LOG2E);
         sum += p_r;
     }
-    const double ln = log(q == 0 ? z : q == 1 ? sum : (double)z_r);
+    const double ln = row_log(q == 0 ? z : q == 1 ? sum : (double)z_r);
     const double ln_z = quad_move<0x00>(ln), ln_s = quad_move<0x55>(ln), ln_r = quad_move<0xAA>(ln);
     if (live && q == 0) {
         double l = cross / sum + ln_z - ln_s;
@@ -263,6 +323,23 @@ static void lsr_distill_quad(hipStream_t stream, const void* scores_d, int64_t n
 #undef LAUNCH
 }
 
+template <int DT, int W, int N>
+static void lsr_distill_team(hipStream_t stream, const void* scores_d, int64_t n_rows, int n_classes, int64_t row_stride,
+                             const float* values_d, const int32_t* index_d, int k, const float* rest_d, double temperature,
+                             const float* weight_d, float* loss_d, void* grad_d) {
+    const auto* scores = (const typename row_type<DT>::type*)scores_d;
+    auto* grad = (typename row_type<DT>::type*)grad_d;
+#define LAUNCH(REST, GRAD)                                                                                                  \
+    hipLaunchKernelGGL((lsr_distill_team_kernel<DT, W, N, REST, GRAD>), dim3((unsigned)n_rows), dim3(64 * W), 0, stream,    \
+                       scores, n_classes, row_stride, values_d, index_d, k, rest_d, temperature, weight_d, loss_d, grad)
+    if (rest_d) {
+        if (grad_d) LAUNCH(true, true); else LAUNCH(true, false);
+    } else {
+        if (grad_d) LAUNCH(false, true); else LAUNCH(false, false);
+    }
+#undef LAUNCH
+}
+
 extern "C" int lsr_distill_scores(lsr_ctx* ctx, const void* scores_d, int dtype, int64_t n_rows, int64_t n_classes,
                                   int64_t row_stride, const float* top_values_d, const int32_t* top_index_d, int k,
                                   const float* rest_d, double temperature, const float* row_weight_d, float* loss_d,
@@ -279,7 +356,6 @@ extern "C" int lsr_distill_scores(lsr_ctx* ctx, const void* scores_d, int dtype,
     if ((uintptr_t)grad_d % row_dtype_bytes(dtype))
         return lsr_fail(ctx, LSR_ERR_ARG, "lsr_distill_scores: gradient is not aligned to its element size");
     LSR_HIP_CHECK(ctx, hipSetDevice(ctx->device));
-    const dim3 grid((unsigned)(n_rows < 65536 ? n_rows : 65536));
     lsr_prof_begin(ctx, LSR_K_DISTILL);
     if (n_classes <= LSR_QUAD_CLASSES) {
         LSR_DTYPE_SWITCH(dtype, LSR_QUAD_SWITCH(n_classes, lsr_distill_quad<DT, E>(ctx->stream, scores_d, n_rows, (int)n_classes,
@@ -290,19 +366,10 @@ extern "C" int lsr_distill_scores(lsr_ctx* ctx, const void* scores_d, int dtype,
         LSR_LAUNCH_CHECK(ctx, "lsr_distill_quad_kernel");
         return LSR_OK;
     }
-    if (dtype == LSR_F32)
-        hipLaunchKernelGGL(lsr_distill_kernel<ROW_F32>, grid, dim3(LSR_ROW_THREADS), 0, ctx->stream, (const float*)scores_d,
-                           n_rows, (int)n_classes, row_stride, top_values_d, top_index_d, k, rest_d, temperature, row_weight_d,
-                           loss_d, (float*)grad_d);
-    else if (dtype == LSR_F16)
-        hipLaunchKernelGGL(lsr_distill_kernel<ROW_F16>, grid, dim3(LSR_ROW_THREADS), 0, ctx->stream, (const _Float16*)scores_d,
-                           n_rows, (int)n_classes, row_stride, top_values_d, top_index_d, k, rest_d, temperature, row_weight_d,
-                           loss_d, (_Float16*)grad_d);
-    else
-        hipLaunchKernelGGL(lsr_distill_kernel<ROW_BF16>, grid, dim3(LSR_ROW_THREADS), 0, ctx->stream, (const __bf16*)scores_d,
-                           n_rows, (int)n_classes, row_stride, top_values_d, top_index_d, k, rest_d, temperature, row_weight_d,
-                           loss_d, (__bf16*)grad_d);
+    LSR_TEAM_SWITCH(dtype, n_classes, lsr_distill_team<DT, W, N>(ctx->stream, scores_d, n_rows, (int)n_classes, row_stride,
+                                                                 top_values_d, top_index_d, k, rest_d, temperature,
+                                                                 row_weight_d, loss_d, grad_d));
     lsr_prof_end(ctx);
-    LSR_LAUNCH_CHECK(ctx, "lsr_distill_kernel");
+    LSR_LAUNCH_CHECK(ctx, "lsr_distill_team_kernel");
     return LSR_OK;
 }

@@ -67,6 +67,29 @@ __device__ __forceinline__ double row_exp2(double y) {
     return __builtin_amdgcn_ldexp(p, (int)n);
 }
 #define ROW_LOG2E 1.4426950408889634
+// Natural logarithm of a positive number to 2^-49 of the result (or 2^-49 for numbers near 1): x = m 2^e with m in
+// [sqrt(1/2), sqrt(2)), ln m = 2 artanh(s) with s = (m - 1) / (m + 1), |s| < 0.172, by its series up to s^19 (the next term
+// is 2^-58).  The library's log needs several times the registers, which long rows do not have to spare.
+__device__ __forceinline__ double row_log(double x) {
+    double m = __builtin_amdgcn_frexp_mant(x);            // [1/2, 1)
+    int e = __builtin_amdgcn_frexp_exp(x);
+    if (m < 0.7071067811865476) {
+        m *= 2;
+        --e;
+    }
+    const double s = (m - 1) / (m + 1), q = s * s;
+    double p = 1.0 / 19;
+    p = __builtin_fma(p, q, 1.0 / 17);
+    p = __builtin_fma(p, q, 1.0 / 15);
+    p = __builtin_fma(p, q, 1.0 / 13);
+    p = __builtin_fma(p, q, 1.0 / 11);
+    p = __builtin_fma(p, q, 1.0 / 9);
+    p = __builtin_fma(p, q, 1.0 / 7);
+    p = __builtin_fma(p, q, 1.0 / 5);
+    p = __builtin_fma(p, q, 1.0 / 3);
+    p = __builtin_fma(p, q, 1.0);
+    return (double)e * 0.6931471805599453 + 2 * s * p;
+}
 
 // Weights of entries as whole numbers: w in [0, 1] in units of 2^-shift, so that sums do not depend on the order of
 // addition.  Adding 2^(52 - shift) leaves the rounded number in the low bits of the double.
@@ -263,4 +286,315 @@ template <int E> __device__ __forceinline__ void quad_sort_head(double (&e)[E]) 
         if ((dtype) == LSR_F32) { constexpr int DT = ROW_F32; __VA_ARGS__; }   \
         else if ((dtype) == LSR_F16) { constexpr int DT = ROW_F16; __VA_ARGS__; } \
         else { constexpr int DT = ROW_BF16; __VA_ARGS__; }                     \
+    } while (0)
+
+// ---- long rows: a team of W wavefronts holds a row ---------------------------------------------------------------------
+// Thread t of a team has the runs of 16 bytes t, t + 64 W, t + 128 W, ... of the row: N of them stay in registers from
+// the first read on (N = 0: the row is too long for that and every pass reads it again, mostly from L2).
+template <int CTRL, int ROWS> __device__ __forceinline__ int wave_shift(int v, int fill) {
+    return __builtin_amdgcn_update_dpp(fill, v, CTRL, ROWS, 0xf, false);
+}
+template <int CTRL, int ROWS> __device__ __forceinline__ float wave_shift(float v, float fill) {
+    return __int_as_float(wave_shift<CTRL, ROWS>(__float_as_int(v), __float_as_int(fill)));
+}
+template <int CTRL, int ROWS> __device__ __forceinline__ uint64_t wave_shift(uint64_t v, uint64_t fill) {
+    const uint32_t lo = wave_shift<CTRL, ROWS>((int)v, (int)fill), hi = wave_shift<CTRL, ROWS>((int)(v >> 32), (int)(fill >> 32));
+    return (uint64_t)hi << 32 | lo;
+}
+template <int CTRL, int ROWS> __device__ __forceinline__ double wave_shift(double v, double fill) {
+    return __longlong_as_double((long long)wave_shift<CTRL, ROWS>((uint64_t)__double_as_longlong(v), (uint64_t)__double_as_longlong(fill)));
+}
+// running combination over the lanes of a wavefront, in the same order every time; lane 63 has the whole
+#define WAVE_SCAN(v, fill, op)                             \
+    do {                                                   \
+        v = op(v, wave_shift<0x111, 0xf>(v, fill));        \
+        v = op(v, wave_shift<0x112, 0xf>(v, fill));        \
+        v = op(v, wave_shift<0x114, 0xf>(v, fill));        \
+        v = op(v, wave_shift<0x118, 0xf>(v, fill));        \
+        v = op(v, wave_shift<0x142, 0xa>(v, fill));        \
+        v = op(v, wave_shift<0x143, 0xc>(v, fill));        \
+    } while (0)
+template <typename V> __device__ __forceinline__ V row_add(V a, V b) { return a + b; }
+__device__ __forceinline__ uint64_t row_max(uint64_t a, uint64_t b) { return a > b ? a : b; }
+__device__ __forceinline__ int row_max(int a, int b) { return max(a, b); }
+
+__device__ __forceinline__ float wave_last(float v) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63)); }
+__device__ __forceinline__ int wave_last(int v) { return __builtin_amdgcn_readlane(v, 63); }
+__device__ __forceinline__ uint64_t wave_last(uint64_t v) {
+    const uint32_t lo = __builtin_amdgcn_readlane((int)v, 63), hi = __builtin_amdgcn_readlane((int)(v >> 32), 63);
+    return (uint64_t)hi << 32 | lo;
+}
+__device__ __forceinline__ double wave_last(double v) {
+    return __longlong_as_double((long long)wave_last((uint64_t)__double_as_longlong(v)));
+}
+template <typename V> __device__ __forceinline__ V wave_running(V v) {
+    WAVE_SCAN(v, (V)0, row_add);
+    return v;
+}
+template <typename V> __device__ __forceinline__ V wave_sum(V v) { return wave_last(wave_running(v)); }
+__device__ __forceinline__ float wave_max(float v) {
+    WAVE_SCAN(v, -INFINITY, row_max);
+    return wave_last(v);
+}
+__device__ __forceinline__ uint64_t wave_max(uint64_t v) {
+    WAVE_SCAN(v, (uint64_t)0, row_max);
+    return wave_last(v);
+}
+
+template <int W> __device__ __forceinline__ void team_sync() {
+    if (W == 1)
+        row_wave_fence();
+    else
+        __syncthreads();
+}
+// Sum / maximum over the team, returned to every thread; `shared` has W places and may be used again at once (two
+// barriers; one wavefront needs none).
+template <int W, typename V> __device__ __forceinline__ V team_sum(V v, V* shared) {
+    v = wave_sum(v);
+    if (W == 1) return v;
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) shared[threadIdx.x >> 6] = v;
+    __syncthreads();
+    V sum = shared[0];
+#pragma unroll
+    for (int i = 1; i < W; ++i) sum += shared[i];
+    return sum;
+}
+template <int W, typename V> __device__ __forceinline__ V team_max(V v, V* shared) {
+    v = wave_max(v);
+    if (W == 1) return v;
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) shared[threadIdx.x >> 6] = v;
+    __syncthreads();
+    V most = shared[0];
+#pragma unroll
+    for (int i = 1; i < W; ++i) most = row_max(most, shared[i]);
+    return most;
+}
+
+template <int DT, int W, int N> struct team_row {
+    using T = typename row_type<DT>::type;
+    static constexpr int RUN = 16 / (int)sizeof(T), THREADS = 64 * W, STEP = THREADS * RUN;   // classes of a run, of a step
+    struct __attribute__((packed, aligned(sizeof(T)))) run { uint32_t w[4]; };
+
+    const T* row;
+    int n_classes, steps;
+    uint4 kept[N ? N : 1];
+
+    static __device__ __forceinline__ uint4 nothing() {   // a run of -infinity
+        const uint32_t w = DT == ROW_F32 ? 0xff800000u : DT == ROW_F16 ? 0xfc00fc00u : 0xff80ff80u;
+        return make_uint4(w, w, w, w);
+    }
+    static __device__ __forceinline__ int first_class(int step) { return step * STEP + (int)threadIdx.x * RUN; }
+
+    // the run of the row's last classes, one element at a time
+    __device__ __forceinline__ uint4 read_end(int c) const {
+        uint32_t w[4] = {nothing().x, nothing().x, nothing().x, nothing().x};
+        for (int j = 0; j < RUN && c + j < n_classes; ++j) {
+            uint32_t b;
+            if constexpr (DT == ROW_F32)
+                b = __float_as_uint(row[c + j]);
+            else
+                b = __builtin_bit_cast(uint16_t, row[c + j]);
+#pragma unroll
+            for (int i = 0; i < RUN; ++i)
+                if (i == j) w[i * 4 / RUN] = RUN == 4 ? b : i & 1 ? (w[i * 4 / RUN] & 0xffffu) | b << 16 : (w[i * 4 / RUN] & 0xffff0000u) | b;
+        }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    __device__ __forceinline__ uint4 read(int step) const {
+        const int c = first_class(step);
+        if (c + RUN > n_classes) return nothing();
+        const run v = *(const run*)(row + c);
+        return make_uint4(v.w[0], v.w[1], v.w[2], v.w[3]);
+    }
+    __device__ __forceinline__ void open(const T* r, int classes) {
+        row = r;
+        n_classes = classes;
+        steps = (classes + STEP - 1) / STEP;
+        if (N) {
+#pragma unroll
+            for (int i = 0; i < (N ? N : 1); ++i) kept[i] = read(i);
+            const int end = first_class(steps - 1);
+            if (end < n_classes && end + RUN > n_classes) {
+                const uint4 u = read_end(end);
+#pragma unroll
+                for (int i = 0; i < (N ? N : 1); ++i)
+                    if (i == steps - 1) kept[i] = u;
+            }
+        }
+    }
+    // Between two passes: the compiler is to decode the runs again, not to keep every decoded value of the first pass in
+    // registers for the second (which would not fit and spill).
+    __device__ __forceinline__ void next_pass() {
+        if (N) {
+#pragma unroll
+            for (int i = 0; i < (N ? N : 1); ++i) asm volatile("" : "+v"(kept[i].x), "+v"(kept[i].y), "+v"(kept[i].z), "+v"(kept[i].w));
+        }
+    }
+    static __device__ __forceinline__ void decode(const uint4& u, float (&v)[RUN]) {
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+        if (DT == ROW_F32) {
+#pragma unroll
+            for (int i = 0; i < RUN; ++i) v[i] = __uint_as_float(w[i & 3]);
+        } else if (DT == ROW_BF16) {
+#pragma unroll
+            for (int i = 0; i < RUN; ++i) v[i] = __uint_as_float(i & 1 ? w[i >> 1 & 3] & 0xffff0000u : w[i >> 1 & 3] << 16);
+        } else {
+#pragma unroll
+            for (int i = 0; i < RUN; ++i)
+                v[i] = (float)__builtin_bit_cast(_Float16, (uint16_t)(i & 1 ? w[i >> 1 & 3] >> 16 : w[i >> 1 & 3]));
+        }
+    }
+    // f(step, run) for every step of the row; rows that are not kept are read `AHEAD` steps at a time, so that as many loads
+    // are on their way while a pass does little with each
+    template <int AHEAD, typename F> __device__ __forceinline__ void each_run(F f) {
+        if (N) {
+#pragma unroll
+            for (int i = 0; i < (N ? N : 1); ++i) f(i, kept[i]);
+        } else {
+            const int end = n_classes % RUN ? steps - 1 : steps;        // the last step may have the run that is cut short
+            int i = 0;
+            for (; i + AHEAD <= end; i += AHEAD) {
+                uint4 u[AHEAD];
+#pragma unroll
+                for (int j = 0; j < AHEAD; ++j) u[j] = read(i + j);
+#pragma unroll
+                for (int j = 0; j < AHEAD; ++j) f(i + j, u[j]);
+            }
+#pragma unroll 1
+            for (; i < steps; ++i) {
+                const int c = first_class(i);
+                uint4 u = c < n_classes && c + RUN > n_classes ? read_end(c) : read(i);
+                f(i, u);
+            }
+        }
+    }
+    // f(step, values of the thread's run, first class of the run)
+    template <int AHEAD, typename F> __device__ __forceinline__ void each(F f) {
+        each_run<AHEAD>([&](int i, const uint4& u) {
+            float v[RUN];
+            decode(u, v);
+            f(i, v, first_class(i));
+        });
+    }
+};
+
+// ---- the first entries of a long row ------------------------------------------------------------------------------------
+// The classes of a row are dealt out to ROW_GROUPS groups or fewer; the kk-th largest of the groups' best scores is a lower
+// bound of the row's kk-th largest score, as kk groups have a score that high.  One pass finds the groups' best, a
+// second collects what reaches the bound: for scores in no particular order about -G ln(1 - kk / G) entries of G = 256
+// groups, 73 for kk = 64.  Their places follow from counting, for each, the entries above it.
+#define ROW_GROUPS 256
+template <int W> struct team_list {
+    static constexpr int ROOM = W == 1 ? 1024 : 2048;
+    uint64_t entry[ROOM];
+    uint32_t group[ROW_GROUPS];
+    int n;
+    uint32_t bound;
+};
+
+// Collects the entries of every group whose best is among the kk best groups; the bound as a score, -FLT_MAX when all
+// present entries are collected.  `list.n` may exceed ROOM: then only some of them are there.
+template <int DT, int W, int N>
+__device__ __forceinline__ float team_collect(team_row<DT, W, N>& row, int kk, team_list<W>& list) {
+    using Row = team_row<DT, W, N>;
+    constexpr int THREADS = 64 * W, RUN = Row::RUN, PER = W == 1 ? 4 : 1;
+    const int tid = threadIdx.x;
+    float most[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) most[i] = -INFINITY;
+    row.template each<4>([&](int step, const float(&v)[RUN], int) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            if (W == 1 && step % PER != i) continue;
+#pragma unroll
+            for (int j = 0; j < RUN; ++j) most[i] = row_max(most[i], v[j]);
+        }
+    });
+    team_sync<W>();                                       // the list is free
+    if (tid == 0) {
+        list.n = 0;
+        list.bound = 0;
+    }
+    if (W == 1) {
+#pragma unroll
+        for (int i = 0; i < ROW_GROUPS / 64; ++i) list.group[i * 64 + tid] = i < PER ? row_key(most[i < PER ? i : 0]) : 0u;
+    } else if (W == 4) {
+        list.group[tid] = row_key(most[0]);
+    } else {
+        const float best = quad_max(most[0]);
+        if ((tid & 3) == 0) list.group[tid >> 2] = row_key(best);
+    }
+    team_sync<W>();
+    for (int g = tid; g < ROW_GROUPS; g += THREADS) {
+        const uint32_t own = list.group[g];
+        int above = 0, equal = 0;
+        for (int i = 0; i < ROW_GROUPS; i += 4) {
+            const uint4 o = *(const uint4*)&list.group[i];
+            above += (o.x > own) + (o.y > own) + (o.z > own) + (o.w > own);
+            equal += (o.x == own) + (o.y == own) + (o.z == own) + (o.w == own);
+        }
+        if (above < kk && kk <= above + equal) list.bound = own;
+    }
+    team_sync<W>();
+    const float bound = list.bound ? row_value(list.bound) : -3.402823466e38f;
+    row.next_pass();
+    row.template each<4>([&](int, const float(&v)[RUN], int c) {
+        bool any = false;
+#pragma unroll
+        for (int j = 0; j < RUN; ++j) any |= v[j] >= bound;
+        if (any) {
+#pragma unroll
+            for (int j = 0; j < RUN; ++j)
+                if (v[j] >= bound) {
+                    const int at = atomicAdd(&list.n, 1);
+                    if (at < team_list<W>::ROOM) list.entry[at] = row_entry(row_key(v[j]), c + j);
+                }
+        }
+    });
+    team_sync<W>();
+    return bound;
+}
+// how many of the list's first n entries are above e
+template <int W> __device__ __forceinline__ int team_above(const team_list<W>& list, int n, uint64_t e) {
+    int above = 0;
+    for (int i = 0; i < n; ++i) above += list.entry[i] > e;
+    return above;
+}
+
+// Wavefronts per row by the row's width.  KEPT: rows that fit stay in registers, the number of runs a thread keeps is the
+// second parameter.
+#define LSR_TEAM_SWITCH(dtype, classes, ...)                                                              \
+    do {                                                                                                  \
+        if ((dtype) == LSR_F32) {                                                                         \
+            constexpr int DT = ROW_F32;                                                                   \
+            if ((classes) <= 1024) { constexpr int W = 1, N = 4; __VA_ARGS__; }                           \
+            else if ((classes) <= 4096) { constexpr int W = 4, N = 4; __VA_ARGS__; }                      \
+            else if ((classes) <= 16384) { constexpr int W = 4, N = 16; __VA_ARGS__; }                    \
+            else if ((classes) <= 32768) { constexpr int W = 16, N = 8; __VA_ARGS__; }                    \
+            else if ((classes) <= 65536) { constexpr int W = 16, N = 16; __VA_ARGS__; }                   \
+            else { constexpr int W = 16, N = 0; __VA_ARGS__; }                                            \
+        } else if ((dtype) == LSR_F16) {                                                                  \
+            constexpr int DT = ROW_F16;                                                                   \
+            LSR_TEAM_SWITCH_16(classes, __VA_ARGS__);                                                     \
+        } else {                                                                                          \
+            constexpr int DT = ROW_BF16;                                                                  \
+            LSR_TEAM_SWITCH_16(classes, __VA_ARGS__);                                                     \
+        }                                                                                                 \
+    } while (0)
+#define LSR_TEAM_SWITCH_16(classes, ...)                                                                  \
+    do {                                                                                                  \
+        if ((classes) <= 1024) { constexpr int W = 1, N = 2; __VA_ARGS__; }                               \
+        else if ((classes) <= 4096) { constexpr int W = 4, N = 2; __VA_ARGS__; }                          \
+        else if ((classes) <= 16384) { constexpr int W = 4, N = 8; __VA_ARGS__; }                         \
+        else if ((classes) <= 65536) { constexpr int W = 16, N = 8; __VA_ARGS__; }                        \
+        else if ((classes) <= 131072) { constexpr int W = 16, N = 16; __VA_ARGS__; }                      \
+        else { constexpr int W = 16, N = 0; __VA_ARGS__; }                                                \
+    } while (0)
+#define LSR_WAVES_SWITCH(classes, ...)                                                                    \
+    do {                                                                                                  \
+        if ((classes) <= 1024) { constexpr int W = 1; __VA_ARGS__; }                                      \
+        else if ((classes) <= 16384) { constexpr int W = 4; __VA_ARGS__; }                                \
+        else { constexpr int W = 16; __VA_ARGS__; }                                                       \
     } while (0)

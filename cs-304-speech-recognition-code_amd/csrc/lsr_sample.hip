@@ -15,137 +15,387 @@ struct sample_args {
     double magic, unit;              // 2^(52 - shift), 2^-shift
 };
 
-template <int DT>
-__global__ __launch_bounds__(LSR_ROW_THREADS) void lsr_sample_kernel(const typename row_type<DT>::type* __restrict__ scores,
-                                                                     int64_t n_rows, int n_classes, int64_t row_stride,
-                                                                     const float* __restrict__ uniform, sample_args a,
-                                                                     int32_t* __restrict__ index, float* __restrict__ logprob) {
-    __shared__ unsigned long long hist[256];
-    __shared__ uint64_t wave_best[LSR_ROW_THREADS / 64];
-    __shared__ uint64_t threshold, left;
-    const int tid = threadIdx.x;
-    for (int64_t r = blockIdx.x; r < n_rows; r += gridDim.x) {
-        const typename row_type<DT>::type* x = scores + r * row_stride;
-        const double t = a.temperature_d ? (double)a.temperature_d[r] : a.temperature;
-        const double top_p = a.top_p_d ? (double)a.top_p_d[r] : a.top_p;
-        const double min_p = a.min_p_d ? (double)a.min_p_d[r] : a.min_p;
-        const int top_k = a.top_k_d ? a.top_k_d[r] : a.top_k;
+// the lowest score that min_p keeps: x >= best + t ln(min_p) in 64 bits, as the next 32-bit number
+__device__ __forceinline__ float sample_floor(float best, double t, double min_p) {
+    const double low = min_p < 1.0 ? (double)best + t * row_log(min_p) : (double)best;
+    const float f = (float)low;
+    return (double)f < low ? nextafterf(f, INFINITY) : f;
+}
+// the mass that top_p asks for: the first whole number that is not below its share of the sum, 1 at least
+__device__ __forceinline__ uint64_t sample_target(double top_p, uint64_t sum) {
+    if (!(top_p < 1.0)) return ~0ull;
+    const double share = ceil(top_p * (double)sum);
+    return share < 1.0 ? 1 : (uint64_t)share;
+}
+// the class sought is the first at which the running weight exceeds this
+__device__ __forceinline__ uint64_t sample_goal(float u, uint64_t sum) {
+    const double at = (double)u * (double)sum;
+    return !(at > 0) ? 0 : at >= (double)sum ? sum - 1 : (uint64_t)at;
+}
 
-        uint64_t best_e = 0;
-        for (int c = tid; c < n_classes; c += LSR_ROW_THREADS) {
-            const uint32_t key = row_key((float)x[c]);
-            const uint64_t e = row_entry(key, c);
-            if (key && e > best_e) best_e = e;
-        }
-        best_e = row_wave_max(best_e);
-        __syncthreads();                                  // the previous row is done with the shared variables
-        if ((tid & 63) == 0) wave_best[tid >> 6] = best_e;
-        __syncthreads();
-        for (int w = 0; w < LSR_ROW_THREADS / 64; ++w) best_e = wave_best[w] > best_e ? wave_best[w] : best_e;
-        if (best_e == 0 || !(t > 0)) {                    // nothing to draw from, or the best entry itself
-            if (tid == 0) {
-                index[r] = best_e ? (int32_t)~(uint32_t)best_e : -1;
-                logprob[r] = best_e ? 0.0f : -INFINITY;
-            }
-            continue;
-        }
-        const float best = row_value((uint32_t)(best_e >> 32));
-        const double inv_t = isinf(best) ? 1.0 : 1.0 / t;
-        uint64_t least = 1;
-        // mass of a class: 1 or its weight, 0 below the threshold
-        auto mass = [&](int c, bool count, uint64_t* e) -> uint64_t {
-            const float v = (float)x[c];
-            const uint32_t key = row_key(v);
-            *e = row_entry(key, c);
-            if (!key || *e < least) return 0;
-            return count ? 1 : row_fixed(v == best ? 1.0 : exp(((double)v - (double)best) * inv_t), a.magic);
-        };
-        auto total = [&]() -> uint64_t {
-            uint64_t sum = 0, e;
-            for (int c = tid; c < n_classes; c += LSR_ROW_THREADS) sum += mass(c, false, &e);
-            sum = row_wave_sum(sum);
-            __syncthreads();
-            if ((tid & 63) == 0) wave_best[tid >> 6] = sum;
-            __syncthreads();
-            return wave_best[0] + wave_best[1] + wave_best[2] + wave_best[3];
-        };
-        // the lowest entry of the shortest head whose mass is at least `target`
-        auto select = [&](uint64_t target, bool count) {
-            if (tid == 0) {
-                threshold = 0;
-                left = target;
-            }
-            for (int shift = 56; shift >= 0; shift -= 8) {
-                hist[tid] = 0;
-                __syncthreads();
-                const uint64_t high = threshold;
-                for (int c = tid; c < n_classes; c += LSR_ROW_THREADS) {
-                    uint64_t e;
-                    const uint64_t m = mass(c, count, &e);
-                    if (m && (shift == 56 || (e >> (shift + 8)) == (high >> (shift + 8))))
-                        atomicAdd(&hist[(e >> shift) & 255], (unsigned long long)m);
-                }
-                __syncthreads();
-                if (tid == 0) {
-                    uint64_t need = left;
-                    int d = 255;
-                    for (; d > 0 && hist[d] < need; --d) need -= hist[d];
-                    left = need;
-                    threshold = high | (uint64_t)d << shift;
-                }
-                __syncthreads();
-            }
-            if (threshold > least) least = threshold;
-            __syncthreads();
-        };
-        if (top_k > 0 && top_k < n_classes) select((uint64_t)top_k, true);
-        if (top_p < 1.0) {
-            double target = ceil((top_p > 0 ? top_p : 0.0) * (double)total());
-            select(target < 1.0 ? 1 : (uint64_t)target, false);
-        }
-        if (min_p > 0) {
-            const double low = (double)best + t * log(min_p < 1.0 ? min_p : 1.0);
-            float f = (float)low;
-            if ((double)f < low) f = nextafterf(f, INFINITY);
-            const uint64_t e = (uint64_t)row_key(f) << 32;
-            if (e > least) least = e;
-        }
-        const uint64_t sum = total();
-        double at = (double)uniform[r] * (double)sum;
-        if (!(at > 0)) at = 0;
-        uint64_t goal = at >= (double)sum ? sum - 1 : (uint64_t)at;
-        const bool count = goal == 0;                     // below half a unit: the first entry that is kept
-        if (tid == 0) {
-            threshold = 0;
-            left = goal;
-        }
-        for (int shift = 16; shift >= 0; shift -= 8) {
-            hist[tid] = 0;
-            __syncthreads();
-            const int high = (int)threshold;
-            for (int c = tid; c < n_classes; c += LSR_ROW_THREADS) {
+// A row in many passes over memory, by radix selection with weights: for rows that the fast form below does not take (an
+// infinite score, a cut that falls among thousands of scores that are alike).
+template <int DT, int W>
+__device__ __forceinline__ void sample_by_radix(const typename row_type<DT>::type* x, int n_classes, float best, double t,
+                                                int top_k, double top_p, double min_p, float u, const sample_args& a,
+                                                uint64_t* hist, uint64_t* shared, int32_t* index, float* logprob) {
+    constexpr int THREADS = 64 * W;
+    const int tid = threadIdx.x;
+    const double unit = isinf(best) ? 1.0 : ROW_LOG2E / t;
+    uint64_t least = 1;
+    // mass of a class: 1 or its weight, 0 below the threshold
+    auto mass = [&](int c, bool count, uint64_t* e) -> uint64_t {
+        const float v = (float)x[c];
+        const uint32_t key = row_key(v);
+        *e = row_entry(key, c);
+        if (!key || *e < least) return 0;
+        return count ? 1 : row_fixed(v == best ? 1.0 : row_exp2(((double)v - (double)best) * unit), a.magic);
+    };
+    auto total = [&]() -> uint64_t {
+        uint64_t sum = 0, e;
+        for (int c = tid; c < n_classes; c += THREADS) sum += mass(c, false, &e);
+        return team_sum<W>(sum, hist);
+    };
+    // the lowest entry of the shortest head whose mass is at least `left` (of thread 0)
+    auto select = [&](uint64_t left, bool count) {
+        uint64_t threshold = 0;
+        for (int shift = 56; shift >= 0; shift -= 8) {
+            team_sync<W>();
+            for (int i = tid; i < 256; i += THREADS) hist[i] = 0;
+            team_sync<W>();
+            for (int c = tid; c < n_classes; c += THREADS) {
                 uint64_t e;
-                if ((c >> (shift + 8)) != (high >> (shift + 8))) continue;
                 const uint64_t m = mass(c, count, &e);
-                if (m) atomicAdd(&hist[(c >> shift) & 255], (unsigned long long)m);
+                if (m && (shift == 56 || (e >> (shift + 8)) == (threshold >> (shift + 8))))
+                    atomicAdd((unsigned long long*)&hist[(e >> shift) & 255], (unsigned long long)m);
             }
-            __syncthreads();
+            team_sync<W>();
             if (tid == 0) {
-                uint64_t over = left;
-                int d = 0;
-                for (; d < 255 && hist[d] <= over; ++d) over -= hist[d];
-                left = over;
-                threshold = (uint64_t)(high | d << shift);
+                int d = 255;
+                for (; d > 0 && hist[d] < left; --d) left -= hist[d];
+                *shared = threshold | (uint64_t)d << shift;
             }
-            __syncthreads();
+            team_sync<W>();
+            threshold = *shared;
         }
+        if (threshold > least) least = threshold;
+    };
+    if (top_k > 0 && top_k < n_classes) select((uint64_t)top_k, true);
+    if (top_p < 1.0) {
+        const double target = ceil((top_p > 0 ? top_p : 0.0) * (double)total());
+        select(target < 1.0 ? 1 : (uint64_t)target, false);
+    }
+    if (min_p > 0) {
+        const uint64_t e = (uint64_t)row_key(sample_floor(best, t, min_p)) << 32;
+        if (e > least) least = e;
+    }
+    const uint64_t sum = total();
+    uint64_t left = sample_goal(u, sum);
+    const bool count = left == 0;                         // below one unit: the first entry that is kept
+    int at = 0;
+    for (int shift = 16; shift >= 0; shift -= 8) {
+        team_sync<W>();
+        for (int i = tid; i < 256; i += THREADS) hist[i] = 0;
+        team_sync<W>();
+        for (int c = tid; c < n_classes; c += THREADS) {
+            uint64_t e;
+            if ((c >> (shift + 8)) != (at >> (shift + 8))) continue;
+            const uint64_t m = mass(c, count, &e);
+            if (m) atomicAdd((unsigned long long*)&hist[(c >> shift) & 255], (unsigned long long)m);
+        }
+        team_sync<W>();
         if (tid == 0) {
-            const int c = (int)threshold;
-            const float v = (float)x[c];
-            index[r] = c;
-            logprob[r] = (float)((v == best ? 0.0 : ((double)v - (double)best) * inv_t) - log((double)sum * a.unit));
+            int d = 0;
+            for (; d < 255 && hist[d] <= left; ++d) left -= hist[d];
+            *shared = (uint64_t)(at | d << shift);
+        }
+        team_sync<W>();
+        at = (int)*shared;
+    }
+    if (tid == 0) {
+        const float v = (float)x[at];
+        *index = at;
+        *logprob = (float)((v == best ? 0.0 : ((double)v - (double)best) * unit * (1 / ROW_LOG2E)) - row_log((double)sum * a.unit));
+    }
+}
+
+// Long rows, a team of W wavefronts per row (lsr_rows.h).
+//
+// With a top_k of at most LSR_MAX_TOP, only the first entries are weighed: they are collected as lsr_top_scores does it,
+// put in order by counting, and everything else happens among them.
+//
+// Otherwise every class is weighed.  A cut by order is found from a histogram over the distance to the best score: the bin
+// in which the cut falls is collected and its entries counted against each other.  Then the weights of what is kept are
+// summed per step of the row, and the step, the run and the class that the uniform number falls on are looked up.
+template <int DT, int W>
+__global__ __launch_bounds__(64 * W) void lsr_sample_team_kernel(const typename row_type<DT>::type* __restrict__ scores,
+                                                                 int n_classes, int64_t row_stride,
+                                                                 const float* __restrict__ uniform, sample_args a,
+                                                                 int32_t* __restrict__ index, float* __restrict__ logprob) {
+    using Row = team_row<DT, W, 0>;
+    constexpr int THREADS = 64 * W, RUN = Row::RUN, ROOM = team_list<W>::ROOM;
+    constexpr int BINS = W == 1 ? 256 : W == 4 ? 1024 : 2048, OWN = BINS / THREADS;
+    constexpr int STEPS = (W == 1 ? 1024 : W == 4 ? 16384 : LSR_MAX_CLASSES) / Row::STEP;
+    __shared__ team_list<W> list;
+    __shared__ uint64_t mass[BINS > STEPS ? BINS : STEPS];          // of a bin, of a step, of an entry
+    __shared__ int bin_n[BINS];
+    __shared__ uint64_t sorted[LSR_MAX_TOP], part[W], above, lowest;
+    __shared__ float part_f[W];
+    __shared__ int cut_bin;
+    const int tid = threadIdx.x;
+    const int64_t r = blockIdx.x;
+    const auto* mine = scores + r * row_stride;
+    Row row;
+    row.open(mine, n_classes);
+    const double t = a.temperature_d ? (double)a.temperature_d[r] : a.temperature;
+    const double top_p = a.top_p_d ? (double)a.top_p_d[r] : a.top_p;
+    const double min_p = a.min_p_d ? (double)a.min_p_d[r] : a.min_p;
+    const int top_k = a.top_k_d ? a.top_k_d[r] : a.top_k;
+    const float u = uniform[r];
+    const double unit = ROW_LOG2E / t;
+
+    if (top_k > 0 && top_k <= LSR_MAX_TOP && top_k < n_classes && t > 0) {
+        team_collect<DT, W, 0>(row, top_k, list);
+        const int n = list.n;
+        if (n == 0) {
+            if (tid == 0) {
+                index[r] = -1;
+                logprob[r] = -INFINITY;
+            }
+            return;
+        }
+        if (n <= ROOM) {
+            for (int i = tid; i < n; i += THREADS) {
+                const uint64_t e = list.entry[i];
+                const int place = team_above(list, n, e);
+                if (place < LSR_MAX_TOP) sorted[place] = e;
+            }
+            team_sync<W>();
+            const int m = n < top_k ? n : top_k;
+            const float best = row_value((uint32_t)(sorted[0] >> 32));
+            if (best < INFINITY) {
+                for (int i = tid; i < m; i += THREADS)
+                    mass[i] = row_fixed(row_exp2(((double)row_value((uint32_t)(sorted[i] >> 32)) - best) * unit), a.magic);
+                team_sync<W>();
+                // how many of the ordered entries are kept: those of which the weight ahead is short of the target
+                uint64_t sum = 0;
+                for (int i = 0; i < m; ++i) sum += mass[i];
+                const uint64_t target = sample_target(top_p, sum);
+                const float floor = min_p > 0 ? sample_floor(best, t, min_p) : -INFINITY;
+                int n_kept = 0;
+                uint64_t run = 0, kept_sum = 0;
+                for (int i = 0; i < m; ++i) {
+                    const bool kept = (i == 0 || run < target) && row_value((uint32_t)(sorted[i] >> 32)) >= floor;
+                    run += mass[i];
+                    if (kept) {
+                        n_kept = i + 1;
+                        kept_sum = run;
+                    }
+                }
+                const uint64_t goal = sample_goal(u, kept_sum);
+                for (int i = tid; i < n_kept; i += THREADS) {
+                    // weight of the kept entries up to this class, in class order
+                    const uint32_t own = (uint32_t)sorted[i];
+                    uint64_t before = 0;
+                    int ahead = 0;
+                    for (int j = 0; j < n_kept; ++j)
+                        if ((uint32_t)sorted[j] > own) {  // complemented: a lower class
+                            before += mass[j];
+                            ++ahead;
+                        }
+                    if (goal == 0 ? ahead == 0 : before <= goal && goal < before + mass[i]) {
+                        const float v = row_value((uint32_t)(sorted[i] >> 32));
+                        index[r] = (int32_t)~own;
+                        logprob[r] = (float)(((double)v - best) / t - row_log((double)kept_sum * a.unit));
+                    }
+                }
+                return;
+            }
         }
     }
+
+    float most = -INFINITY;
+    row.template each<4>([&](int, const float(&v)[RUN], int) {
+#pragma unroll
+        for (int j = 0; j < RUN; ++j) most = row_max(most, v[j]);
+    });
+    const float best = team_max<W>(most, part_f);
+    if (best == -INFINITY || !(t > 0)) {                  // nothing to draw from, or the best entry itself
+        int at = 1 << 30;
+        row.template each<4>([&](int, const float(&v)[RUN], int c) {
+#pragma unroll
+            for (int j = 0; j < RUN; ++j)
+                if (v[j] == best) at = min(at, c + j);
+        });
+        at = (int)~(uint32_t)team_max<W>((uint64_t)(uint32_t)~at, part);
+        if (tid == 0) {
+            index[r] = best == -INFINITY ? -1 : at;
+            logprob[r] = best == -INFINITY ? -INFINITY : 0.0f;
+        }
+        return;
+    }
+    auto slowly = [&]() {
+        sample_by_radix<DT, W>(mine, n_classes, best, t, top_k, top_p, min_p, u, a, mass, &above, index + r, logprob + r);
+    };
+    if (best == INFINITY) return slowly();
+
+    float last = -INFINITY;                               // kept: above this score, or equal up to this class
+    int last_class = -1;
+    auto keeps = [&](float v, int c) { return v > last || (v == last && c <= last_class); };
+    auto weigh = [&](float v) { return row_fixed(row_exp2(((double)v - best) * unit), a.magic); };
+    const float per_bin = (float)fmin(BINS / 32 / t, 1e30);
+    auto bin_of = [&](float v) { return (int)fminf((best - v) * per_bin, (float)(BINS - 1)); };
+
+    // cuts the row where the mass of a head first reaches the target: by number of entries, then by weight
+    for (int by_weight = 0; by_weight < 2; ++by_weight) {
+        if (by_weight ? !(top_p < 1.0) : top_k <= 0 || top_k >= n_classes) continue;
+        team_sync<W>();
+        for (int i = tid; i < BINS; i += THREADS) {
+            mass[i] = 0;
+            bin_n[i] = 0;
+        }
+        if (tid == 0) {
+            list.n = 0;
+            lowest = ~0ull;
+        }
+        team_sync<W>();
+        row.template each<1>([&](int, const float(&v)[RUN], int c) {
+#pragma unroll
+            for (int j = 0; j < RUN; ++j)
+                if (keeps(v[j], c + j)) {
+                    const int b = bin_of(v[j]);
+                    atomicAdd(&bin_n[b], 1);
+                    if (by_weight) atomicAdd((unsigned long long*)&mass[b], (unsigned long long)weigh(v[j]));
+                }
+        });
+        team_sync<W>();
+        uint64_t own = 0;
+#pragma unroll
+        for (int i = 0; i < OWN; ++i) own += by_weight ? mass[tid * OWN + i] : (uint64_t)bin_n[tid * OWN + i];
+        uint64_t run = wave_running(own);
+        if ((tid & 63) == 63) part[tid >> 6] = run;
+        team_sync<W>();
+        uint64_t sum = 0;
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+            if (i < (tid >> 6)) run += part[i];
+            sum += part[i];
+        }
+        const uint64_t target = by_weight ? sample_target(top_p, sum) : (uint64_t)top_k;
+        if (target > sum) continue;                       // fewer entries than that: all are kept
+        run -= own;
+        if (run < target && target <= run + own) {
+#pragma unroll
+            for (int i = 0; i < OWN; ++i) {
+                const uint64_t m = by_weight ? mass[tid * OWN + i] : (uint64_t)bin_n[tid * OWN + i];
+                if (run < target && target <= run + m) {
+                    cut_bin = tid * OWN + i;
+                    above = run;
+                }
+                run += m;
+            }
+        }
+        team_sync<W>();
+        const int b = cut_bin;
+        const uint64_t ahead = above;
+        if (bin_n[b] > ROOM) return slowly();
+        row.template each<4>([&](int, const float(&v)[RUN], int c) {
+#pragma unroll
+            for (int j = 0; j < RUN; ++j)
+                if (keeps(v[j], c + j) && bin_of(v[j]) == b) list.entry[atomicAdd(&list.n, 1)] = row_entry(row_key(v[j]), c + j);
+        });
+        team_sync<W>();
+        const int n = list.n;
+        for (int i = tid; i < n; i += THREADS) {
+            const uint64_t e = list.entry[i];
+            uint64_t before = ahead;
+            for (int j = 0; j < n; ++j)
+                if (list.entry[j] > e) before += by_weight ? weigh(row_value((uint32_t)(list.entry[j] >> 32))) : 1;
+            if (before < target) atomicMin((unsigned long long*)&lowest, (unsigned long long)e);
+        }
+        team_sync<W>();
+        last = row_value((uint32_t)(lowest >> 32));
+        last_class = (int)~(uint32_t)lowest;
+    }
+    if (min_p > 0) {
+        const float floor = sample_floor(best, t, min_p);
+        if (floor > last) {
+            last = floor;
+            last_class = n_classes;
+        }
+    }
+    // weight of every step, and the step in which the goal lies
+    team_sync<W>();
+    for (int i = tid; i < row.steps; i += THREADS) mass[i] = 0;
+    team_sync<W>();
+    row.template each<1>([&](int step, const float(&v)[RUN], int c) {
+        uint64_t sum = 0;
+#pragma unroll
+        for (int j = 0; j < RUN; ++j)
+            if (keeps(v[j], c + j)) sum += weigh(v[j]);
+        sum = wave_sum(sum);
+        if ((tid & 63) == 0 && sum) atomicAdd((unsigned long long*)&mass[step], (unsigned long long)sum);
+    });
+    team_sync<W>();
+    uint64_t sum = 0;
+    for (int i = 0; i < row.steps; ++i) sum += mass[i];
+    const uint64_t goal = sample_goal(u, sum);
+    const double log_sum = row_log((double)sum * a.unit);
+    auto answer = [&](float v, int c) {
+        index[r] = c;
+        logprob[r] = (float)(((double)v - best) / t - log_sum);
+    };
+    if (goal == 0) {                                      // below one unit: the first entry that is kept
+        int at = 1 << 30;
+        row.template each<4>([&](int, const float(&v)[RUN], int c) {
+#pragma unroll
+            for (int j = 0; j < RUN; ++j)
+                if (keeps(v[j], c + j)) at = min(at, c + j);
+        });
+        at = (int)~(uint32_t)team_max<W>((uint64_t)(uint32_t)~at, part);
+        if (tid == 0) answer((float)mine[at], at);
+        return;
+    }
+    uint64_t run = 0;
+    int step = 0;
+    while (run + mass[step] <= goal) run += mass[step++];
+    {
+        const int c = Row::first_class(step);
+        float v[RUN];
+        Row::decode(c < n_classes && c + RUN > n_classes ? row.read_end(c) : row.read(step), v);
+        uint64_t own = 0;
+#pragma unroll
+        for (int j = 0; j < RUN; ++j)
+            if (keeps(v[j], c + j)) own += weigh(v[j]);
+        uint64_t before = wave_running(own);
+        if (W > 1) {
+            if ((tid & 63) == 63) part[tid >> 6] = before;
+            team_sync<W>();
+#pragma unroll
+            for (int k = 0; k < W; ++k)
+                if (k < (tid >> 6)) before += part[k];
+        }
+        before += run - own;
+        if (before <= goal && goal < before + own) {
+            bool found = false;
+#pragma unroll
+            for (int j = 0; j < RUN; ++j) {
+                const uint64_t m = keeps(v[j], c + j) ? weigh(v[j]) : 0;
+                if (!found && goal < before + m) {
+                    found = true;
+                    answer(v[j], c + j);
+                }
+                before += m;
+            }
+        }
+    }
+}
+
+template <int DT, int W>
+static void lsr_sample_team(hipStream_t stream, const void* scores_d, int64_t n_rows, int n_classes, int64_t row_stride,
+                            const float* uniform_d, const sample_args& a, int32_t* index_d, float* logprob_d) {
+    hipLaunchKernelGGL((lsr_sample_team_kernel<DT, W>), dim3((unsigned)n_rows), dim3(64 * W), 0, stream,
+                       (const typename row_type<DT>::type*)scores_d, n_classes, row_stride, uniform_d, a, index_d, logprob_d);
 }
 
 // Short rows (at most LSR_QUAD_CLASSES classes), a quad per row.  ORDER: some row is cut by its order, so the entries are
@@ -217,11 +467,9 @@ __global__ __launch_bounds__(LSR_ROW_THREADS) void lsr_sample_quad_kernel(const 
         }
     }
     if (min_p > 0) {
-        const double low = (double)best + t * log(min_p < 1.0 ? min_p : 1.0);
-        float f = (float)low;
-        if ((double)f < low) f = nextafterf(f, INFINITY);
-        if (f > last) {
-            last = f;
+        const float floor = sample_floor(best, t, min_p);
+        if (floor > last) {
+            last = floor;
             last_class = n_classes;
         }
     }
@@ -270,7 +518,7 @@ __global__ __launch_bounds__(LSR_ROW_THREADS) void lsr_sample_quad_kernel(const 
     float share = -INFINITY;
     if (!none && !greedy) {
         const float v = (float)scores[r * row_stride + at];
-        share = (float)((isinf(v) ? 0.0 : ((double)v - best) / t) - log(total));
+        share = (float)((isinf(v) ? 0.0 : ((double)v - best) / t) - row_log(total));
     }
     logprob[r] = !none && greedy ? 0.0f : share;
 }
@@ -306,7 +554,6 @@ extern "C" int lsr_sample_scores(lsr_ctx* ctx, const void* scores_d, int dtype, 
     if (shift > 52) shift = 52;
     sample_args a = {temperature, top_p,  min_p, top_k, temperature_d, top_p_d, min_p_d, top_k_d, ldexp(1.0, 52 - shift),
                      ldexp(1.0, -shift)};
-    const dim3 grid((unsigned)(n_rows < 65536 ? n_rows : 65536));
     const bool order = top_k_d || top_p_d || (top_k > 0 && top_k < n_classes) || top_p < 1;
     lsr_prof_begin(ctx, LSR_K_SAMPLE);
     if (n_classes <= LSR_QUAD_CLASSES) {
@@ -317,16 +564,9 @@ extern "C" int lsr_sample_scores(lsr_ctx* ctx, const void* scores_d, int dtype, 
         LSR_LAUNCH_CHECK(ctx, "lsr_sample_quad_kernel");
         return LSR_OK;
     }
-    if (dtype == LSR_F32)
-        hipLaunchKernelGGL(lsr_sample_kernel<ROW_F32>, grid, dim3(LSR_ROW_THREADS), 0, ctx->stream, (const float*)scores_d,
-                           n_rows, (int)n_classes, row_stride, uniform_d, a, index_d, logprob_d);
-    else if (dtype == LSR_F16)
-        hipLaunchKernelGGL(lsr_sample_kernel<ROW_F16>, grid, dim3(LSR_ROW_THREADS), 0, ctx->stream, (const _Float16*)scores_d,
-                           n_rows, (int)n_classes, row_stride, uniform_d, a, index_d, logprob_d);
-    else
-        hipLaunchKernelGGL(lsr_sample_kernel<ROW_BF16>, grid, dim3(LSR_ROW_THREADS), 0, ctx->stream, (const __bf16*)scores_d,
-                           n_rows, (int)n_classes, row_stride, uniform_d, a, index_d, logprob_d);
+    LSR_DTYPE_SWITCH(dtype, LSR_WAVES_SWITCH(n_classes, lsr_sample_team<DT, W>(ctx->stream, scores_d, n_rows, (int)n_classes,
+                                                                               row_stride, uniform_d, a, index_d, logprob_d)));
     lsr_prof_end(ctx);
-    LSR_LAUNCH_CHECK(ctx, "lsr_sample_kernel");
+    LSR_LAUNCH_CHECK(ctx, "lsr_sample_team_kernel");
     return LSR_OK;
 }

@@ -1,7 +1,4 @@
 // The k best classes of every row of log scores, and the log weight of the rest.
-//
-// Radix selection: the threshold of the first k entries (lsr_rows.h) is found eight bits at a time from a histogram of
-// the entries that still match it; the entries at or above it go to a list in LDS, which is sorted and written.
 #include <math.h>
 
 #include "lsr_rows.h"
@@ -19,101 +16,139 @@ int lsr_check_rows(lsr_ctx* ctx, const char* name, const void* scores_d, int dty
     return LSR_OK;
 }
 
-template <int DT>
-__global__ __launch_bounds__(LSR_ROW_THREADS) void lsr_top_kernel(const typename row_type<DT>::type* __restrict__ scores,
-                                                                  int64_t n_rows, int n_classes, int64_t row_stride, int k,
-                                                                  float inv_t, float* __restrict__ values,
-                                                                  int32_t* __restrict__ index, float* __restrict__ rest) {
-    __shared__ int hist[256];
-    __shared__ uint64_t list[LSR_MAX_TOP];
-    __shared__ uint64_t threshold;
-    __shared__ int left, n_list;
-    __shared__ float part[LSR_ROW_THREADS / 64];
+// The lowest of the row's first `want` entries by radix selection, eight bits at a time from a histogram of the entries
+// that still match; what the group bound cannot narrow down (tens of thousands of equal scores) comes here.
+template <int DT, int W>
+__device__ __forceinline__ uint64_t top_radix(const typename row_type<DT>::type* x, int n_classes, int want, int* hist,
+                                              uint64_t* shared) {
+    constexpr int THREADS = 64 * W;
     const int tid = threadIdx.x;
-    for (int64_t r = blockIdx.x; r < n_rows; r += gridDim.x) {
-        const typename row_type<DT>::type* x = scores + r * row_stride;
-        if (tid == 0) {
-            threshold = 0;
-            left = k;
-            n_list = 0;
-        }
-        for (int shift = 56; shift >= 0; shift -= 8) {
-            hist[tid] = 0;
-            __syncthreads();
-            const uint64_t high = threshold;
-            for (int c = tid; c < n_classes; c += LSR_ROW_THREADS) {
-                const uint32_t key = row_key((float)x[c]);
-                const uint64_t e = row_entry(key, c);
-                if (key && (shift == 56 || (e >> (shift + 8)) == (high >> (shift + 8))))
-                    atomicAdd(&hist[(e >> shift) & 255], 1);
-            }
-            __syncthreads();
-            if (tid == 0) {
-                int need = left, d = 255;
-                for (; d > 0 && hist[d] < need; --d) need -= hist[d];
-                left = need;
-                threshold = high | (uint64_t)d << shift;
-            }
-            __syncthreads();
-        }
-        const uint64_t least = threshold;
-        list[tid] = 0;
-        __syncthreads();
-        for (int c = tid; c < n_classes; c += LSR_ROW_THREADS) {
+    int left = want;                                      // of thread 0
+    uint64_t threshold = 0;
+    for (int shift = 56; shift >= 0; shift -= 8) {
+        for (int i = tid; i < 256; i += THREADS) hist[i] = 0;
+        team_sync<W>();
+        for (int c = tid; c < n_classes; c += THREADS) {
             const uint32_t key = row_key((float)x[c]);
             const uint64_t e = row_entry(key, c);
-            if (key && e >= least) {
-                const int at = atomicAdd(&n_list, 1);
-                if (at < LSR_MAX_TOP) list[at] = e;
-            }
+            if (key && (shift == 56 || (e >> (shift + 8)) == (threshold >> (shift + 8)))) atomicAdd(&hist[(e >> shift) & 255], 1);
         }
-        __syncthreads();
-        for (int size = 2; size <= LSR_MAX_TOP; size <<= 1)
-            for (int step = size >> 1; step; step >>= 1) {
-                const int other = tid ^ step;
-                if (other > tid) {
-                    const uint64_t a = list[tid], b = list[other];
-                    if (((tid & size) == 0) == (a < b)) {
-                        list[tid] = b;
-                        list[other] = a;
-                    }
-                }
-                __syncthreads();
-            }
-        if (tid < k) {
-            const uint64_t e = list[tid];
-            values[r * k + tid] = e ? row_value((uint32_t)(e >> 32)) : -INFINITY;
-            index[r * k + tid] = e ? (int32_t)~(uint32_t)e : -1;
+        team_sync<W>();
+        if (tid == 0) {
+            int d = 255;
+            for (; d > 0 && hist[d] < left; --d) left -= hist[d];
+            *shared = threshold | (uint64_t)d << shift;
         }
-        if (rest) {
-            // relative to the highest score of the rest: relative to the row's best it could underflow to nothing
-            const float best = list[0] ? row_value((uint32_t)(list[0] >> 32)) : 0.0f;
-            float high = -INFINITY;
-            for (int c = tid; c < n_classes; c += LSR_ROW_THREADS) {
-                const float v = (float)x[c];
-                const uint32_t key = row_key(v);
-                if (key && row_entry(key, c) < least) high = fmaxf(high, v);
-            }
-            for (int d = 32; d; d >>= 1) high = fmaxf(high, __shfl_xor(high, d));
-            if ((tid & 63) == 0) part[tid >> 6] = high;
-            __syncthreads();
-            high = fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
-            __syncthreads();
-            float sum = 0.0f;
-            for (int c = tid; c < n_classes; c += LSR_ROW_THREADS) {
-                const float v = (float)x[c];
-                const uint32_t key = row_key(v);
-                if (key && row_entry(key, c) < least) sum += v == high ? 1.0f : expf((v - high) * inv_t);
-            }
-            sum = row_wave_sum(sum);
-            if ((tid & 63) == 0) part[tid >> 6] = sum;
-            __syncthreads();
-            if (tid == 0)
-                rest[r] = high > -INFINITY ? (high == best ? 0.0f : (high - best) * inv_t) + logf(part[0] + part[1] + part[2] + part[3])
-                                           : -INFINITY;
-        }
-        __syncthreads();
+        team_sync<W>();
+        threshold = *shared;
     }
+    return threshold;
+}
+
+// Long rows, a team of W wavefronts per row (lsr_rows.h).
+template <int DT, int W, int N, bool REST>
+__global__ __launch_bounds__(64 * W) void lsr_top_team_kernel(const typename row_type<DT>::type* __restrict__ scores,
+                                                              int n_classes, int64_t row_stride, int k, float inv_t,
+                                                              float* __restrict__ values, int32_t* __restrict__ index,
+                                                              float* __restrict__ rest) {
+    using Row = team_row<DT, W, N>;
+    constexpr int THREADS = 64 * W, RUN = Row::RUN, ROOM = team_list<W>::ROOM;
+    __shared__ team_list<W> list;
+    __shared__ int hist[256];
+    __shared__ uint64_t one;
+    __shared__ float part[W], best, high;
+    const int tid = threadIdx.x;
+    const int64_t r = blockIdx.x;
+    const int kk = k + (REST ? 1 : 0);                    // the first entry of the rest as well
+    Row row;
+    row.open(scores + r * row_stride, n_classes);
+    float bound = team_collect<DT, W, N>(row, kk, list);
+    int n = list.n, bound_class = -1;                     // collected: above the bound, or equal up to this class
+    bool equal = true;                                    // every score that equals the bound is collected
+    if (n > ROOM) {
+        const uint64_t least = top_radix<DT, W>(scores + r * row_stride, n_classes, kk, hist, &one);
+        bound = row_value((uint32_t)(least >> 32));
+        bound_class = (int)~(uint32_t)least;
+        equal = false;
+        if (tid == 0) list.n = 0;
+        team_sync<W>();
+        row.next_pass();
+        row.template each<4>([&](int, const float(&v)[RUN], int c) {
+#pragma unroll
+            for (int j = 0; j < RUN; ++j)
+                if (v[j] > bound || (v[j] == bound && c + j <= bound_class)) list.entry[atomicAdd(&list.n, 1)] = row_entry(row_key(v[j]), c + j);
+        });
+        team_sync<W>();
+        n = list.n;
+    }
+    float sum = 0.0f;
+    if (tid == 0) {
+        best = 0.0f;
+        high = -INFINITY;
+    }
+    team_sync<W>();
+    int place[ROOM / THREADS];
+#pragma unroll
+    for (int i = 0; i < ROOM / THREADS; ++i) {
+        const int at = i * THREADS + tid;
+        place[i] = 1 << 30;
+        if (at >= n) continue;
+        const uint64_t e = list.entry[at];
+        const float v = row_value((uint32_t)(e >> 32));
+        place[i] = team_above(list, n, e);
+        if (place[i] < k) {
+            values[r * k + place[i]] = v;
+            index[r * k + place[i]] = (int32_t)~(uint32_t)e;
+        }
+        if (REST && place[i] == 0) best = v;
+        if (REST && place[i] == k) high = v;
+    }
+    for (int i = n + tid; i < k; i += THREADS) {          // places without an entry
+        values[r * k + i] = -INFINITY;
+        index[r * k + i] = -1;
+    }
+    if (!REST) return;
+    team_sync<W>();
+    // relative to the highest score of the rest: relative to the row's best it could underflow to nothing
+    const float from = high, unit = inv_t * 1.44269504f;
+#pragma unroll
+    for (int i = 0; i < ROOM / THREADS; ++i) {
+        const int at = i * THREADS + tid;
+        if (at >= n || place[i] < k) continue;
+        const float v = row_value((uint32_t)(list.entry[at] >> 32));
+        sum += v == from ? 1.0f : __builtin_amdgcn_exp2f((v - from) * unit);
+    }
+    if (from > -INFINITY) {
+        row.next_pass();
+        if (equal) {
+            row.template each<4>([&](int, const float(&v)[RUN], int) {
+#pragma unroll
+                for (int j = 0; j < RUN; ++j) sum += v[j] < bound ? __builtin_amdgcn_exp2f((v[j] - from) * unit) : 0.0f;
+            });
+        } else {
+            row.template each<4>([&](int, const float(&v)[RUN], int c) {
+#pragma unroll
+                for (int j = 0; j < RUN; ++j)
+                    if (v[j] < bound || (v[j] == bound && c + j > bound_class))
+                        sum += v[j] == from ? 1.0f : __builtin_amdgcn_exp2f((v[j] - from) * unit);
+            });
+        }
+    }
+    sum = team_sum<W>(sum, part);
+    if (tid == 0) rest[r] = from > -INFINITY ? (from == best ? 0.0f : (from - best) * inv_t) + logf(sum) : -INFINITY;
+}
+
+template <int DT, int W, int N>
+static void lsr_top_team(hipStream_t stream, const void* scores_d, int64_t n_rows, int n_classes, int64_t row_stride, int k,
+                         float inv_t, float* values_d, int32_t* index_d, float* rest_d) {
+    const auto* scores = (const typename row_type<DT>::type*)scores_d;
+    const dim3 grid((unsigned)n_rows), block(64 * W);
+    if (rest_d)
+        hipLaunchKernelGGL((lsr_top_team_kernel<DT, W, N, true>), grid, block, 0, stream, scores, n_classes, row_stride, k,
+                           inv_t, values_d, index_d, rest_d);
+    else
+        hipLaunchKernelGGL((lsr_top_team_kernel<DT, W, N, false>), grid, block, 0, stream, scores, n_classes, row_stride, k,
+                           inv_t, values_d, index_d, rest_d);
 }
 
 // Short rows (at most LSR_QUAD_CLASSES classes), a quad per row: the entries are sorted by a network over the quad's
@@ -206,7 +241,6 @@ extern "C" int lsr_top_scores(lsr_ctx* ctx, const void* scores_d, int dtype, int
     if (n_rows == 0) return LSR_OK;
     if (!values_d || !index_d) return lsr_fail(ctx, LSR_ERR_ARG, "lsr_top_scores: null pointer");
     LSR_HIP_CHECK(ctx, hipSetDevice(ctx->device));
-    const dim3 grid((unsigned)(n_rows < 65536 ? n_rows : 65536));
     const float inv_t = (float)(1.0 / temperature);
     lsr_prof_begin(ctx, LSR_K_TOP);
     if (n_classes <= LSR_QUAD_CLASSES) {
@@ -216,16 +250,9 @@ extern "C" int lsr_top_scores(lsr_ctx* ctx, const void* scores_d, int dtype, int
         LSR_LAUNCH_CHECK(ctx, "lsr_top_quad_kernel");
         return LSR_OK;
     }
-    if (dtype == LSR_F32)
-        hipLaunchKernelGGL(lsr_top_kernel<ROW_F32>, grid, dim3(LSR_ROW_THREADS), 0, ctx->stream, (const float*)scores_d,
-                           n_rows, (int)n_classes, row_stride, k, inv_t, values_d, index_d, rest_d);
-    else if (dtype == LSR_F16)
-        hipLaunchKernelGGL(lsr_top_kernel<ROW_F16>, grid, dim3(LSR_ROW_THREADS), 0, ctx->stream, (const _Float16*)scores_d,
-                           n_rows, (int)n_classes, row_stride, k, inv_t, values_d, index_d, rest_d);
-    else
-        hipLaunchKernelGGL(lsr_top_kernel<ROW_BF16>, grid, dim3(LSR_ROW_THREADS), 0, ctx->stream, (const __bf16*)scores_d,
-                           n_rows, (int)n_classes, row_stride, k, inv_t, values_d, index_d, rest_d);
+    LSR_TEAM_SWITCH(dtype, n_classes, lsr_top_team<DT, W, N>(ctx->stream, scores_d, n_rows, (int)n_classes, row_stride, k, inv_t,
+                                                             values_d, index_d, rest_d));
     lsr_prof_end(ctx);
-    LSR_LAUNCH_CHECK(ctx, "lsr_top_kernel");
+    LSR_LAUNCH_CHECK(ctx, "lsr_top_team_kernel");
     return LSR_OK;
 }

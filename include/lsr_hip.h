@@ -413,7 +413,7 @@ int lsr_sample_scores(lsr_ctx* ctx, const void* scores_d, int dtype, int64_t n_r
  * grad_d (elements of `dtype`, rows of n_classes back to back, must not overlap the scores; may be NULL) is the gradient of
  * the sum of the losses.  Loss and gradient are exactly 0 for a row whose weight is 0, whose teacher has no entry or whose
  * scores are all -infinity, and NaN for any other row with a NaN or +infinity among its scores.  k = 1 with temperature 1
- * and no rest is the cross entropy with a class label. */
+ * and no rest is the cross entropy with a class label.  A rest of -infinity or NaN has no weight. */
 int lsr_distill_scores(lsr_ctx* ctx, const void* scores_d, int dtype, int64_t n_rows, int64_t n_classes, int64_t row_stride,
                        const float* top_values_d, const int32_t* top_index_d, int k, const float* rest_d, double temperature,
                        const float* row_weight_d, float* loss_d, void* grad_d);
