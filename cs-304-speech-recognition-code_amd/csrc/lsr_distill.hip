@@ -11,7 +11,7 @@
 
 #include "lsr_rows.h"
 
-// Long rows, a team of W wavefronts per row (lsr_rows.h).  Wavefront 0 handles the list while the row is on its way; the
+// Long rows, a team of W wavefronts per row (lsr_rows.h).  Wavefront 0 handles the list while the row is on its way.  The
 // listed classes are marked in a bit map, and where there is an outcome for the rest they are blanked in the registers, so
 // that maximum, sum and gradient run over the others alone.  The gradient of the listed classes is written over afterwards.
 template <int DT, int W, int N, bool REST, bool GRAD>
@@ -28,32 +28,82 @@ __global__ __launch_bounds__(64 * W) void lsr_distill_team_kernel(
     __shared__ float teacher[LSR_MAX_TOP];                // values, then weights relative to the best
     __shared__ float student[LSR_MAX_TOP];                // scores of the listed classes
     __shared__ bool first[LSR_MAX_TOP];                   // the class has not been listed before
-    __shared__ float part_f[W];
-    __shared__ double part_d[W], constant[5];
-    __shared__ int again, state;
+    __shared__ float part_f[W], list_best, list_high;
+    __shared__ double part_d[W], list_sum, list_cross, list_z;
+    __shared__ int again;
     const int tid = threadIdx.x;
     const int64_t r = blockIdx.x;
     const T* mine = scores + r * row_stride;
     Row row;
+    // The list is requested before the row: loads are waited for in order, and the list's part below is to run while the
+    // row is still on its way.
+    constexpr int PER = THREADS < LSR_MAX_TOP ? LSR_MAX_TOP / THREADS : 1;
+    int c[PER];
+    float tv[PER];
+    T sv[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const int j = i * THREADS + tid;
+        c[i] = j < k ? index[r * k + j] : -1;
+        tv[i] = j < k ? values[r * k + j] : -INFINITY;
+        if (!(c[i] >= 0 && c[i] < n_classes && tv[i] > -INFINITY)) c[i] = -1;
+        sv[i] = mine[c[i] < 0 ? 0 : c[i]];
+    }
     row.open(mine, n_classes);
     for (int i = tid; i < MAP / 32; i += THREADS) map[i] = 0;
     if (tid == 0) again = 0;
     team_sync<W>();
-    for (int j = tid; j < k; j += THREADS) {
-        const int c = index[r * k + j];
-        const float v = values[r * k + j];
-        const bool there = c >= 0 && c < n_classes && v > -INFINITY;
-        cls[j] = there ? c : -1;
-        teacher[j] = there ? v : -INFINITY;
-        student[j] = there ? (float)mine[c] : -INFINITY;
-        first[j] = there;
-        if (there && (atomicOr(&map[(c & (MAP - 1)) >> 5], 1u << (c & 31)) >> (c & 31) & 1)) again = 1;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const int j = i * THREADS + tid;
+        if (j >= k) continue;
+        cls[j] = c[i];
+        teacher[j] = c[i] < 0 ? -INFINITY : tv[i];
+        student[j] = c[i] < 0 ? -INFINITY : (float)sv[i];
+        first[j] = c[i] >= 0;
+        if (c[i] >= 0 && (atomicOr(&map[(c[i] & (MAP - 1)) >> 5], 1u << (c[i] & 31)) >> (c[i] & 31) & 1)) again = 1;
     }
     team_sync<W>();
-    if (again)                                            // a class, or in very long rows two that share a bit, came again
-        for (int j = tid; j < k; j += THREADS)
-            for (int i = 0; i < j; ++i)
-                if (cls[i] == cls[j]) first[j] = false;
+    const double inv_t = 1.0 / temperature, unit = inv_t * ROW_LOG2E;
+    if (tid < 64) {                                       // the list, in 64 bits, while the row is on its way
+        if (again)                                        // a class, or in very long rows two that share a bit, came again
+#pragma unroll 1
+            for (int j = tid; j < k; j += 64)
+#pragma unroll 1
+                for (int i = 0; i < j; ++i)
+                    if (cls[i] == cls[j]) first[j] = false;
+        float best = -INFINITY, high = -INFINITY;
+#pragma unroll 1
+        for (int j = tid; j < k; j += 64) {
+            best = row_max(best, teacher[j]);
+            high = row_max(high, student[j]);
+        }
+        best = wave_max(best);
+        high = wave_max(high);
+        // sum of the teacher's weights e^y, of e^y (y - z), of the student's e^z; z relative to the list's highest score
+        double sum = 0, cross = 0, z_l = 0;
+#pragma unroll 1
+        for (int j = tid; j < k; j += 64) {
+            if (cls[j] < 0) continue;
+            const double y = teacher[j] == best ? 0.0 : ((double)teacher[j] - best) * unit;
+            const double z = ((double)student[j] - (high > -INFINITY ? high : 0.0f)) * unit, p = row_exp2(y);
+            sum += p;
+            if (p > 0) cross += p * (y - z);
+            if (REST && first[j]) z_l += student[j] < INFINITY ? row_exp2(z) : NAN;
+            teacher[j] = (float)p;
+        }
+        sum = wave_sum(sum);
+        cross = wave_sum(cross);
+        if (REST) z_l = wave_sum(z_l);
+        if (tid == 0) {
+            list_best = best;
+            list_high = high;
+            list_sum = sum;
+            list_cross = cross * (1.0 / ROW_LOG2E);
+            list_z = z_l;
+        }
+    }
+    row.arrive();
     // the runs of the row without the listed classes
     auto blank = [&](int step, uint4& u) {
         const int c = Row::first_class(step);
@@ -61,6 +111,7 @@ __global__ __launch_bounds__(64 * W) void lsr_distill_team_kernel(
         if (b == 0) return;
         if (n_classes > MAP) {                            // the bit may be another class's
             uint32_t sure = 0;
+#pragma unroll 1
             for (int j = 0; j < k; ++j)
                 if (cls[j] >= c && cls[j] < c + RUN) sure |= 1u << (cls[j] - c);
             b &= sure;
@@ -97,7 +148,6 @@ __global__ __launch_bounds__(64 * W) void lsr_distill_team_kernel(
         for (int j = 0; j < RUN; ++j) high = row_max(high, v[j]);
     });
     const float m_r = team_max<W>(high, part_f);
-    const double inv_t = 1.0 / temperature, unit = inv_t * ROW_LOG2E;
     const float unit_f = (float)unit, from = m_r > -INFINITY ? m_r : 0.0f;
     float part = 0;
     each([&](const float(&v)[RUN], int) {
@@ -106,62 +156,36 @@ __global__ __launch_bounds__(64 * W) void lsr_distill_team_kernel(
     });
     const double z_r = team_sum<W>((double)part, part_d);
 
-    if (tid < 64) {                                       // the list, in 64 bits
-        const double w = weight ? (double)weight[r] : 1.0;
-        float best = -INFINITY, m = m_r;
-        for (int j = tid; j < k; j += 64) {
-            best = row_max(best, teacher[j]);
-            if (REST) m = row_max(m, student[j]);
+    // every thread for itself: no barrier between the sum and the gradient
+    const double w = weight ? (double)weight[r] : 1.0, rest_log = REST ? (double)rest[r] : 0.0;
+    const float high_l = list_high, m = REST ? row_max(m_r, high_l) : m_r;
+    // NaN or +infinity among the scores: their exponentials, and with them the sum, are NaN
+    const double shift = !REST ? 1.0 : z_r == 0 ? 0.0 : row_exp2(((double)m_r - m) * unit);
+    const double shift_l = high_l > -INFINITY ? row_exp2(((double)high_l - m) * unit) : 1.0;
+    const double z = (REST ? shift_l * list_z : 0.0) + (z_r == 0 ? 0.0 : shift * z_r);
+    const double p_r = REST ? row_exp2(rest_log * ROW_LOG2E) : 0.0, sum = list_sum + p_r;
+    const bool nan = z != z, used = w != 0 && list_best > -INFINITY && (m > -INFINITY || nan);
+    const double scale = w * temperature;
+    if (tid == 0) {
+        double l = 0;
+        if (used && !nan) {
+            // the list's scores were taken relative to its own highest
+            const double ln_z = row_log(z), gap = (high_l > -INFINITY ? (double)high_l - m : 0.0) * inv_t;
+            l = (list_cross - list_sum * gap) / sum + ln_z - row_log(sum);
+            if (REST && p_r > 0) l += p_r / sum * (z_r > 0 ? rest_log - row_log(z_r) - ((double)m_r - m) * inv_t : INFINITY);
         }
-        best = wave_max(best);
-        if (REST) m = wave_max(m);
-        double sum = 0, cross = 0, z_l = 0;
-        for (int j = tid; j < k; j += 64) {
-            if (cls[j] < 0) continue;
-            const double y = teacher[j] == best ? 0.0 : ((double)teacher[j] - best) * unit, z = ((double)student[j] - m) * unit;
-            const double p = row_exp2(y);
-            sum += p;
-            if (p > 0) cross += p * (y - z);
-            if (REST && first[j]) z_l += student[j] < INFINITY ? row_exp2(z) : NAN;
-            teacher[j] = (float)p;
-        }
-        sum = wave_sum(sum);
-        cross = wave_sum(cross) * (1.0 / ROW_LOG2E);
-        z_l = wave_sum(z_l);
-        // NaN or +infinity among the scores: their exponentials, and with them the sum, are NaN
-        const double shift = REST ? (z_r > 0 ? row_exp2(((double)m_r - m) * unit) : 0.0) : 1.0, z = z_l + (REST && z_r == 0 ? 0.0 : shift * z_r);
-        const bool nan = z != z || z_r != z_r, used = w != 0 && best > -INFINITY && (m > -INFINITY || nan);
-        double rest_log = 0, p_r = 0;
-        if (REST) {
-            rest_log = (double)rest[r];
-            p_r = row_exp2(rest_log * ROW_LOG2E);
-            sum += p_r;
-        }
-        const double ln = row_log(tid == 0 ? z : tid == 1 ? sum : z_r);
-        const double ln_z = __shfl(ln, 0), ln_s = __shfl(ln, 1), ln_r = __shfl(ln, 2);
-        if (tid == 0) {
-            double l = cross / sum + ln_z - ln_s;
-            if (REST && p_r > 0) l += p_r / sum * (z_r > 0 ? rest_log - ln_r - ((double)m_r - m) * inv_t : INFINITY);
-            loss[r] = used ? (nan ? NAN : (float)(w * temperature * temperature * l)) : 0.0f;
-            const double scale = w * temperature;
-            state = used ? (nan ? 2 : 1) : 0;
-            constant[0] = REST ? (z_r > 0 ? scale * (shift / z - p_r / sum / z_r) : 0.0) : scale / z;   // others
-            constant[1] = scale / z;                      // listed: student's part,
-            constant[2] = scale / sum;                    // teacher's part
-            constant[3] = (double)m;
-        }
+        loss[r] = used ? (nan ? NAN : (float)(w * temperature * temperature * l)) : 0.0f;
     }
     if (!GRAD) return;
-    team_sync<W>();
     T* g = grad + r * n_classes;
-    const int how = state;
-    const float scale = (float)constant[0];
+    // the row's constant for the others
+    const float others = (float)(!REST ? scale / z : z_r > 0 ? scale * (shift / z - p_r / sum / z_r) : 0.0);
     each([&](const float(&v)[RUN], int c) {
         struct __attribute__((packed, aligned(sizeof(T)))) { T e[RUN]; } out;
 #pragma unroll
         for (int j = 0; j < RUN; ++j) {
-            const float d = scale * __builtin_amdgcn_exp2f((v[j] - from) * unit_f);
-            out.e[j] = (T)(how == 1 ? d : how ? NAN : 0.0f);
+            const float d = others * __builtin_amdgcn_exp2f((v[j] - from) * unit_f);
+            out.e[j] = (T)(used ? (nan ? NAN : d) : 0.0f);
         }
         if (c + RUN <= n_classes) {
             *(decltype(out)*)(g + c) = out;
@@ -171,16 +195,18 @@ __global__ __launch_bounds__(64 * W) void lsr_distill_team_kernel(
                 if (c + j < n_classes) g[c + j] = out.e[j];
         }
     });
-    if (how != 1) return;
+    if (!used || nan) return;
     team_sync<W>();                                       // the listed classes are written after the pass over the row
+#pragma unroll 1
     for (int j = tid; j < k; j += THREADS) {
         if (!first[j]) continue;
         float p = teacher[j];
         if (again) {
             p = 0;
+#pragma unroll 1
             for (int i = 0; i < k; ++i) p += cls[i] == cls[j] ? teacher[i] : 0.0f;
         }
-        g[cls[j]] = (T)(float)(constant[1] * row_exp2(((double)student[j] - constant[3]) * unit) - constant[2] * p);
+        g[cls[j]] = (T)(float)(scale * (row_exp2(((double)student[j] - m) * unit) / z - p / sum));
     }
 }
 

@@ -402,11 +402,22 @@ template <int DT, int W, int N> struct team_row {
         }
         return make_uint4(w[0], w[1], w[2], w[3]);
     }
+    // Loads are not under a condition (the compiler would wait for each before the next): a run that is not whole takes the
+    // row's first one, and `settle` blanks it.
     __device__ __forceinline__ uint4 read(int step) const {
         const int c = first_class(step);
-        if (c + RUN > n_classes) return nothing();
-        const run v = *(const run*)(row + c);
+        // 32-bit offset from a wave-uniform address: one address register per load
+        const uint32_t at = c + RUN <= n_classes ? (uint32_t)c * (uint32_t)sizeof(T) : 0u;
+        const run v = *(const run*)((const char*)row + at);
         return make_uint4(v.w[0], v.w[1], v.w[2], v.w[3]);
+    }
+    __device__ __forceinline__ uint4 settle(int step, const uint4& u) const {
+        const bool whole = first_class(step) + RUN <= n_classes;
+        return make_uint4(whole ? u.x : nothing().x, whole ? u.y : nothing().y, whole ? u.z : nothing().z, whole ? u.w : nothing().w);
+    }
+    __device__ __forceinline__ uint4 read_any(int step) const {
+        const int c = first_class(step);
+        return c < n_classes && c + RUN > n_classes ? read_end(c) : settle(step, read(step));
     }
     __device__ __forceinline__ void open(const T* r, int classes) {
         row = r;
@@ -415,6 +426,13 @@ template <int DT, int W, int N> struct team_row {
         if (N) {
 #pragma unroll
             for (int i = 0; i < (N ? N : 1); ++i) kept[i] = read(i);
+        }
+    }
+    // waits for the row that `open` has requested
+    __device__ __forceinline__ void arrive() {
+        if (N) {
+#pragma unroll
+            for (int i = 0; i < (N ? N : 1); ++i) kept[i] = settle(i, kept[i]);
             const int end = first_class(steps - 1);
             if (end < n_classes && end + RUN > n_classes) {
                 const uint4 u = read_end(end);
@@ -460,13 +478,11 @@ template <int DT, int W, int N> struct team_row {
 #pragma unroll
                 for (int j = 0; j < AHEAD; ++j) u[j] = read(i + j);
 #pragma unroll
-                for (int j = 0; j < AHEAD; ++j) f(i + j, u[j]);
+                for (int j = 0; j < AHEAD; ++j) f(i + j, settle(i + j, u[j]));
             }
 #pragma unroll 1
             for (; i < steps; ++i) {
-                const int c = first_class(i);
-                uint4 u = c < n_classes && c + RUN > n_classes ? read_end(c) : read(i);
-                f(i, u);
+                f(i, read_any(i));
             }
         }
     }
@@ -522,6 +538,9 @@ __device__ __forceinline__ float team_collect(team_row<DT, W, N>& row, int kk, t
         for (int i = 0; i < ROW_GROUPS / 64; ++i) list.group[i * 64 + tid] = i < PER ? row_key(most[i < PER ? i : 0]) : 0u;
     } else if (W == 4) {
         list.group[tid] = row_key(most[0]);
+    } else if (W == 8) {
+        const float best = row_max(most[0], quad_move<QUAD_XOR1>(most[0]));
+        if ((tid & 1) == 0) list.group[tid >> 1] = row_key(best);
     } else {
         const float best = quad_max(most[0]);
         if ((tid & 3) == 0) list.group[tid >> 2] = row_key(best);
@@ -571,8 +590,9 @@ template <int W> __device__ __forceinline__ int team_above(const team_list<W>& l
             constexpr int DT = ROW_F32;                                                                   \
             if ((classes) <= 1024) { constexpr int W = 1, N = 4; __VA_ARGS__; }                           \
             else if ((classes) <= 4096) { constexpr int W = 4, N = 4; __VA_ARGS__; }                      \
-            else if ((classes) <= 16384) { constexpr int W = 4, N = 16; __VA_ARGS__; }                    \
-            else if ((classes) <= 32768) { constexpr int W = 16, N = 8; __VA_ARGS__; }                    \
+            else if ((classes) <= 8192) { constexpr int W = 4, N = 8; __VA_ARGS__; }                      \
+            else if ((classes) <= 16384) { constexpr int W = 8, N = 8; __VA_ARGS__; }                     \
+            else if ((classes) <= 32768) { constexpr int W = 8, N = 16; __VA_ARGS__; }                    \
             else if ((classes) <= 65536) { constexpr int W = 16, N = 16; __VA_ARGS__; }                   \
             else { constexpr int W = 16, N = 0; __VA_ARGS__; }                                            \
         } else if ((dtype) == LSR_F16) {                                                                  \
@@ -588,7 +608,8 @@ template <int W> __device__ __forceinline__ int team_above(const team_list<W>& l
         if ((classes) <= 1024) { constexpr int W = 1, N = 2; __VA_ARGS__; }                               \
         else if ((classes) <= 4096) { constexpr int W = 4, N = 2; __VA_ARGS__; }                          \
         else if ((classes) <= 16384) { constexpr int W = 4, N = 8; __VA_ARGS__; }                         \
-        else if ((classes) <= 65536) { constexpr int W = 16, N = 8; __VA_ARGS__; }                        \
+        else if ((classes) <= 32768) { constexpr int W = 8, N = 8; __VA_ARGS__; }                         \
+        else if ((classes) <= 65536) { constexpr int W = 8, N = 16; __VA_ARGS__; }                        \
         else if ((classes) <= 131072) { constexpr int W = 16, N = 16; __VA_ARGS__; }                      \
         else { constexpr int W = 16, N = 0; __VA_ARGS__; }                                                \
     } while (0)

@@ -362,7 +362,7 @@ __global__ __launch_bounds__(64 * W) void lsr_sample_team_kernel(const typename 
     {
         const int c = Row::first_class(step);
         float v[RUN];
-        Row::decode(c < n_classes && c + RUN > n_classes ? row.read_end(c) : row.read(step), v);
+        Row::decode(row.read_any(step), v);
         uint64_t own = 0;
 #pragma unroll
         for (int j = 0; j < RUN; ++j)

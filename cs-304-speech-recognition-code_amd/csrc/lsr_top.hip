@@ -56,12 +56,13 @@ __global__ __launch_bounds__(64 * W) void lsr_top_team_kernel(const typename row
     __shared__ team_list<W> list;
     __shared__ int hist[256];
     __shared__ uint64_t one;
-    __shared__ float part[W], best, high;
+    __shared__ float part[W], tail[REST ? ROOM : 1], best, high;
     const int tid = threadIdx.x;
     const int64_t r = blockIdx.x;
     const int kk = k + (REST ? 1 : 0);                    // the first entry of the rest as well
     Row row;
     row.open(scores + r * row_stride, n_classes);
+    row.arrive();
     float bound = team_collect<DT, W, N>(row, kk, list);
     int n = list.n, bound_class = -1;                     // collected: above the bound, or equal up to this class
     bool equal = true;                                    // every score that equals the bound is collected
@@ -116,8 +117,11 @@ __global__ __launch_bounds__(64 * W) void lsr_top_team_kernel(const typename row
         const int at = i * THREADS + tid;
         if (at >= n || place[i] < k) continue;
         const float v = row_value((uint32_t)(list.entry[at] >> 32));
-        sum += v == from ? 1.0f : __builtin_amdgcn_exp2f((v - from) * unit);
+        // by place: the list itself is in the order in which it was filled, which is not the same every time
+        tail[place[i]] = v == from ? 1.0f : __builtin_amdgcn_exp2f((v - from) * unit);
     }
+    team_sync<W>();
+    for (int i = k + tid; i < n; i += THREADS) sum += tail[i];
     if (from > -INFINITY) {
         row.next_pass();
         if (equal) {
