@@ -22,6 +22,7 @@ __global__ __launch_bounds__(64 * W) void lsr_distill_team_kernel(
     typename row_type<DT>::type* __restrict__ grad) {
     using T = typename row_type<DT>::type;
     using Row = team_row<DT, W, N>;
+    const row_exp2_t row_exp2;
     constexpr int THREADS = 64 * W, RUN = Row::RUN, MAP = W == 1 ? 1024 : W == 4 ? 16384 : 131072;   // bits of the map
     __shared__ uint32_t map[MAP / 32];
     __shared__ int cls[LSR_MAX_TOP];                      // listed classes, -1 for absent entries
@@ -223,6 +224,7 @@ __global__ __launch_bounds__(LSR_ROW_THREADS) void lsr_distill_quad_kernel(
     typename row_type<DT>::type* __restrict__ grad) {
     // 16 floats of padding: the runs that 16 lanes read at once, four rows', lie in different banks
     __shared__ float listed[LSR_QUAD_ROWS][4 * E + 16];
+    const row_exp2_t row_exp2;
     const int q = threadIdx.x & 3, slot = threadIdx.x >> 2;
     const int64_t row = (int64_t)blockIdx.x * LSR_QUAD_ROWS + slot;
     const bool live = row < n_rows;

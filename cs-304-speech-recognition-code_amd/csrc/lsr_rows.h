@@ -48,24 +48,34 @@ __device__ __forceinline__ uint64_t row_wave_max(uint64_t v) {
 }
 
 // 2^y for y <= 0 to 2^-50 of the result: the fraction in [-1/2, 1/2] goes through a polynomial of degree 10 that is 1 at 0
-// (interpolation of (2^f - 1) / f at the Chebyshev nodes, largest relative error 5.6e-16).  16 instructions of the same
-// rate as 32-bit ones here; the library's exp takes about three times as many.
-__device__ __forceinline__ double row_exp2(double y) {
-    y = y > -1200.0 ? y : -1200.0;
-    const double n = __builtin_rint(y), f = y - n;
-    double p = 7.070977866508138e-09;
-    p = __builtin_fma(p, f, 1.0205905413765595e-07);
-    p = __builtin_fma(p, f, 1.3215451633221434e-06);
-    p = __builtin_fma(p, f, 1.5252672924850737e-05);
-    p = __builtin_fma(p, f, 0.00015403530424776529);
-    p = __builtin_fma(p, f, 0.0013333558200794592);
-    p = __builtin_fma(p, f, 0.009618129107618665);
-    p = __builtin_fma(p, f, 0.05550410866465167);
-    p = __builtin_fma(p, f, 0.24022650695910075);
-    p = __builtin_fma(p, f, 0.6931471805599462);
-    p = __builtin_fma(p, f, 1.0);
-    return __builtin_amdgcn_ldexp(p, (int)n);
-}
+// (interpolation of (2^f - 1) / f at the Chebyshev nodes, largest relative error 5.6e-16).  16 instructions, all of them of
+// the rate of 32-bit ones on this part; the library's exp takes about three times as many.  The coefficients are held in
+// scalar registers from the object's creation on: as literals each would be moved into the accumulator first, two
+// instructions more per step.  0 for -infinity and NaN.
+struct row_exp2_t {
+    double c10 = 7.070977866508138e-09, c9 = 1.0205905413765595e-07, c8 = 1.3215451633221434e-06, c7 = 1.5252672924850737e-05,
+           c6 = 0.00015403530424776529, c5 = 0.0013333558200794592, c4 = 0.009618129107618665, c3 = 0.05550410866465167,
+           c2 = 0.24022650695910075, c1 = 0.6931471805599462, low = -1200.0;
+    __device__ __forceinline__ row_exp2_t() {
+        asm("" : "+s"(c10), "+s"(c9), "+s"(c8), "+s"(c7), "+s"(c6), "+s"(c5));
+        asm("" : "+s"(c4), "+s"(c3), "+s"(c2), "+s"(c1), "+s"(low));
+    }
+    __device__ __forceinline__ double operator()(double y) const {
+        y = fmax(y, low);
+        const double n = __builtin_rint(y), f = y - n;
+        double p = __builtin_fma(f, c10, c9);
+        p = __builtin_fma(p, f, c8);
+        p = __builtin_fma(p, f, c7);
+        p = __builtin_fma(p, f, c6);
+        p = __builtin_fma(p, f, c5);
+        p = __builtin_fma(p, f, c4);
+        p = __builtin_fma(p, f, c3);
+        p = __builtin_fma(p, f, c2);
+        p = __builtin_fma(p, f, c1);
+        p = __builtin_fma(p, f, 1.0);
+        return __builtin_amdgcn_ldexp(p, (int)n);
+    }
+};
 #define ROW_LOG2E 1.4426950408889634
 // Natural logarithm of a positive number to 2^-49 of the result (or 2^-49 for numbers near 1): x = m 2^e with m in
 // [sqrt(1/2), sqrt(2)), ln m = 2 artanh(s) with s = (m - 1) / (m + 1), |s| < 0.172, by its series up to s^19 (the next term
@@ -245,16 +255,16 @@ template <int E> __device__ __forceinline__ void quad_sort(double (&e)[E], int q
 #pragma unroll
     for (int i = 0; i < E; ++i) o[i] = quad_move<QUAD_XOR1>(e[E - 1 - i]);
 #pragma unroll
-    for (int i = 0; i < E; ++i) e[i] = odd ? row_min(e[i], o[i]) : row_max(e[i], o[i]);
+    for (int i = 0; i < E; ++i) e[i] = (e[i] < o[i]) != odd ? o[i] : e[i];
     quad_merge_lane(e);
 #pragma unroll
     for (int i = 0; i < E; ++i) o[i] = quad_move<QUAD_XOR3>(e[E - 1 - i]);
 #pragma unroll
-    for (int i = 0; i < E; ++i) e[i] = upper ? row_min(e[i], o[i]) : row_max(e[i], o[i]);
+    for (int i = 0; i < E; ++i) e[i] = (e[i] < o[i]) != upper ? o[i] : e[i];
 #pragma unroll
     for (int i = 0; i < E; ++i) o[i] = quad_move<QUAD_XOR1>(e[i]);
 #pragma unroll
-    for (int i = 0; i < E; ++i) e[i] = odd ? row_min(e[i], o[i]) : row_max(e[i], o[i]);
+    for (int i = 0; i < E; ++i) e[i] = (e[i] < o[i]) != odd ? o[i] : e[i];
     quad_merge_lane(e);
 }
 // The first E of the quad's entries in descending order, the same in all four lanes.

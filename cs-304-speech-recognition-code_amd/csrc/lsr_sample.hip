@@ -40,6 +40,7 @@ __device__ __forceinline__ void sample_by_radix(const typename row_type<DT>::typ
                                                 int top_k, double top_p, double min_p, float u, const sample_args& a,
                                                 uint64_t* hist, uint64_t* shared, int32_t* index, float* logprob) {
     constexpr int THREADS = 64 * W;
+    const row_exp2_t row_exp2;
     const int tid = threadIdx.x;
     const double unit = isinf(best) ? 1.0 : ROW_LOG2E / t;
     uint64_t least = 1;
@@ -142,6 +143,7 @@ __global__ __launch_bounds__(64 * W) void lsr_sample_team_kernel(const typename 
     __shared__ uint64_t sorted[LSR_MAX_TOP], part[W], above, lowest;
     __shared__ float part_f[W];
     __shared__ int cut_bin;
+    const row_exp2_t row_exp2;
     const int tid = threadIdx.x;
     const int64_t r = blockIdx.x;
     const auto* mine = scores + r * row_stride;
@@ -241,7 +243,7 @@ __global__ __launch_bounds__(64 * W) void lsr_sample_team_kernel(const typename 
 
     float last = -INFINITY;                               // kept: above this score, or equal up to this class
     int last_class = -1;
-    auto keeps = [&](float v, int c) { return v > last || (v == last && c <= last_class); };
+    auto keeps = [&](float v, int c) { return (v > last) | ((v == last) & (c <= last_class)); };
     auto weigh = [&](float v) { return row_fixed(row_exp2(((double)v - best) * unit), a.magic); };
     const float per_bin = (float)fmin(BINS / 32 / t, 1e30);
     auto bin_of = [&](float v) { return (int)fminf((best - v) * per_bin, (float)(BINS - 1)); };
@@ -398,15 +400,17 @@ static void lsr_sample_team(hipStream_t stream, const void* scores_d, int64_t n_
                        (const typename row_type<DT>::type*)scores_d, n_classes, row_stride, uniform_d, a, index_d, logprob_d);
 }
 
-// Short rows (at most LSR_QUAD_CLASSES classes), a quad per row.  ORDER: some row is cut by its order, so the entries are
-// sorted; the sorted weights give the threshold, which the registers in class order are then compared with.  The sums are
-// 64-bit floating ones in a fixed order.
+// Short rows (at most LSR_QUAD_CLASSES classes), a quad per row.  ORDER: some row is cut by its order.  The weights fall
+// with the scores, so a sorted copy of them, without the classes, says which weight is the last one that is kept and how
+// many entries of that weight; where not all of those are, they are taken one by one.  The sums are 64-bit floating ones in
+// a fixed order.
 template <int DT, int E, bool ORDER>
 __global__ __launch_bounds__(LSR_ROW_THREADS) void lsr_sample_quad_kernel(const typename row_type<DT>::type* __restrict__ scores,
                                                                           int64_t n_rows, int n_classes, int64_t row_stride,
                                                                           const float* __restrict__ uniform, sample_args a,
                                                                           int32_t* __restrict__ index,
                                                                           float* __restrict__ logprob) {
+    const row_exp2_t row_exp2;
     const int q = threadIdx.x & 3;
     const int64_t row = (int64_t)blockIdx.x * LSR_QUAD_ROWS + (threadIdx.x >> 2);
     const bool live = row < n_rows;
@@ -429,58 +433,72 @@ __global__ __launch_bounds__(LSR_ROW_THREADS) void lsr_sample_quad_kernel(const 
             if (best == INFINITY) x[i] = x[i] == INFINITY ? 0.0f : -INFINITY;
         if (best == INFINITY) best = 0.0f;
     }
+    const bool greedy = !(t > 0);
     const double unit = ROW_LOG2E / t;
-    float last = -INFINITY;                               // the last entry that is kept
-    int last_class = n_classes;
+    const float floor = min_p > 0 ? sample_floor(best, t, min_p) : -INFINITY;
+    double w[E];
+#pragma unroll
+    for (int i = 0; i < E; ++i) w[i] = row_exp2(((double)x[i] - best) * unit);      // 0 for -infinity
     if (ORDER) {
         const double top_p = a.top_p_d ? (double)a.top_p_d[r] : a.top_p;
         const int cut = a.top_k_d ? a.top_k_d[r] : a.top_k;
         const int top_k = cut > 0 ? cut : 4 * E;
-        double e[E], w[E];
+        double s[E], sum = 0;
 #pragma unroll
-        for (int i = 0; i < E; ++i) e[i] = quad_entry(row_key(x[i]), quad_class(i, q));
-        quad_sort<E>(e, q);
-        double sum = 0, least = 3.9;
+        for (int i = 0; i < E; ++i) s[i] = w[i];
+        quad_sort<E>(s, q);
 #pragma unroll
-        for (int i = 0; i < E; ++i) w[i] = 0;
-        if (__any(top_p < 1)) {
-#pragma unroll
-            for (int i = 0; i < E; ++i) {
-                const uint32_t key = quad_entry_key(e[i]);
-                w[i] = key && q * E + i < top_k ? row_exp2(((double)row_value(key) - best) * unit) : 0.0;
-                sum += w[i];
-            }
-        }
+        for (int i = 0; i < E; ++i) sum += q * E + i < top_k ? s[i] : 0.0;
         const double target = top_p < 1 ? top_p * quad_sum(sum) : INFINITY;
-        double run = quad_before(sum, q);
+        double run = quad_before(sum, q), least = INFINITY;
+        int kept = 0;                                     // places: one is kept while the weight ahead of it is short
 #pragma unroll
         for (int i = 0; i < E; ++i) {
             const int place = q * E + i;
-            // a place is kept while the weight ahead of it is short of the target
-            if (place < top_k && (place == 0 || run < target) && quad_entry_key(e[i])) least = row_min(least, e[i]);
-            run += w[i];
+            const bool in = (place < top_k) & ((place == 0) | (run < target));
+            least = in ? s[i] : least;
+            kept += in;
+            run += s[i];
         }
         least = quad_min(least);
-        if (!none) {
-            last = row_value(quad_entry_key(least));
-            last_class = quad_entry_class(least);
-        }
-    }
-    if (min_p > 0) {
-        const float floor = sample_floor(best, t, min_p);
-        if (floor > last) {
-            last = floor;
-            last_class = n_classes;
-        }
-    }
-    double w[E], total = 0;
-    const bool greedy = !(t > 0);
+        kept = quad_sum(kept);
+        // entries above the last weight that is kept, and of that weight
+        int above = 0, same = 0;
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-        const bool kept = x[i] > last || (x[i] == last && quad_class(i, q) <= last_class);
-        w[i] = kept && x[i] > -INFINITY ? row_exp2(((double)x[i] - best) * unit) : 0.0;
+        for (int i = 0; i < E; ++i) {
+            above += w[i] > least;
+            same += w[i] == least;
+        }
+        above = quad_sum(above);
+        int need = kept - above, taken = 0;               // entries of the last weight still to take; bits of those taken
+        const bool some = need < quad_sum(same) && least > 0;
+        if (__any(some)) {                                // by score, equal ones by class
+            while (__any(some && need > 0)) {
+                float high = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < E; ++i)
+                    if ((w[i] == least) & !(taken >> i & 1)) high = row_max(high, x[i]);
+                high = quad_max(high);
+                int first = 1 << 30;
+#pragma unroll
+                for (int i = 0; i < E; ++i)
+                    if ((w[i] == least) & !(taken >> i & 1) & (x[i] == high)) first = min(first, quad_class(i, q));
+                first = quad_min(first);
+#pragma unroll
+                for (int i = 0; i < E; ++i)
+                    if ((need > 0) & (quad_class(i, q) == first)) taken |= 1 << i;
+                --need;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < E; ++i)
+            if ((w[i] < least) | (some & (w[i] == least) & !(taken >> i & 1))) w[i] = 0;
     }
+    double total = 0;
     double lane[E / 4];
+#pragma unroll
+    for (int i = 0; i < E; ++i)
+        if (x[i] < floor) w[i] = 0;
 #pragma unroll
     for (int g = 0; g < E / 4; ++g) {
         lane[g] = (w[4 * g] + w[4 * g + 1]) + (w[4 * g + 2] + w[4 * g + 3]);
@@ -495,10 +513,9 @@ __global__ __launch_bounds__(LSR_ROW_THREADS) void lsr_sample_quad_kernel(const 
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             run += w[4 * g + j];
-            if (w[4 * g + j] > 0) {
-                end = quad_class(4 * g + j, q);
-                if (run > goal) at = min(at, end);
-            }
+            const bool there = w[4 * g + j] > 0;
+            end = there ? quad_class(4 * g + j, q) : end;
+            at = (there & (run > goal)) ? min(at, end) : at;
         }
         base += quad_sum(lane[g]);
     }

@@ -203,7 +203,7 @@ __global__ __launch_bounds__(LSR_ROW_THREADS) void lsr_top_quad_kernel(const typ
     float high = -INFINITY;
 #pragma unroll
     for (int i = 0; i < E; ++i) {
-        const bool beyond = x[i] < last || (x[i] == last && quad_class(i, q) > last_class);
+        const bool beyond = (x[i] < last) | ((x[i] == last) & (quad_class(i, q) > last_class));
         x[i] = beyond ? x[i] : -INFINITY;
         high = row_max(high, x[i]);
     }

@@ -213,6 +213,10 @@ class Engine:
             raise NativeError(f"lsr_ctx_create({device}) failed with code {rc}")
         self.ctx = ctx
         self._stream = torch.cuda.current_stream(self.device)
+        self._stream_handle = self._stream.cuda_stream
+        # the raw handle of the current stream without making a Stream object of it (a sixth of the time), where torch has it
+        self._raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+            lambda index: torch.cuda.current_stream(index).cuda_stream)
         self._check(self.lib.lsr_set_stream(self.ctx, c_void_p(self._stream.cuda_stream)))
         self._model_token = None
         self._graph_token = None
@@ -253,6 +257,7 @@ class Engine:
             stream = self.torch.cuda.current_stream(self.device)
         self._check(self.lib.lsr_set_stream(self.ctx, c_void_p(stream.cuda_stream)))
         self._stream = stream
+        self._stream_handle = stream.cuda_stream
 
     def on_current_stream(self, fn, *args) -> None:
         """``fn(ctx, *args)`` on torch's current stream, after the work already queued on the engine's stream (the two are
@@ -260,21 +265,24 @@ class Engine:
         engine's earlier work is not waited for: a capture starts from finished work."""
         cuda = self.torch.cuda
         before = cuda.current_device()
-        stream = cuda.current_stream(self.device)
+        handle = self._raw_stream(self.device_index)
         try:
-            if stream == self._stream:
-                self._check(fn(self.ctx, *args))
-                return
-            if not cuda.is_current_stream_capturing():
-                stream.wait_stream(self._stream)
-            self._check(self.lib.lsr_set_stream(self.ctx, c_void_p(stream.cuda_stream)))
-            try:
-                self._check(fn(self.ctx, *args))
-            finally:
-                self._check(self.lib.lsr_set_stream(self.ctx, c_void_p(self._stream.cuda_stream)))
+            if handle == self._stream_handle:
+                rc = fn(self.ctx, *args)
+            else:
+                stream = cuda.current_stream(self.device)
+                if not cuda.is_current_stream_capturing():
+                    stream.wait_stream(self._stream)
+                self._check(self.lib.lsr_set_stream(self.ctx, c_void_p(handle)))
+                try:
+                    rc = fn(self.ctx, *args)
+                finally:
+                    self._check(self.lib.lsr_set_stream(self.ctx, c_void_p(self._stream_handle)))
         finally:
             if before != self.device_index:              # the library makes its own device the current one
                 cuda.set_device(before)
+        if rc:
+            self._check(rc)
 
     @staticmethod
     def _ptr(t) -> c_void_p:
