@@ -507,23 +507,23 @@ template <int DT, int W, int N> struct team_row {
 };
 
 // ---- the first entries of a long row ------------------------------------------------------------------------------------
-// The classes of a row are dealt out to ROW_GROUPS groups or fewer; the kk-th largest of the groups' best scores is a lower
-// bound of the row's kk-th largest score, as kk groups have a score that high.  One pass finds the groups' best, a
-// second collects what reaches the bound: for scores in no particular order about -G ln(1 - kk / G) entries of G = 256
-// groups, 73 for kk = 64.  Their places follow from counting, for each, the entries above it.
+// The classes of a row are dealt out to ROW_GROUPS groups; the kk-th largest of the groups' best scores is a lower bound of
+// the row's kk-th largest score, as kk groups have a score that high.  One pass finds the groups' best, a second collects
+// what reaches the bound: for scores in no particular order about -G ln(1 - kk / G) entries of G = 256 groups, 73 for
+// kk = 64.  Places follow from counting, for each entry, the entries above it.
 #define ROW_GROUPS 256
-template <int W> struct team_list {
-    static constexpr int ROOM = W == 1 ? 1024 : 2048;
-    uint64_t entry[ROOM];
-    uint32_t group[ROW_GROUPS];
+template <int W, int SIZE> struct team_list {
+    static constexpr int ROOM = SIZE;
+    uint64_t entry[SIZE];
+    alignas(16) uint32_t group[ROW_GROUPS];
     int n;
     uint32_t bound;
 };
 
-// Collects the entries of every group whose best is among the kk best groups; the bound as a score, -FLT_MAX when all
-// present entries are collected.  `list.n` may exceed ROOM: then only some of them are there.
-template <int DT, int W, int N>
-__device__ __forceinline__ float team_collect(team_row<DT, W, N>& row, int kk, team_list<W>& list) {
+// Collects the entries that reach the bound of kk; returns the bound as a score, -FLT_MAX when there are fewer groups with
+// a score and all present entries are collected.  `list.n` may exceed ROOM: then only some of them are there.
+template <int DT, int W, int N, int SIZE>
+__device__ __forceinline__ float team_collect(team_row<DT, W, N>& row, int kk, team_list<W, SIZE>& list) {
     using Row = team_row<DT, W, N>;
     constexpr int THREADS = 64 * W, RUN = Row::RUN, PER = W == 1 ? 4 : 1;
     const int tid = threadIdx.x;
@@ -545,40 +545,40 @@ __device__ __forceinline__ float team_collect(team_row<DT, W, N>& row, int kk, t
     }
     if (W == 1) {
 #pragma unroll
-        for (int i = 0; i < ROW_GROUPS / 64; ++i) list.group[i * 64 + tid] = i < PER ? row_key(most[i < PER ? i : 0]) : 0u;
-    } else if (W == 4) {
-        list.group[tid] = row_key(most[0]);
-    } else if (W == 8) {
-        const float best = row_max(most[0], quad_move<QUAD_XOR1>(most[0]));
-        if ((tid & 1) == 0) list.group[tid >> 1] = row_key(best);
+        for (int i = 0; i < ROW_GROUPS / 64; ++i) list.group[i * 64 + tid] = row_key(most[i < PER ? i : 0]);
     } else {
-        const float best = quad_max(most[0]);
-        if ((tid & 3) == 0) list.group[tid >> 2] = row_key(best);
+        float best = most[0];
+        if (W >= 8) best = row_max(best, quad_move<QUAD_XOR1>(best));
+        if (W >= 16) best = row_max(best, quad_move<QUAD_XOR2>(best));
+        constexpr int LANES = W == 1 ? 1 : THREADS / ROW_GROUPS;        // of a group
+        if (tid % LANES == 0) list.group[tid / LANES] = row_key(best);
     }
     team_sync<W>();
-    for (int g = tid; g < ROW_GROUPS; g += THREADS) {
-        const uint32_t own = list.group[g];
-        int above = 0, equal = 0;
-        for (int i = 0; i < ROW_GROUPS; i += 4) {
-            const uint4 o = *(const uint4*)&list.group[i];
-            above += (o.x > own) + (o.y > own) + (o.z > own) + (o.w > own);
-            equal += (o.x == own) + (o.y == own) + (o.z == own) + (o.w == own);
+    if (tid < 64) {                                       // the largest number that kk groups reach, bit by bit
+        const uint4 o = *(const uint4*)&list.group[tid * 4];
+        uint32_t bound = 0;
+#pragma unroll 1
+        for (uint32_t bit = 1u << 31; bit; bit >>= 1) {
+            const uint32_t b = bound | bit;
+            const int reach = __popcll(__ballot(o.x >= b)) + __popcll(__ballot(o.y >= b)) + __popcll(__ballot(o.z >= b)) +
+                              __popcll(__ballot(o.w >= b));
+            if (reach >= kk) bound = b;
         }
-        if (above < kk && kk <= above + equal) list.bound = own;
+        if (tid == 0) list.bound = bound;
     }
     team_sync<W>();
     const float bound = list.bound ? row_value(list.bound) : -3.402823466e38f;
     row.next_pass();
     row.template each<4>([&](int, const float(&v)[RUN], int c) {
-        bool any = false;
+        float high = v[0];
 #pragma unroll
-        for (int j = 0; j < RUN; ++j) any |= v[j] >= bound;
-        if (any) {
+        for (int j = 1; j < RUN; ++j) high = row_max(high, v[j]);
+        if (high >= bound) {
 #pragma unroll
             for (int j = 0; j < RUN; ++j)
                 if (v[j] >= bound) {
                     const int at = atomicAdd(&list.n, 1);
-                    if (at < team_list<W>::ROOM) list.entry[at] = row_entry(row_key(v[j]), c + j);
+                    if (at < SIZE) list.entry[at] = row_entry(row_key(v[j]), c + j);
                 }
         }
     });
@@ -586,8 +586,9 @@ __device__ __forceinline__ float team_collect(team_row<DT, W, N>& row, int kk, t
     return bound;
 }
 // how many of the list's first n entries are above e
-template <int W> __device__ __forceinline__ int team_above(const team_list<W>& list, int n, uint64_t e) {
+template <int W, int SIZE> __device__ __forceinline__ int team_above(const team_list<W, SIZE>& list, int n, uint64_t e) {
     int above = 0;
+#pragma unroll 8
     for (int i = 0; i < n; ++i) above += list.entry[i] > e;
     return above;
 }

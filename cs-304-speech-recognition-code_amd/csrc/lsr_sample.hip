@@ -33,6 +33,44 @@ __device__ __forceinline__ uint64_t sample_goal(float u, uint64_t sum) {
     return !(at > 0) ? 0 : at >= (double)sum ? sum - 1 : (uint64_t)at;
 }
 
+// The lowest entry of the shortest head of a list whose mass is at least `left`, eight bits at a time; `hist` has 256 places.
+template <int W>
+__device__ __forceinline__ uint64_t list_by_radix(const uint64_t* entry, const uint64_t* mass, int n, uint64_t left,
+                                                  uint64_t* hist, uint64_t* shared) {
+    constexpr int THREADS = 64 * W;
+    const int tid = threadIdx.x;
+    uint64_t threshold = 0;
+    for (int shift = 56; shift >= 0; shift -= 8) {
+        team_sync<W>();
+        for (int i = tid; i < 256; i += THREADS) hist[i] = 0;
+        team_sync<W>();
+        for (int i = tid; i < n; i += THREADS) {
+            const uint64_t e = entry[i];
+            if (shift == 56 || (e >> (shift + 8)) == (threshold >> (shift + 8)))
+                atomicAdd((unsigned long long*)&hist[(e >> shift) & 255], (unsigned long long)mass[i]);
+        }
+        team_sync<W>();
+        if (tid < 64) {                                   // lane l has the digits 255 - 4 l ... 252 - 4 l
+            uint64_t m[4], own = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) own += m[i] = hist[255 - 4 * tid - i];
+            uint64_t run = wave_running(own) - own;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (run < left && left <= run + m[i]) {
+                    shared[0] = threshold | (uint64_t)(255 - 4 * tid - i) << shift;
+                    hist[0] = left - run;
+                }
+                run += m[i];
+            }
+        }
+        team_sync<W>();
+        threshold = shared[0];
+        left = hist[0];
+    }
+    return threshold;
+}
+
 // A row in many passes over memory, by radix selection with weights: for rows that the fast form below does not take (an
 // infinite score, a cut that falls among thousands of scores that are alike).
 template <int DT, int W>
@@ -134,15 +172,15 @@ __global__ __launch_bounds__(64 * W) void lsr_sample_team_kernel(const typename 
                                                                  const float* __restrict__ uniform, sample_args a,
                                                                  int32_t* __restrict__ index, float* __restrict__ logprob) {
     using Row = team_row<DT, W, 0>;
-    constexpr int THREADS = 64 * W, RUN = Row::RUN, ROOM = team_list<W>::ROOM;
-    constexpr int BINS = W == 1 ? 256 : W == 4 ? 1024 : 2048, OWN = BINS / THREADS;
+    constexpr int THREADS = 64 * W, RUN = Row::RUN, ROOM = W == 1 ? 512 : 2048;
+    constexpr int BINS = W == 1 ? 512 : W == 4 ? 2048 : 4096, OWN = BINS / THREADS;
     constexpr int STEPS = (W == 1 ? 1024 : W == 4 ? 16384 : LSR_MAX_CLASSES) / Row::STEP;
-    __shared__ team_list<W> list;
-    __shared__ uint64_t mass[BINS > STEPS ? BINS : STEPS];          // of a bin, of a step, of an entry
+    __shared__ team_list<W, ROOM> list;
+    __shared__ uint64_t mass[BINS > STEPS ? BINS : STEPS];          // of a bin, of an entry of the list, of a step
     __shared__ int bin_n[BINS];
-    __shared__ uint64_t sorted[LSR_MAX_TOP], part[W], above, lowest;
+    __shared__ uint64_t sorted[LSR_MAX_TOP], part[W], above, lowest, kept_sum;
     __shared__ float part_f[W];
-    __shared__ int cut_bin;
+    __shared__ int cut_bin, n_kept;
     const row_exp2_t row_exp2;
     const int tid = threadIdx.x;
     const int64_t r = blockIdx.x;
@@ -157,7 +195,7 @@ __global__ __launch_bounds__(64 * W) void lsr_sample_team_kernel(const typename 
     const double unit = ROW_LOG2E / t;
 
     if (top_k > 0 && top_k <= LSR_MAX_TOP && top_k < n_classes && t > 0) {
-        team_collect<DT, W, 0>(row, top_k, list);
+        team_collect(row, top_k, list);
         const int n = list.n;
         if (n == 0) {
             if (tid == 0) {
@@ -176,35 +214,53 @@ __global__ __launch_bounds__(64 * W) void lsr_sample_team_kernel(const typename 
             const int m = n < top_k ? n : top_k;
             const float best = row_value((uint32_t)(sorted[0] >> 32));
             if (best < INFINITY) {
-                for (int i = tid; i < m; i += THREADS)
-                    mass[i] = row_fixed(row_exp2(((double)row_value((uint32_t)(sorted[i] >> 32)) - best) * unit), a.magic);
-                team_sync<W>();
-                // how many of the ordered entries are kept: those of which the weight ahead is short of the target
-                uint64_t sum = 0;
-                for (int i = 0; i < m; ++i) sum += mass[i];
-                const uint64_t target = sample_target(top_p, sum);
-                const float floor = min_p > 0 ? sample_floor(best, t, min_p) : -INFINITY;
-                int n_kept = 0;
-                uint64_t run = 0, kept_sum = 0;
-                for (int i = 0; i < m; ++i) {
-                    const bool kept = (i == 0 || run < target) && row_value((uint32_t)(sorted[i] >> 32)) >= floor;
-                    run += mass[i];
-                    if (kept) {
-                        n_kept = i + 1;
-                        kept_sum = run;
+                if (tid < 64) {                           // lane l has the places 4 l ... 4 l + 3
+                    const float floor = min_p > 0 ? sample_floor(best, t, min_p) : -INFINITY;
+                    constexpr int FOUR = LSR_MAX_TOP / 64;
+                    uint64_t w[FOUR], own = 0;
+                    float v[FOUR];
+#pragma unroll
+                    for (int i = 0; i < FOUR; ++i) {
+                        const int place = tid * FOUR + i;
+                        v[i] = place < m ? row_value((uint32_t)(sorted[place] >> 32)) : -INFINITY;
+                        w[i] = row_fixed(row_exp2(((double)v[i] - best) * unit), a.magic);
+                        own += w[i];
+                    }
+                    uint64_t run = wave_running(own);
+                    const uint64_t target = sample_target(top_p, wave_last(run));
+                    run -= own;
+                    uint64_t sum = 0;
+                    int kept = 0;
+#pragma unroll
+                    for (int i = 0; i < FOUR; ++i) {      // kept: the weight ahead of it is short of the target
+                        const int place = tid * FOUR + i;
+                        const bool in = (place < m) & ((place == 0) | (run < target)) & (v[i] >= floor);
+                        run += w[i];
+                        sum += in ? w[i] : 0;
+                        kept += in;
+                        mass[place] = w[i];
+                    }
+                    sum = wave_sum(sum);
+                    kept = wave_sum(kept);
+                    if (tid == 0) {
+                        kept_sum = sum;
+                        n_kept = kept;
                     }
                 }
+                team_sync<W>();
+                const int kept = n_kept;
                 const uint64_t goal = sample_goal(u, kept_sum);
-                for (int i = tid; i < n_kept; i += THREADS) {
-                    // weight of the kept entries up to this class, in class order
+                for (int i = tid; i < kept; i += THREADS) {
+                    // weight of the kept entries of lower classes
                     const uint32_t own = (uint32_t)sorted[i];
                     uint64_t before = 0;
                     int ahead = 0;
-                    for (int j = 0; j < n_kept; ++j)
-                        if ((uint32_t)sorted[j] > own) {  // complemented: a lower class
-                            before += mass[j];
-                            ++ahead;
-                        }
+#pragma unroll 8
+                    for (int j = 0; j < kept; ++j) {
+                        const bool lower = (uint32_t)sorted[j] > own;            // classes are complemented
+                        before += lower ? mass[j] : 0;
+                        ahead += lower;
+                    }
                     if (goal == 0 ? ahead == 0 : before <= goal && goal < before + mass[i]) {
                         const float v = row_value((uint32_t)(sorted[i] >> 32));
                         index[r] = (int32_t)~own;
@@ -245,7 +301,7 @@ __global__ __launch_bounds__(64 * W) void lsr_sample_team_kernel(const typename 
     int last_class = -1;
     auto keeps = [&](float v, int c) { return (v > last) | ((v == last) & (c <= last_class)); };
     auto weigh = [&](float v) { return row_fixed(row_exp2(((double)v - best) * unit), a.magic); };
-    const float per_bin = (float)fmin(BINS / 32 / t, 1e30);
+    const float per_bin = (float)fmin(BINS / 24.0 / t, 1e30);
     auto bin_of = [&](float v) { return (int)fminf((best - v) * per_bin, (float)(BINS - 1)); };
 
     // cuts the row where the mass of a head first reaches the target: by number of entries, then by weight
@@ -308,11 +364,19 @@ __global__ __launch_bounds__(64 * W) void lsr_sample_team_kernel(const typename 
         });
         team_sync<W>();
         const int n = list.n;
+        for (int i = tid; i < n; i += THREADS) mass[i] = by_weight ? weigh(row_value((uint32_t)(list.entry[i] >> 32))) : 1;
+        team_sync<W>();
+        if (n > (THREADS < 256 ? THREADS : 256)) {        // many: radix selection in the list
+            const uint64_t least = list_by_radix<W>(list.entry, mass, n, target - ahead, sorted, &lowest);
+            last = row_value((uint32_t)(least >> 32));
+            last_class = (int)~(uint32_t)least;
+            continue;
+        }
         for (int i = tid; i < n; i += THREADS) {
             const uint64_t e = list.entry[i];
             uint64_t before = ahead;
-            for (int j = 0; j < n; ++j)
-                if (list.entry[j] > e) before += by_weight ? weigh(row_value((uint32_t)(list.entry[j] >> 32))) : 1;
+#pragma unroll 4
+            for (int j = 0; j < n; ++j) before += list.entry[j] > e ? mass[j] : 0;
             if (before < target) atomicMin((unsigned long long*)&lowest, (unsigned long long)e);
         }
         team_sync<W>();
@@ -330,11 +394,24 @@ __global__ __launch_bounds__(64 * W) void lsr_sample_team_kernel(const typename 
     team_sync<W>();
     for (int i = tid; i < row.steps; i += THREADS) mass[i] = 0;
     team_sync<W>();
-    row.template each<1>([&](int step, const float(&v)[RUN], int c) {
+    const bool all = last == -INFINITY;
+    const uint64_t zero = (uint64_t)__double_as_longlong(a.magic);
+    row.template each<2>([&](int step, const float(&v)[RUN], int c) {
         uint64_t sum = 0;
+        if (all) {                                        // what is absent weighs nothing by itself
 #pragma unroll
-        for (int j = 0; j < RUN; ++j)
-            if (keeps(v[j], c + j)) sum += weigh(v[j]);
+            for (int j = 0; j < RUN; ++j)
+                sum += (uint64_t)__double_as_longlong(row_exp2(((double)v[j] - best) * unit) + a.magic);
+            sum -= RUN * zero;
+        } else {
+            bool any = false;
+#pragma unroll
+            for (int j = 0; j < RUN; ++j) any |= keeps(v[j], c + j);
+            if (any) {
+#pragma unroll
+                for (int j = 0; j < RUN; ++j) sum += keeps(v[j], c + j) ? weigh(v[j]) : 0;
+            }
+        }
         sum = wave_sum(sum);
         if ((tid & 63) == 0 && sum) atomicAdd((unsigned long long*)&mass[step], (unsigned long long)sum);
     });

@@ -52,8 +52,8 @@ __global__ __launch_bounds__(64 * W) void lsr_top_team_kernel(const typename row
                                                               float* __restrict__ values, int32_t* __restrict__ index,
                                                               float* __restrict__ rest) {
     using Row = team_row<DT, W, N>;
-    constexpr int THREADS = 64 * W, RUN = Row::RUN, ROOM = team_list<W>::ROOM;
-    __shared__ team_list<W> list;
+    constexpr int THREADS = 64 * W, RUN = Row::RUN, ROOM = W == 1 ? 1024 : 2048;
+    __shared__ team_list<W, ROOM> list;
     __shared__ int hist[256];
     __shared__ uint64_t one;
     __shared__ float part[W], tail[REST ? ROOM : 1], best, high;
@@ -63,7 +63,7 @@ __global__ __launch_bounds__(64 * W) void lsr_top_team_kernel(const typename row
     Row row;
     row.open(scores + r * row_stride, n_classes);
     row.arrive();
-    float bound = team_collect<DT, W, N>(row, kk, list);
+    float bound = team_collect(row, kk, list);
     int n = list.n, bound_class = -1;                     // collected: above the bound, or equal up to this class
     bool equal = true;                                    // every score that equals the bound is collected
     if (n > ROOM) {
@@ -147,11 +147,14 @@ static void lsr_top_team(hipStream_t stream, const void* scores_d, int64_t n_row
                          float inv_t, float* values_d, int32_t* index_d, float* rest_d) {
     const auto* scores = (const typename row_type<DT>::type*)scores_d;
     const dim3 grid((unsigned)n_rows), block(64 * W);
+    // 64 registers of 32-bit scores and what the passes need do not fit together: 96 x 50001 with the rest takes 37 us kept
+    // and spilling, 16.5 us read again
+    constexpr int KEEP = DT == ROW_F32 && W == 16 ? 0 : N;
     if (rest_d)
-        hipLaunchKernelGGL((lsr_top_team_kernel<DT, W, N, true>), grid, block, 0, stream, scores, n_classes, row_stride, k,
+        hipLaunchKernelGGL((lsr_top_team_kernel<DT, W, KEEP, true>), grid, block, 0, stream, scores, n_classes, row_stride, k,
                            inv_t, values_d, index_d, rest_d);
     else
-        hipLaunchKernelGGL((lsr_top_team_kernel<DT, W, N, false>), grid, block, 0, stream, scores, n_classes, row_stride, k,
+        hipLaunchKernelGGL((lsr_top_team_kernel<DT, W, KEEP, false>), grid, block, 0, stream, scores, n_classes, row_stride, k,
                            inv_t, values_d, index_d, rest_d);
 }
 
