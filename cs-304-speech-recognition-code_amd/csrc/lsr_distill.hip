@@ -238,34 +238,31 @@ __global__ __launch_bounds__(LSR_ROW_THREADS) void lsr_distill_quad_kernel(
     row_wave_fence();
     const double inv_t = 1.0 / temperature, unit = inv_t * ROW_LOG2E;
     float m = -INFINITY;
-    int nan = 0;
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-        nan |= !(x[i] < INFINITY);
-        m = row_max(m, x[i]);
-    }
+    for (int i = 0; i < E; ++i) m = row_max(m, x[i]);
     m = quad_max(m);
-    nan = quad_max(nan);
     float best = -INFINITY;
     for (int j = q; j < k; j += 4) {
         const int c = index[r * k + j];
         const float v = values[r * k + j];
-        if (c >= 0 && c < n_classes && v > best) best = v;
+        if ((c >= 0) & (c < n_classes) & (v > best)) best = v;
     }
     best = quad_max(best);
     const double w = weight ? (double)weight[r] : 1.0;
-    const bool used = w != 0 && best > -INFINITY && (m > -INFINITY || nan);
-    double sum = 0, cross = 0;
+    // sums over the list: the teacher's weights, those times (y - z), the student's weights of the listed classes
+    double sum = 0, cross = 0, z_l = 0;
     for (int j = q; j < k; j += 4) {
         const int c = index[r * k + j];
         const float v = values[r * k + j];
         if (c < 0 || c >= n_classes || !(v > -INFINITY)) continue;
-        const double y = v == best ? 0.0 : ((double)v - best) * unit, z = ((double)(float)mine[c] - m) * unit;
+        const float s = (float)mine[c];
+        const double y = v == best ? 0.0 : ((double)v - best) * unit, z = ((double)s - m) * unit;
         const double p = row_exp2(y);
         sum += p;
         if (p > 0) cross += p * (y - z);
-        // at least the smallest normal number: what is in the list is what is not 0
-        atomicAdd(&listed[slot][c], fmaxf((float)p, 1.17549435e-38f));
+        // at least the smallest normal number: what is in the list is what is not 0; the first to find 0 counts the class
+        const float old = atomicAdd(&listed[slot][c], fmaxf((float)p, 1.17549435e-38f));
+        if (REST && old == 0) z_l += s < INFINITY ? row_exp2(z) : NAN;
     }
     row_wave_fence();
     sum = quad_sum(sum);
@@ -279,57 +276,73 @@ __global__ __launch_bounds__(LSR_ROW_THREADS) void lsr_distill_quad_kernel(
         p[4 * g + 2] = f.z;
         p[4 * g + 3] = f.w;
     }
-    // sums of e^z relative to m for what is listed and relative to m_r for the others (relative to m for all without rest)
+    // the others' maximum and sum of e^z relative to it (without an outcome for the rest: of all classes)
     float m_r = m;
     if (REST) {
         m_r = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < E; ++i)
-            if (!(p[i] > 0)) m_r = row_max(m_r, x[i]);
+        for (int i = 0; i < E; ++i) {
+            x[i] = p[i] > 0 ? -INFINITY : x[i];
+            m_r = row_max(m_r, x[i]);
+        }
         m_r = quad_max(m_r);
+        z_l = quad_sum(z_l);
     }
     const float unit_f = (float)unit, from = m_r > -INFINITY ? m_r : 0.0f;
-    float z_l = 0, z_r = 0;
+    float part = 0;
 #pragma unroll
     for (int i = 0; i < E; ++i) {
-        const bool in = REST && p[i] > 0;
-        x[i] = __builtin_amdgcn_exp2f((x[i] - (in ? m : from)) * unit_f);
-        if (in)
-            z_l += x[i];
-        else
-            z_r += x[i];
+        x[i] = __builtin_amdgcn_exp2f((x[i] - from) * unit_f);
+        part += x[i];
     }
-    z_l = quad_sum(z_l);
-    z_r = quad_sum(z_r);
-    const double shift = REST && z_r > 0 ? row_exp2(((double)m_r - m) * unit) : 1.0;
-    const double z = REST ? z_l + shift * z_r : z_r;
+    const double z_r = quad_sum(part);
+    const double shift = !REST ? 1.0 : z_r == 0 ? 0.0 : row_exp2(((double)m_r - m) * unit);
+    const double z = z_l + (z_r == 0 ? 0.0 : shift * z_r);
+    // NaN or +infinity among the scores: their exponentials, and with them the sum, are NaN
+    const bool nan = z != z, used = (w != 0) & (best > -INFINITY) & ((m > -INFINITY) | nan);
     double p_r = 0, rest_log = 0;
     if (REST) {
         rest_log = (double)rest[r];
         p_r = row_exp2(rest_log * ROW_LOG2E);
         sum += p_r;
     }
-    const double ln = row_log(q == 0 ? z : q == 1 ? sum : (double)z_r);
+    const double ln = row_log(q == 0 ? z : q == 1 ? sum : z_r);
     const double ln_z = quad_move<0x00>(ln), ln_s = quad_move<0x55>(ln), ln_r = quad_move<0xAA>(ln);
     if (live && q == 0) {
         double l = cross / sum + ln_z - ln_s;
         if (REST && p_r > 0) l += p_r / sum * (z_r > 0 ? rest_log - ln_r - ((double)m_r - m) * inv_t : INFINITY);
         loss[r] = used ? (nan ? NAN : (float)(w * temperature * temperature * l)) : 0.0f;
     }
-    if (!GRAD || !live) return;
+    if (!GRAD) return;
     const double scale = w * temperature;
     const float c_l = (float)(scale / z), c_p = (float)(scale / sum);
     const float c_r = REST ? (z_r > 0 ? (float)(scale * (shift / z - p_r / sum / z_r)) : 0.0f) : c_l;
+    if (REST) {
+        // the student's weights of the listed classes take the place of the teacher's, which are in registers now
+        row_wave_fence();
+        for (int j = q; j < k; j += 4) {
+            const int c = index[r * k + j];
+            if ((c >= 0) & (c < n_classes) & (values[r * k + j] > -INFINITY))
+                listed[slot][c] = __builtin_amdgcn_exp2f(((float)mine[c] - m) * unit_f);
+        }
+        row_wave_fence();
+    }
+    const bool plain = __all(used & !nan);
 #pragma unroll
     for (int g = 0; g < E / 4; ++g) {
+        const float4 f = REST ? own[g * 4] : make_float4(0, 0, 0, 0);
+        const float s[4] = {f.x, f.y, f.z, f.w};
         float d[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const int i = 4 * g + j;
-            d[j] = (REST && p[i] > 0 ? c_l : c_r) * x[i] - c_p * p[i];
-            d[j] = used ? (nan ? NAN : d[j]) : 0.0f;
+            d[j] = __builtin_fmaf(c_r, x[4 * g + j], -c_p * p[4 * g + j]);
+            if (REST) d[j] = __builtin_fmaf(c_l, s[j], d[j]);
         }
-        quad_store(grad + r * n_classes, n_classes, g, q, d);
+        if (!plain) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) d[j] = used ? (nan ? NAN : d[j]) : 0.0f;
+        }
+        if (live) quad_store(grad + r * n_classes, n_classes, g, q, d);
     }
 }
 

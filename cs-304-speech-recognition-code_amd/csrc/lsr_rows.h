@@ -177,18 +177,26 @@ __device__ __forceinline__ void quad_load(const typename row_type<DT>::type* row
 #pragma unroll
     for (int g = 0; g < E / 4; ++g) {
         const int c = g * 16 + q * 4;
-        row_four<T> f = {};
-        if (c < n_classes) {
-            if (c + 4 <= left) {
-                f = *(const row_four<T>*)(row + c);
-            } else {
-                for (int j = 0; j < 4 && c + j < n_classes; ++j) f.v[j] = row[c + j];
-            }
-        }
+        if (g * 16 + 16 <= n_classes) {                   // the same in all rows: no lane reaches the row's end
+            const row_four<T> f = *(const row_four<T>*)(row + c);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x[g * 4 + j] = c + j < n_classes ? (float)f.v[j] : -INFINITY;
+            for (int j = 0; j < 4; ++j) x[g * 4 + j] = (float)f.v[j];
+        } else {
+            row_four<T> f = {};
+            if (c < n_classes) {
+                if (c + 4 <= left) {
+                    f = *(const row_four<T>*)(row + c);
+                } else {
+                    for (int j = 0; j < 4 && c + j < n_classes; ++j) f.v[j] = row[c + j];
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[g * 4 + j] = c + j < n_classes ? (float)f.v[j] : -INFINITY;
+        }
     }
 }
+// -infinity for NaN, +0 for -0: the sum quietens a signalling NaN, a maximum passes over a quiet one
+__device__ __forceinline__ float row_clean(float x) { return fmaxf(x + 0.0f, -INFINITY); }
 
 // The run of four elements that register group g of lane q stands for, into a row of n_classes elements.
 template <typename T> __device__ __forceinline__ void quad_store(T* row, int n_classes, int g, int q, const float (&v)[4]) {
@@ -211,14 +219,14 @@ __device__ __forceinline__ void row_wave_fence() {
     __builtin_amdgcn_wave_barrier();
 }
 
-// An entry of a short row as a double in [2, 4): key and complemented class in the low 39 bits.  Doubles of one sign sort
-// like their bits, so one maximum and one minimum instruction order two entries.  An absent score gives QUAD_NONE + class
-// bits, below every entry.
-#define QUAD_NONE 0x4000000000000000ll
-__device__ __forceinline__ double quad_entry(uint32_t key, int cls) {
-    return __longlong_as_double(QUAD_NONE | (long long)key << 7 | (127 - cls));
+// An entry of a short row as a double in [2, 4): the score's key and the complemented class in the low 39 bits.  Doubles of
+// one sign sort like their bits, so one maximum and one minimum instruction order two entries.  An absent score, cleaned
+// to -infinity, has a key like any other, below those of all scores that are present.
+__device__ __forceinline__ double quad_entry(float x, int cls) {
+    const uint32_t u = __float_as_uint(x), key = u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
+    return __longlong_as_double(0x4000000000000000ll | (long long)key << 7 | (127 - cls));
 }
-__device__ __forceinline__ uint32_t quad_entry_key(double e) { return (uint32_t)(__double_as_longlong(e) >> 7); }
+__device__ __forceinline__ float quad_entry_value(double e) { return row_value((uint32_t)(__double_as_longlong(e) >> 7)); }
 __device__ __forceinline__ int quad_entry_class(double e) { return 127 - (int)(__double_as_longlong(e) & 127); }
 
 // larger one first
@@ -267,20 +275,45 @@ template <int E> __device__ __forceinline__ void quad_sort(double (&e)[E], int q
     for (int i = 0; i < E; ++i) e[i] = (e[i] < o[i]) != odd ? o[i] : e[i];
     quad_merge_lane(e);
 }
-// The first E of the quad's entries in descending order, the same in all four lanes.
-template <int E> __device__ __forceinline__ void quad_sort_head(double (&e)[E]) {
-    double o[E];
-    quad_sort_lane(e);
+// The first H of the quad's entries in descending order in e[0 ... H - 1], the same in all four lanes (H a power of two, at
+// most E): runs of H are sorted, then two at a time only the better half of them is kept and put in order again.
+template <int E, int H> __device__ __forceinline__ void quad_sort_head(double (&e)[E]) {
 #pragma unroll
-    for (int i = 0; i < E; ++i) o[i] = quad_move<QUAD_XOR1>(e[E - 1 - i]);
+    for (int g = 0; g < E; g += H) {
+        double s[H];
 #pragma unroll
-    for (int i = 0; i < E; ++i) e[i] = row_max(e[i], o[i]);
-    quad_merge_lane(e);
+        for (int i = 0; i < H; ++i) s[i] = e[g + i];
+        quad_sort_lane<H>(s);
 #pragma unroll
-    for (int i = 0; i < E; ++i) o[i] = quad_move<QUAD_XOR2>(e[E - 1 - i]);
+        for (int i = 0; i < H; ++i) e[g + i] = s[i];
+    }
+    double h[H], o[H];
 #pragma unroll
-    for (int i = 0; i < E; ++i) e[i] = row_max(e[i], o[i]);
-    quad_merge_lane(e);
+    for (int n = E / H; n > 1; n /= 2)
+#pragma unroll
+        for (int g = 0; g < n / 2; ++g) {
+#pragma unroll
+            for (int i = 0; i < H; ++i) h[i] = row_max(e[2 * g * H + i], e[(2 * g + 1) * H + H - 1 - i]);
+            quad_merge_lane<H>(h);
+#pragma unroll
+            for (int i = 0; i < H; ++i) e[g * H + i] = h[i];
+        }
+#pragma unroll
+    for (int i = 0; i < H; ++i) h[i] = e[i];
+#pragma unroll
+    for (int i = 0; i < H; ++i) o[i] = quad_move<QUAD_XOR1>(h[H - 1 - i]);
+#pragma unroll
+    for (int i = 0; i < H; ++i) h[i] = row_max(h[i], o[i]);
+    quad_merge_lane<H>(h);
+#pragma unroll
+    for (int i = 0; i < H; ++i) o[i] = quad_move<QUAD_XOR2>(h[H - 1 - i]);
+#pragma unroll
+    for (int i = 0; i < H; ++i) e[i] = row_max(h[i], o[i]);
+#pragma unroll
+    for (int i = 0; i < H; ++i) h[i] = e[i];
+    quad_merge_lane<H>(h);
+#pragma unroll
+    for (int i = 0; i < H; ++i) e[i] = h[i];
 }
 
 // the instantiation for a row's width: registers per lane
@@ -517,15 +550,13 @@ template <int W, int SIZE> struct team_list {
     uint64_t entry[SIZE];
     alignas(16) uint32_t group[ROW_GROUPS];
     int n;
-    uint32_t bound;
+    uint32_t bound;                                       // a key
 };
 
-// Collects the entries that reach the bound of kk; returns the bound as a score, -FLT_MAX when there are fewer groups with
-// a score and all present entries are collected.  `list.n` may exceed ROOM: then only some of them are there.
+// The groups' best scores of a row, and the row's.
 template <int DT, int W, int N, int SIZE>
-__device__ __forceinline__ float team_collect(team_row<DT, W, N>& row, int kk, team_list<W, SIZE>& list) {
-    using Row = team_row<DT, W, N>;
-    constexpr int THREADS = 64 * W, RUN = Row::RUN, PER = W == 1 ? 4 : 1;
+__device__ __forceinline__ float team_groups(team_row<DT, W, N>& row, team_list<W, SIZE>& list) {
+    constexpr int THREADS = 64 * W, RUN = team_row<DT, W, N>::RUN, PER = W == 1 ? 4 : 1;
     const int tid = threadIdx.x;
     float most[PER];
 #pragma unroll
@@ -538,11 +569,6 @@ __device__ __forceinline__ float team_collect(team_row<DT, W, N>& row, int kk, t
             for (int j = 0; j < RUN; ++j) most[i] = row_max(most[i], v[j]);
         }
     });
-    team_sync<W>();                                       // the list is free
-    if (tid == 0) {
-        list.n = 0;
-        list.bound = 0;
-    }
     if (W == 1) {
 #pragma unroll
         for (int i = 0; i < ROW_GROUPS / 64; ++i) list.group[i * 64 + tid] = row_key(most[i < PER ? i : 0]);
@@ -554,6 +580,17 @@ __device__ __forceinline__ float team_collect(team_row<DT, W, N>& row, int kk, t
         if (tid % LANES == 0) list.group[tid / LANES] = row_key(best);
     }
     team_sync<W>();
+    const uint4 o = *(const uint4*)&list.group[(tid & 63) * 4];         // every wavefront for itself
+    const uint32_t a = o.x > o.y ? o.x : o.y, b = o.z > o.w ? o.z : o.w;
+    const uint32_t best = (uint32_t)wave_max((uint64_t)(a > b ? a : b));
+    return best ? row_value(best) : -INFINITY;
+}
+// Collects the entries that reach the bound of kk; returns the bound as a score, -FLT_MAX when there are fewer groups with
+// a score and all present entries are collected.  `list.n` may exceed the list's size: then only some of them are there.
+template <int DT, int W, int N, int SIZE>
+__device__ __forceinline__ float team_collect(team_row<DT, W, N>& row, int kk, team_list<W, SIZE>& list) {
+    constexpr int RUN = team_row<DT, W, N>::RUN;
+    const int tid = threadIdx.x;
     if (tid < 64) {                                       // the largest number that kk groups reach, bit by bit
         const uint4 o = *(const uint4*)&list.group[tid * 4];
         uint32_t bound = 0;
@@ -564,7 +601,10 @@ __device__ __forceinline__ float team_collect(team_row<DT, W, N>& row, int kk, t
                               __popcll(__ballot(o.w >= b));
             if (reach >= kk) bound = b;
         }
-        if (tid == 0) list.bound = bound;
+        if (tid == 0) {
+            list.bound = bound;
+            list.n = 0;
+        }
     }
     team_sync<W>();
     const float bound = list.bound ? row_value(list.bound) : -3.402823466e38f;

@@ -33,20 +33,23 @@ __device__ __forceinline__ uint64_t sample_goal(float u, uint64_t sum) {
     return !(at > 0) ? 0 : at >= (double)sum ? sum - 1 : (uint64_t)at;
 }
 
-// The lowest entry of the shortest head of a list whose mass is at least `left`, eight bits at a time; `hist` has 256 places.
+// The lowest entry of the shortest head of a list whose mass is at least `left`, eight bits at a time from a histogram of
+// the entries that still match.  The search is over as soon as a digit's whole mass is needed; then the result, with zeros
+// in the digits that are left, lies below the entry.  `hist` has 257 places.
 template <int W>
-__device__ __forceinline__ uint64_t list_by_radix(const uint64_t* entry, const uint64_t* mass, int n, uint64_t left,
-                                                  uint64_t* hist, uint64_t* shared) {
+__device__ __forceinline__ uint64_t list_by_radix(const uint64_t* entry, const uint64_t* mass, int n, uint64_t left, uint64_t* hist) {
     constexpr int THREADS = 64 * W;
     const int tid = threadIdx.x;
-    uint64_t threshold = 0;
+    uint64_t found = 0;
+#pragma unroll 1
     for (int shift = 56; shift >= 0; shift -= 8) {
         team_sync<W>();
         for (int i = tid; i < 256; i += THREADS) hist[i] = 0;
         team_sync<W>();
+#pragma unroll 1
         for (int i = tid; i < n; i += THREADS) {
             const uint64_t e = entry[i];
-            if (shift == 56 || (e >> (shift + 8)) == (threshold >> (shift + 8)))
+            if (shift == 56 || (e >> (shift + 8)) == (found >> (shift + 8)))
                 atomicAdd((unsigned long long*)&hist[(e >> shift) & 255], (unsigned long long)mass[i]);
         }
         team_sync<W>();
@@ -58,17 +61,19 @@ __device__ __forceinline__ uint64_t list_by_radix(const uint64_t* entry, const u
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 if (run < left && left <= run + m[i]) {
-                    shared[0] = threshold | (uint64_t)(255 - 4 * tid - i) << shift;
                     hist[0] = left - run;
+                    hist[1] = left == run + m[i];
+                    hist[256] = found | (uint64_t)(255 - 4 * tid - i) << shift;
                 }
                 run += m[i];
             }
         }
         team_sync<W>();
-        threshold = shared[0];
+        found = hist[256];
         left = hist[0];
+        if (hist[1]) break;
     }
-    return threshold;
+    return found;
 }
 
 // A row in many passes over memory, by radix selection with weights: for rows that the fast form below does not take (an
@@ -160,8 +165,10 @@ __device__ __forceinline__ void sample_by_radix(const typename row_type<DT>::typ
 
 // Long rows, a team of W wavefronts per row (lsr_rows.h).
 //
-// With a top_k of at most LSR_MAX_TOP, only the first entries are weighed: they are collected as lsr_top_scores does it,
-// put in order by counting, and everything else happens among them.
+// With a top_k of at most LSR_MAX_TOP, only the first entries are weighed: they are collected as lsr_top_scores does it, put
+// in order by counting, and everything else happens among them (a radix selection by number, weight and class instead of
+// the counting was measured: 22 us against 15 for one row of 131072 and a top_k of 50).  A nucleus that looks short is
+// taken in the same way, with the weight of the whole row beside the list.
 //
 // Otherwise every class is weighed.  A cut by order is found from a histogram over the distance to the best score: the bin
 // in which the cut falls is collected and its entries counted against each other.  Then the weights of what is kept are
@@ -178,9 +185,10 @@ __global__ __launch_bounds__(64 * W) void lsr_sample_team_kernel(const typename 
     __shared__ team_list<W, ROOM> list;
     __shared__ uint64_t mass[BINS > STEPS ? BINS : STEPS];          // of a bin, of an entry of the list, of a step
     __shared__ int bin_n[BINS];
-    __shared__ uint64_t sorted[LSR_MAX_TOP], part[W], above, lowest, kept_sum;
+    __shared__ uint64_t sorted[257], part[W], above, lowest, kept_sum;
     __shared__ float part_f[W];
     __shared__ int cut_bin, n_kept;
+    constexpr int NUCLEUS = 128;                          // entries that a nucleus is first looked for in
     const row_exp2_t row_exp2;
     const int tid = threadIdx.x;
     const int64_t r = blockIdx.x;
@@ -194,97 +202,15 @@ __global__ __launch_bounds__(64 * W) void lsr_sample_team_kernel(const typename 
     const float u = uniform[r];
     const double unit = ROW_LOG2E / t;
 
-    if (top_k > 0 && top_k <= LSR_MAX_TOP && top_k < n_classes && t > 0) {
-        team_collect(row, top_k, list);
-        const int n = list.n;
-        if (n == 0) {
-            if (tid == 0) {
-                index[r] = -1;
-                logprob[r] = -INFINITY;
-            }
-            return;
-        }
-        if (n <= ROOM) {
-            for (int i = tid; i < n; i += THREADS) {
-                const uint64_t e = list.entry[i];
-                const int place = team_above(list, n, e);
-                if (place < LSR_MAX_TOP) sorted[place] = e;
-            }
-            team_sync<W>();
-            const int m = n < top_k ? n : top_k;
-            const float best = row_value((uint32_t)(sorted[0] >> 32));
-            if (best < INFINITY) {
-                if (tid < 64) {                           // lane l has the places 4 l ... 4 l + 3
-                    const float floor = min_p > 0 ? sample_floor(best, t, min_p) : -INFINITY;
-                    constexpr int FOUR = LSR_MAX_TOP / 64;
-                    uint64_t w[FOUR], own = 0;
-                    float v[FOUR];
-#pragma unroll
-                    for (int i = 0; i < FOUR; ++i) {
-                        const int place = tid * FOUR + i;
-                        v[i] = place < m ? row_value((uint32_t)(sorted[place] >> 32)) : -INFINITY;
-                        w[i] = row_fixed(row_exp2(((double)v[i] - best) * unit), a.magic);
-                        own += w[i];
-                    }
-                    uint64_t run = wave_running(own);
-                    const uint64_t target = sample_target(top_p, wave_last(run));
-                    run -= own;
-                    uint64_t sum = 0;
-                    int kept = 0;
-#pragma unroll
-                    for (int i = 0; i < FOUR; ++i) {      // kept: the weight ahead of it is short of the target
-                        const int place = tid * FOUR + i;
-                        const bool in = (place < m) & ((place == 0) | (run < target)) & (v[i] >= floor);
-                        run += w[i];
-                        sum += in ? w[i] : 0;
-                        kept += in;
-                        mass[place] = w[i];
-                    }
-                    sum = wave_sum(sum);
-                    kept = wave_sum(kept);
-                    if (tid == 0) {
-                        kept_sum = sum;
-                        n_kept = kept;
-                    }
-                }
-                team_sync<W>();
-                const int kept = n_kept;
-                const uint64_t goal = sample_goal(u, kept_sum);
-                for (int i = tid; i < kept; i += THREADS) {
-                    // weight of the kept entries of lower classes
-                    const uint32_t own = (uint32_t)sorted[i];
-                    uint64_t before = 0;
-                    int ahead = 0;
-#pragma unroll 8
-                    for (int j = 0; j < kept; ++j) {
-                        const bool lower = (uint32_t)sorted[j] > own;            // classes are complemented
-                        before += lower ? mass[j] : 0;
-                        ahead += lower;
-                    }
-                    if (goal == 0 ? ahead == 0 : before <= goal && goal < before + mass[i]) {
-                        const float v = row_value((uint32_t)(sorted[i] >> 32));
-                        index[r] = (int32_t)~own;
-                        logprob[r] = (float)(((double)v - best) / t - row_log((double)kept_sum * a.unit));
-                    }
-                }
-                return;
-            }
-        }
-    }
-
-    float most = -INFINITY;
-    row.template each<4>([&](int, const float(&v)[RUN], int) {
-#pragma unroll
-        for (int j = 0; j < RUN; ++j) most = row_max(most, v[j]);
-    });
-    const float best = team_max<W>(most, part_f);
+    const float best = team_groups(row, list);
     if (best == -INFINITY || !(t > 0)) {                  // nothing to draw from, or the best entry itself
         int at = 1 << 30;
-        row.template each<4>([&](int, const float(&v)[RUN], int c) {
+        if (best > -INFINITY)
+            row.template each<4>([&](int, const float(&v)[RUN], int c) {
 #pragma unroll
-            for (int j = 0; j < RUN; ++j)
-                if (v[j] == best) at = min(at, c + j);
-        });
+                for (int j = 0; j < RUN; ++j)
+                    if (v[j] == best) at = min(at, c + j);
+            });
         at = (int)~(uint32_t)team_max<W>((uint64_t)(uint32_t)~at, part);
         if (tid == 0) {
             index[r] = best == -INFINITY ? -1 : at;
@@ -296,6 +222,102 @@ __global__ __launch_bounds__(64 * W) void lsr_sample_team_kernel(const typename 
         sample_by_radix<DT, W>(mine, n_classes, best, t, top_k, top_p, min_p, u, a, mass, &above, index + r, logprob + r);
     };
     if (best == INFINITY) return slowly();
+
+    // few: a small top_k; nucleus: top_p alone, where it looks as if a short head will do: where the best scores of the
+    // groups hold that share of the row's weight, both in 32 bits
+    const bool cut = top_k > 0 && top_k < n_classes, few = cut && top_k <= LSR_MAX_TOP;
+    bool nucleus = !cut && top_p < 1;
+    if (nucleus) {
+        const float unit_f = (float)unit;
+        float guess = 0, head = 0;
+        row.template each<4>([&](int, const float(&v)[RUN], int) {
+#pragma unroll
+            for (int j = 0; j < RUN; ++j) guess += __builtin_amdgcn_exp2f((v[j] - best) * unit_f);
+        });
+        for (int i = tid; i < ROW_GROUPS; i += THREADS)
+            if (list.group[i]) head += __builtin_amdgcn_exp2f((row_value(list.group[i]) - best) * unit_f);
+        nucleus = team_sum<W>(head, part_f) >= (float)top_p * team_sum<W>(guess, part_f);
+    }
+    if (few || nucleus) {
+        const int want = few ? top_k : NUCLEUS < n_classes ? NUCLEUS : n_classes;
+        team_collect(row, want, list);
+        const int n = list.n;
+        if (n <= ROOM) {
+#pragma unroll 1
+            for (int i = tid; i < n; i += THREADS) {
+                const uint64_t e = list.entry[i];
+                const int place = team_above(list, n, e);
+                if (place < LSR_MAX_TOP) sorted[place] = e;
+            }
+            uint64_t all = 0;                             // weight of the row, where the list does not hold what top_p is a share of
+            if (nucleus) {
+                row.template each<2>([&](int, const float(&v)[RUN], int) {
+#pragma unroll
+                    for (int j = 0; j < RUN; ++j)
+                        all += (uint64_t)__double_as_longlong(row_exp2(((double)v[j] - best) * unit) + a.magic);
+                    all -= RUN * (uint64_t)__double_as_longlong(a.magic);
+                });
+                all = team_sum<W>(all, part);
+            }
+            team_sync<W>();
+            const int most = few ? top_k : LSR_MAX_TOP, m = n < most ? n : most;     // the list is the head of the row, all of it
+            if (tid < 64) {                               // lane l has the places 4 l ... 4 l + 3
+                const float floor = min_p > 0 ? sample_floor(best, t, min_p) : -INFINITY;
+                constexpr int FOUR = LSR_MAX_TOP / 64;
+                uint64_t w[FOUR], own = 0;
+                float v[FOUR];
+#pragma unroll
+                for (int i = 0; i < FOUR; ++i) {
+                    const int place = tid * FOUR + i;
+                    v[i] = place < m ? row_value((uint32_t)(sorted[place] >> 32)) : -INFINITY;
+                    w[i] = row_fixed(row_exp2(((double)v[i] - best) * unit), a.magic);
+                    own += w[i];
+                }
+                uint64_t run = wave_running(own);
+                const uint64_t listed = wave_last(run), target = sample_target(top_p, few ? listed : all);
+                run -= own;
+                uint64_t sum = 0;
+                int kept = 0;
+#pragma unroll
+                for (int i = 0; i < FOUR; ++i) {          // kept: the weight ahead of it is short of the target
+                    const int place = tid * FOUR + i;
+                    const bool in = (place < m) & ((place == 0) | (run < target)) & (v[i] >= floor);
+                    run += w[i];
+                    sum += in ? w[i] : 0;
+                    kept += in;
+                    mass[place] = w[i];
+                }
+                sum = wave_sum(sum);
+                kept = wave_sum(kept);
+                if (tid == 0) {
+                    kept_sum = sum;
+                    n_kept = few || listed >= target ? kept : 0;                 // 0: the list is too short for top_p
+                }
+            }
+            team_sync<W>();
+            const int kept = n_kept;
+            const uint64_t goal = sample_goal(u, kept_sum);
+#pragma unroll 1
+            for (int i = tid; i < kept; i += THREADS) {
+                // weight of the kept entries of lower classes
+                const uint32_t own = (uint32_t)sorted[i];
+                uint64_t before = 0;
+                int ahead = 0;
+#pragma unroll 8
+                for (int j = 0; j < kept; ++j) {
+                    const bool lower = (uint32_t)sorted[j] > own;                // classes are complemented
+                    before += lower ? mass[j] : 0;
+                    ahead += lower;
+                }
+                if (goal == 0 ? ahead == 0 : before <= goal && goal < before + mass[i]) {
+                    const float v = row_value((uint32_t)(sorted[i] >> 32));
+                    index[r] = (int32_t)~own;
+                    logprob[r] = (float)(((double)v - best) / t - row_log((double)kept_sum * a.unit));
+                }
+            }
+            if (kept > 0) return;
+        }
+    }
 
     float last = -INFINITY;                               // kept: above this score, or equal up to this class
     int last_class = -1;
@@ -317,15 +339,24 @@ __global__ __launch_bounds__(64 * W) void lsr_sample_team_kernel(const typename 
             lowest = ~0ull;
         }
         team_sync<W>();
-        row.template each<1>([&](int, const float(&v)[RUN], int c) {
+        if (by_weight) {                                  // what is cut or absent weighs nothing
+            row.template each<2>([&](int, const float(&v)[RUN], int c) {
+                float s[RUN];
 #pragma unroll
-            for (int j = 0; j < RUN; ++j)
-                if (keeps(v[j], c + j)) {
-                    const int b = bin_of(v[j]);
-                    atomicAdd(&bin_n[b], 1);
-                    if (by_weight) atomicAdd((unsigned long long*)&mass[b], (unsigned long long)weigh(v[j]));
+                for (int j = 0; j < RUN; ++j) s[j] = keeps(v[j], c + j) ? v[j] : -INFINITY;
+#pragma unroll
+                for (int j = 0; j < RUN; ++j) {
+                    const uint64_t m = weigh(s[j]);
+                    if (m) atomicAdd((unsigned long long*)&mass[bin_of(s[j])], (unsigned long long)m);
                 }
-        });
+            });
+        } else {
+            row.template each<4>([&](int, const float(&v)[RUN], int) {
+#pragma unroll
+                for (int j = 0; j < RUN; ++j)
+                    if (v[j] > -INFINITY) atomicAdd(&bin_n[bin_of(v[j])], 1);
+            });
+        }
         team_sync<W>();
         uint64_t own = 0;
 #pragma unroll
@@ -356,20 +387,25 @@ __global__ __launch_bounds__(64 * W) void lsr_sample_team_kernel(const typename 
         team_sync<W>();
         const int b = cut_bin;
         const uint64_t ahead = above;
-        if (bin_n[b] > ROOM) return slowly();
         row.template each<4>([&](int, const float(&v)[RUN], int c) {
 #pragma unroll
             for (int j = 0; j < RUN; ++j)
-                if (keeps(v[j], c + j) && bin_of(v[j]) == b) list.entry[atomicAdd(&list.n, 1)] = row_entry(row_key(v[j]), c + j);
+                if (keeps(v[j], c + j) && bin_of(v[j]) == b) {
+                    const int at = atomicAdd(&list.n, 1);
+                    if (at < ROOM) list.entry[at] = row_entry(row_key(v[j]), c + j);
+                }
         });
         team_sync<W>();
         const int n = list.n;
+        if (n > ROOM) return slowly();
         for (int i = tid; i < n; i += THREADS) mass[i] = by_weight ? weigh(row_value((uint32_t)(list.entry[i] >> 32))) : 1;
         team_sync<W>();
         if (n > (THREADS < 256 ? THREADS : 256)) {        // many: radix selection in the list
-            const uint64_t least = list_by_radix<W>(list.entry, mass, n, target - ahead, sorted, &lowest);
-            last = row_value((uint32_t)(least >> 32));
-            last_class = (int)~(uint32_t)least;
+            const uint64_t least = list_by_radix<W>(list.entry, mass, n, target - ahead, sorted);
+            // a threshold between entries rather than one of them: its class may be any number, its key below every score's
+            const uint32_t key = (uint32_t)(least >> 32), beyond = ~(uint32_t)least;
+            last = key > 0x007fffffu ? row_value(key) : -3.402823466e38f;
+            last_class = key > 0x007fffffu && beyond < (uint32_t)n_classes ? (int)beyond : n_classes;
             continue;
         }
         for (int i = tid; i < n; i += THREADS) {
@@ -394,22 +430,27 @@ __global__ __launch_bounds__(64 * W) void lsr_sample_team_kernel(const typename 
     team_sync<W>();
     for (int i = tid; i < row.steps; i += THREADS) mass[i] = 0;
     team_sync<W>();
-    const bool all = last == -INFINITY;
     const uint64_t zero = (uint64_t)__double_as_longlong(a.magic);
+    const bool all = last == -INFINITY;
     row.template each<2>([&](int step, const float(&v)[RUN], int c) {
         uint64_t sum = 0;
-        if (all) {                                        // what is absent weighs nothing by itself
+        if (all) {                                        // what is absent weighs nothing
 #pragma unroll
             for (int j = 0; j < RUN; ++j)
                 sum += (uint64_t)__double_as_longlong(row_exp2(((double)v[j] - best) * unit) + a.magic);
             sum -= RUN * zero;
         } else {
-            bool any = false;
+            float s[RUN], high = -INFINITY;
 #pragma unroll
-            for (int j = 0; j < RUN; ++j) any |= keeps(v[j], c + j);
-            if (any) {
+            for (int j = 0; j < RUN; ++j) {
+                s[j] = keeps(v[j], c + j) ? v[j] : -INFINITY;
+                high = row_max(high, s[j]);
+            }
+            if (high > -INFINITY) {
 #pragma unroll
-                for (int j = 0; j < RUN; ++j) sum += keeps(v[j], c + j) ? weigh(v[j]) : 0;
+                for (int j = 0; j < RUN; ++j)
+                    sum += (uint64_t)__double_as_longlong(row_exp2(((double)s[j] - best) * unit) + a.magic);
+                sum -= RUN * zero;
             }
         }
         sum = wave_sum(sum);
@@ -499,7 +540,7 @@ __global__ __launch_bounds__(LSR_ROW_THREADS) void lsr_sample_quad_kernel(const 
     float best = -INFINITY;
 #pragma unroll
     for (int i = 0; i < E; ++i) {
-        x[i] = x[i] > -INFINITY ? x[i] : -INFINITY;       // NaN is absent
+        x[i] = row_clean(x[i]);
         best = row_max(best, x[i]);
     }
     best = quad_max(best);
@@ -573,9 +614,10 @@ __global__ __launch_bounds__(LSR_ROW_THREADS) void lsr_sample_quad_kernel(const 
     }
     double total = 0;
     double lane[E / 4];
+    if (__any(min_p > 0)) {
 #pragma unroll
-    for (int i = 0; i < E; ++i)
-        if (x[i] < floor) w[i] = 0;
+        for (int i = 0; i < E; ++i) w[i] = x[i] < floor ? 0.0 : w[i];
+    }
 #pragma unroll
     for (int g = 0; g < E / 4; ++g) {
         lane[g] = (w[4 * g] + w[4 * g + 1]) + (w[4 * g + 2] + w[4 * g + 3]);

@@ -52,17 +52,19 @@ __global__ __launch_bounds__(64 * W) void lsr_top_team_kernel(const typename row
                                                               float* __restrict__ values, int32_t* __restrict__ index,
                                                               float* __restrict__ rest) {
     using Row = team_row<DT, W, N>;
-    constexpr int THREADS = 64 * W, RUN = Row::RUN, ROOM = W == 1 ? 1024 : 2048;
+    constexpr int THREADS = 64 * W, RUN = Row::RUN, ROOM = W == 1 ? 512 : 2048;
     __shared__ team_list<W, ROOM> list;
     __shared__ int hist[256];
     __shared__ uint64_t one;
-    __shared__ float part[W], tail[REST ? ROOM : 1], best, high;
+    __shared__ uint64_t sorted[ROOM];                     // by place: the list itself is in the order in which it was filled
+    __shared__ float part[W];
     const int tid = threadIdx.x;
     const int64_t r = blockIdx.x;
     const int kk = k + (REST ? 1 : 0);                    // the first entry of the rest as well
     Row row;
     row.open(scores + r * row_stride, n_classes);
     row.arrive();
+    team_groups(row, list);
     float bound = team_collect(row, kk, list);
     int n = list.n, bound_class = -1;                     // collected: above the bound, or equal up to this class
     bool equal = true;                                    // every score that equals the bound is collected
@@ -82,46 +84,26 @@ __global__ __launch_bounds__(64 * W) void lsr_top_team_kernel(const typename row
         team_sync<W>();
         n = list.n;
     }
-    float sum = 0.0f;
-    if (tid == 0) {
-        best = 0.0f;
-        high = -INFINITY;
+    team_sync<W>();
+    for (int i = tid; i < n; i += THREADS) {
+        const uint64_t e = list.entry[i];
+        sorted[team_above(list, n, e)] = e;
     }
     team_sync<W>();
-    int place[ROOM / THREADS];
-#pragma unroll
-    for (int i = 0; i < ROOM / THREADS; ++i) {
-        const int at = i * THREADS + tid;
-        place[i] = 1 << 30;
-        if (at >= n) continue;
-        const uint64_t e = list.entry[at];
-        const float v = row_value((uint32_t)(e >> 32));
-        place[i] = team_above(list, n, e);
-        if (place[i] < k) {
-            values[r * k + place[i]] = v;
-            index[r * k + place[i]] = (int32_t)~(uint32_t)e;
-        }
-        if (REST && place[i] == 0) best = v;
-        if (REST && place[i] == k) high = v;
-    }
-    for (int i = n + tid; i < k; i += THREADS) {          // places without an entry
-        values[r * k + i] = -INFINITY;
-        index[r * k + i] = -1;
+    for (int i = tid; i < k; i += THREADS) {              // places without an entry: -infinity, -1
+        const uint64_t e = i < n ? sorted[i] : 0;
+        values[r * k + i] = e ? row_value((uint32_t)(e >> 32)) : -INFINITY;
+        index[r * k + i] = e ? (int32_t)~(uint32_t)e : -1;
     }
     if (!REST) return;
-    team_sync<W>();
     // relative to the highest score of the rest: relative to the row's best it could underflow to nothing
-    const float from = high, unit = inv_t * 1.44269504f;
-#pragma unroll
-    for (int i = 0; i < ROOM / THREADS; ++i) {
-        const int at = i * THREADS + tid;
-        if (at >= n || place[i] < k) continue;
-        const float v = row_value((uint32_t)(list.entry[at] >> 32));
-        // by place: the list itself is in the order in which it was filled, which is not the same every time
-        tail[place[i]] = v == from ? 1.0f : __builtin_amdgcn_exp2f((v - from) * unit);
+    const float from = n > k ? row_value((uint32_t)(sorted[k] >> 32)) : -INFINITY, unit = inv_t * 1.44269504f;
+    const float best = n > 0 ? row_value((uint32_t)(sorted[0] >> 32)) : 0.0f;
+    float sum = 0.0f;
+    for (int i = k + tid; i < n; i += THREADS) {
+        const float v = row_value((uint32_t)(sorted[i] >> 32));
+        sum += v == from ? 1.0f : __builtin_amdgcn_exp2f((v - from) * unit);
     }
-    team_sync<W>();
-    for (int i = k + tid; i < n; i += THREADS) sum += tail[i];
     if (from > -INFINITY) {
         row.next_pass();
         if (equal) {
@@ -159,8 +141,8 @@ static void lsr_top_team(hipStream_t stream, const void* scores_d, int64_t n_row
 }
 
 // Short rows (at most LSR_QUAD_CLASSES classes), a quad per row: the entries are sorted by a network over the quad's
-// registers; for k <= E only the first E places are merged, which drops half of every exchange between lanes.
-template <int DT, int E, bool HEAD, bool REST>
+// registers.  HEAD: the number of places that are put in order, 0 for all (k > E).
+template <int DT, int E, int HEAD, bool REST>
 __global__ __launch_bounds__(LSR_ROW_THREADS) void lsr_top_quad_kernel(const typename row_type<DT>::type* __restrict__ scores,
                                                                        int64_t n_rows, int n_classes, int64_t row_stride, int k,
                                                                        float inv_t, float* __restrict__ values,
@@ -174,34 +156,32 @@ __global__ __launch_bounds__(LSR_ROW_THREADS) void lsr_top_quad_kernel(const typ
     double e[E];
 #pragma unroll
     for (int i = 0; i < E; ++i) {
-        x[i] = x[i] > -INFINITY ? x[i] : -INFINITY;      // NaN is absent
-        e[i] = quad_entry(row_key(x[i]), quad_class(i, q));
+        x[i] = row_clean(x[i]);
+        e[i] = quad_entry(x[i], quad_class(i, q));
     }
-    if (HEAD)
-        quad_sort_head<E>(e);
+    if constexpr (HEAD > 0)
+        quad_sort_head<E, HEAD>(e);
     else
         quad_sort<E>(e, q);
     double least = 3.9;                                   // entry at place k - 1
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
+    for (int i = 0; i < (HEAD ? HEAD : E); ++i) {
         const int place = HEAD ? i : q * E + i;
         if (REST) least = place == k - 1 ? e[i] : least;
         // with HEAD all lanes hold the same places: lane q writes the places that are q modulo 4
         if (live && place < k && (!HEAD || (place & 3) == q)) {
-            const uint32_t key = quad_entry_key(e[i]);
-            values[r * k + place] = key ? row_value(key) : -INFINITY;
-            index[r * k + place] = key ? quad_entry_class(e[i]) : -1;
+            const float v = quad_entry_value(e[i]);
+            values[r * k + place] = v;
+            index[r * k + place] = v > -INFINITY ? quad_entry_class(e[i]) : -1;
         }
     }
     if (!REST) return;
     if (!HEAD) least = quad_min(least);
     // the best entry is at place 0
     const double top = HEAD ? e[0] : quad_move<0x00>(e[0]);
-    const uint32_t best_key = quad_entry_key(top);
-    const float best = best_key ? row_value(best_key) : 0.0f;
+    const float best = quad_entry_value(top);
     // relative to the highest score of the rest: relative to the row's best it could underflow to nothing
-    const uint32_t last_key = quad_entry_key(least);
-    const float last = last_key ? row_value(last_key) : -INFINITY;
+    const float last = quad_entry_value(least);
     const int last_class = quad_entry_class(least);
     float high = -INFINITY;
 #pragma unroll
@@ -214,7 +194,7 @@ __global__ __launch_bounds__(LSR_ROW_THREADS) void lsr_top_quad_kernel(const typ
     float sum = 0.0f;
     const float unit = inv_t * 1.44269504f;
 #pragma unroll
-    for (int i = 0; i < E; ++i) sum += x[i] == high ? 1.0f : __builtin_amdgcn_exp2f((x[i] - high) * unit);
+    for (int i = 0; i < E; ++i) sum += __builtin_amdgcn_exp2f(fminf((x[i] - high) * unit, 0.0f));   // 1 for infinity - infinity
     sum = quad_sum(sum);
     if (live && q == 0)
         rest[r] = high > -INFINITY ? (high == best ? 0.0f : (high - best) * inv_t) + logf(sum) : -INFINITY;
@@ -228,10 +208,13 @@ static void lsr_top_quad(hipStream_t stream, const void* scores_d, int64_t n_row
 #define LAUNCH(HEAD, REST)                                                                                                   \
     hipLaunchKernelGGL((lsr_top_quad_kernel<DT, E, HEAD, REST>), grid, dim3(LSR_ROW_THREADS), 0, stream, scores, n_rows,       \
                        n_classes, row_stride, k, inv_t, values_d, index_d, rest_d)
-    if (k <= E) {
-        if (rest_d) LAUNCH(true, true); else LAUNCH(true, false);
+    constexpr int HALF = E > 8 ? 8 : E;
+    if (k <= HALF) {
+        if (rest_d) LAUNCH(HALF, true); else LAUNCH(HALF, false);
+    } else if (k <= E) {
+        if (rest_d) LAUNCH(E, true); else LAUNCH(E, false);
     } else {
-        if (rest_d) LAUNCH(false, true); else LAUNCH(false, false);
+        if (rest_d) LAUNCH(0, true); else LAUNCH(0, false);
     }
 #undef LAUNCH
 }
