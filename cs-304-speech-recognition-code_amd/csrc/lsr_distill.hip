@@ -216,7 +216,8 @@ __global__ __launch_bounds__(64 * W) void lsr_distill_team_kernel(
 // With z = (x - m) / T, y = (t - best) / T, S the sum of the teacher's weights e^y and of e^rest:
 //   KL = 1/S sum_j e^{y_j} (y_j - z_j) + ln Z - ln S + p_R (rest - ln q_R - ln Z),
 // one logarithm instruction sequence for Z, S and the rest together, a lane each.
-template <int DT, int E, bool REST, bool GRAD>
+// HELD: entries of the list that a lane keeps in registers (k <= 4 HELD), 0 to read them again in each of the three loops.
+template <int DT, int E, int HELD, bool REST, bool GRAD>
 __global__ __launch_bounds__(LSR_ROW_THREADS) void lsr_distill_quad_kernel(
     const typename row_type<DT>::type* __restrict__ scores, int64_t n_rows, int n_classes, int64_t row_stride,
     const float* __restrict__ values, const int32_t* __restrict__ index, int k, const float* __restrict__ rest,
@@ -230,8 +231,40 @@ __global__ __launch_bounds__(LSR_ROW_THREADS) void lsr_distill_quad_kernel(
     const bool live = row < n_rows;
     const int64_t r = live ? row : n_rows - 1;            // every lane takes part in the exchanges
     const auto* mine = scores + r * row_stride;
+    using T = typename row_type<DT>::type;
+    // class (-1: absent), value and student's score of an entry
+    int held_c[HELD ? HELD : 1];
+    float held_v[HELD ? HELD : 1];
+    T held_s[HELD ? HELD : 1];
+    auto entry = [&](int j, int& c, float& v) {
+        c = j < k ? index[r * k + j] : -1;
+        v = j < k ? values[r * k + j] : -INFINITY;
+        c = ((c >= 0) & (c < n_classes) & (v > -INFINITY)) ? c : -1;
+    };
+    if (HELD) {
+#pragma unroll
+        for (int i = 0; i < HELD; ++i) entry(q + 4 * i, held_c[i], held_v[i]);
+    }
     float x[E];
     quad_load<DT, E>(mine, n_classes, (n_rows - 1 - r) * row_stride + n_classes, q, x);
+    if (HELD) {
+#pragma unroll
+        for (int i = 0; i < HELD; ++i) held_s[i] = mine[held_c[i] < 0 ? 0 : held_c[i]];
+    }
+    auto each_entry = [&](auto f) {                       // f(class, value, student's score) for the entries that are there
+        if (HELD) {
+#pragma unroll
+            for (int i = 0; i < HELD; ++i)
+                if (held_c[i] >= 0) f(held_c[i], held_v[i], (float)held_s[i]);
+        } else {
+            for (int j = q; j < k; j += 4) {
+                int c;
+                float v;
+                entry(j, c, v);
+                if (c >= 0) f(c, v, (float)mine[c]);
+            }
+        }
+    };
     float4* own = (float4*)&listed[slot][q * 4];
 #pragma unroll
     for (int g = 0; g < E / 4; ++g) own[g * 4] = make_float4(0, 0, 0, 0);
@@ -242,20 +275,12 @@ __global__ __launch_bounds__(LSR_ROW_THREADS) void lsr_distill_quad_kernel(
     for (int i = 0; i < E; ++i) m = row_max(m, x[i]);
     m = quad_max(m);
     float best = -INFINITY;
-    for (int j = q; j < k; j += 4) {
-        const int c = index[r * k + j];
-        const float v = values[r * k + j];
-        if ((c >= 0) & (c < n_classes) & (v > best)) best = v;
-    }
+    each_entry([&](int, float v, float) { best = row_max(best, v); });
     best = quad_max(best);
     const double w = weight ? (double)weight[r] : 1.0;
     // sums over the list: the teacher's weights, those times (y - z), the student's weights of the listed classes
     double sum = 0, cross = 0, z_l = 0;
-    for (int j = q; j < k; j += 4) {
-        const int c = index[r * k + j];
-        const float v = values[r * k + j];
-        if (c < 0 || c >= n_classes || !(v > -INFINITY)) continue;
-        const float s = (float)mine[c];
+    each_entry([&](int c, float v, float s) {
         const double y = v == best ? 0.0 : ((double)v - best) * unit, z = ((double)s - m) * unit;
         const double p = row_exp2(y);
         sum += p;
@@ -263,7 +288,7 @@ __global__ __launch_bounds__(LSR_ROW_THREADS) void lsr_distill_quad_kernel(
         // at least the smallest normal number: what is in the list is what is not 0; the first to find 0 counts the class
         const float old = atomicAdd(&listed[slot][c], fmaxf((float)p, 1.17549435e-38f));
         if (REST && old == 0) z_l += s < INFINITY ? row_exp2(z) : NAN;
-    }
+    });
     row_wave_fence();
     sum = quad_sum(sum);
     cross = quad_sum(cross) * (1.0 / ROW_LOG2E);
@@ -320,11 +345,7 @@ __global__ __launch_bounds__(LSR_ROW_THREADS) void lsr_distill_quad_kernel(
     if (REST) {
         // the student's weights of the listed classes take the place of the teacher's, which are in registers now
         row_wave_fence();
-        for (int j = q; j < k; j += 4) {
-            const int c = index[r * k + j];
-            if ((c >= 0) & (c < n_classes) & (values[r * k + j] > -INFINITY))
-                listed[slot][c] = __builtin_amdgcn_exp2f(((float)mine[c] - m) * unit_f);
-        }
+        each_entry([&](int c, float, float s) { listed[slot][c] = __builtin_amdgcn_exp2f((s - m) * unit_f); });
         row_wave_fence();
     }
     const bool plain = __all(used & !nan);
@@ -354,14 +375,17 @@ static void lsr_distill_quad(hipStream_t stream, const void* scores_d, int64_t n
     auto* grad = (typename row_type<DT>::type*)grad_d;
     const dim3 grid((unsigned)((n_rows + LSR_QUAD_ROWS - 1) / LSR_QUAD_ROWS));
 #define LAUNCH(REST, GRAD)                                                                                                   \
-    hipLaunchKernelGGL((lsr_distill_quad_kernel<DT, E, REST, GRAD>), grid, dim3(LSR_ROW_THREADS), 0, stream, scores, n_rows,   \
+    if (k <= 8) LAUNCH_HELD(2, REST, GRAD); else LAUNCH_HELD(0, REST, GRAD)
+#define LAUNCH_HELD(HELD, REST, GRAD)                                                                                        \
+    hipLaunchKernelGGL((lsr_distill_quad_kernel<DT, E, HELD, REST, GRAD>), grid, dim3(LSR_ROW_THREADS), 0, stream, scores, n_rows,   \
                        n_classes, row_stride, values_d, index_d, k, rest_d, temperature, weight_d, loss_d, grad)
     if (rest_d) {
-        if (grad_d) LAUNCH(true, true); else LAUNCH(true, false);
+        if (grad_d) { LAUNCH(true, true); } else { LAUNCH(true, false); }
     } else {
-        if (grad_d) LAUNCH(false, true); else LAUNCH(false, false);
+        if (grad_d) { LAUNCH(false, true); } else { LAUNCH(false, false); }
     }
 #undef LAUNCH
+#undef LAUNCH_HELD
 }
 
 template <int DT, int W, int N>
