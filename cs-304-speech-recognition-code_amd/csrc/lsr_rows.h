@@ -587,8 +587,10 @@ __device__ __forceinline__ float team_groups(team_row<DT, W, N>& row, team_list<
 }
 // Collects the entries that reach the bound of kk; returns the bound as a score, -FLT_MAX when there are fewer groups with
 // a score and all present entries are collected.  `list.n` may exceed the list's size: then only some of them are there.
-template <int DT, int W, int N, int SIZE>
-__device__ __forceinline__ float team_collect(team_row<DT, W, N>& row, int kk, team_list<W, SIZE>& list) {
+// SUM: also this thread's sum of e^((x - bound) unit ln 2) over what stays below the bound, in the same pass; NaN where the
+// thread has seen one.
+template <bool SUM, int DT, int W, int N, int SIZE>
+__device__ __forceinline__ float team_collect(team_row<DT, W, N>& row, int kk, team_list<W, SIZE>& list, float unit, float& below) {
     constexpr int RUN = team_row<DT, W, N>::RUN;
     const int tid = threadIdx.x;
     if (tid < 64) {                                       // the largest number that kk groups reach, bit by bit
@@ -610,20 +612,30 @@ __device__ __forceinline__ float team_collect(team_row<DT, W, N>& row, int kk, t
     const float bound = list.bound ? row_value(list.bound) : -3.402823466e38f;
     row.next_pass();
     row.template each<4>([&](int, const float(&v)[RUN], int c) {
-        float high = v[0];
+        bool any = false;
 #pragma unroll
-        for (int j = 1; j < RUN; ++j) high = row_max(high, v[j]);
-        if (high >= bound) {
+        for (int j = 0; j < RUN; ++j) any |= v[j] >= bound;
+        if (any) {
 #pragma unroll
-            for (int j = 0; j < RUN; ++j)
+            for (int j = 0; j < RUN; ++j) {
                 if (v[j] >= bound) {
                     const int at = atomicAdd(&list.n, 1);
                     if (at < SIZE) list.entry[at] = row_entry(row_key(v[j]), c + j);
                 }
+                if (SUM) below += v[j] < bound ? __builtin_amdgcn_exp2f((v[j] - bound) * unit) : 0.0f;
+            }
+        } else if (SUM) {
+#pragma unroll
+            for (int j = 0; j < RUN; ++j) below += __builtin_amdgcn_exp2f((v[j] - bound) * unit);
         }
     });
     team_sync<W>();
     return bound;
+}
+template <int DT, int W, int N, int SIZE>
+__device__ __forceinline__ float team_collect(team_row<DT, W, N>& row, int kk, team_list<W, SIZE>& list) {
+    float none = 0;
+    return team_collect<false>(row, kk, list, 0.0f, none);
 }
 // how many of the list's first n entries are above e
 template <int W, int SIZE> __device__ __forceinline__ int team_above(const team_list<W, SIZE>& list, int n, uint64_t e) {

@@ -65,7 +65,9 @@ __global__ __launch_bounds__(64 * W) void lsr_top_team_kernel(const typename row
     row.open(scores + r * row_stride, n_classes);
     row.arrive();
     team_groups(row, list);
-    float bound = team_collect(row, kk, list);
+    const float unit = inv_t * 1.44269504f;
+    float below = 0.0f;
+    float bound = team_collect<REST>(row, kk, list, unit, below);
     int n = list.n, bound_class = -1;                     // collected: above the bound, or equal up to this class
     bool equal = true;                                    // every score that equals the bound is collected
     if (n > ROOM) {
@@ -97,25 +99,24 @@ __global__ __launch_bounds__(64 * W) void lsr_top_team_kernel(const typename row
     }
     if (!REST) return;
     // relative to the highest score of the rest: relative to the row's best it could underflow to nothing
-    const float from = n > k ? row_value((uint32_t)(sorted[k] >> 32)) : -INFINITY, unit = inv_t * 1.44269504f;
+    const float from = n > k ? row_value((uint32_t)(sorted[k] >> 32)) : -INFINITY;
     const float best = n > 0 ? row_value((uint32_t)(sorted[0] >> 32)) : 0.0f;
     float sum = 0.0f;
     for (int i = k + tid; i < n; i += THREADS) {
         const float v = row_value((uint32_t)(sorted[i] >> 32));
         sum += v == from ? 1.0f : __builtin_amdgcn_exp2f((v - from) * unit);
     }
+    // a NaN among the scores, absent like -infinity, spoils the sum of the pass that collected: once more, one by one
+    const bool spoilt = equal && team_max<W>(below != below ? 1.0f : 0.0f, part) > 0;
     if (from > -INFINITY) {
-        row.next_pass();
-        if (equal) {
-            row.template each<4>([&](int, const float(&v)[RUN], int) {
-#pragma unroll
-                for (int j = 0; j < RUN; ++j) sum += v[j] < bound ? __builtin_amdgcn_exp2f((v[j] - from) * unit) : 0.0f;
-            });
+        if (equal && !spoilt) {                                      // relative to the bound, which an entry of the rest reaches
+            if (below > 0) sum += below * __builtin_amdgcn_exp2f((bound - from) * unit);
         } else {
+            row.next_pass();
             row.template each<4>([&](int, const float(&v)[RUN], int c) {
 #pragma unroll
                 for (int j = 0; j < RUN; ++j)
-                    if (v[j] < bound || (v[j] == bound && c + j > bound_class))
+                    if (v[j] < bound || (!equal && v[j] == bound && c + j > bound_class))
                         sum += v[j] == from ? 1.0f : __builtin_amdgcn_exp2f((v[j] - from) * unit);
             });
         }
