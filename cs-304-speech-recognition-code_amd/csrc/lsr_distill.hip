@@ -107,7 +107,7 @@ __global__ __launch_bounds__(64 * W) void lsr_distill_team_kernel(
     row.arrive();
     // the runs of the row without the listed classes
     auto blank = [&](int step, uint4& u) {
-        const int c = Row::first_class(step);
+        const int c = row.first_class(step);
         uint32_t b = map[(c & (MAP - 1)) >> 5] >> (c & 31) & ((1u << RUN) - 1);
         if (b == 0) return;
         if (n_classes > MAP) {                            // the bit may be another class's
@@ -140,7 +140,7 @@ __global__ __launch_bounds__(64 * W) void lsr_distill_team_kernel(
             if (REST && !N) blank(step, u);
             float v[RUN];
             Row::decode(u, v);
-            f(v, Row::first_class(step));
+            f(v, row.first_class(step));
         });
     };
     float high = -INFINITY;

@@ -421,14 +421,14 @@ template <int DT, int W, int N> struct team_row {
     struct __attribute__((packed, aligned(sizeof(T)))) run { uint32_t w[4]; };
 
     const T* row;
-    int n_classes, steps;
+    int n_classes, steps, thread;
     uint4 kept[N ? N : 1];
 
     static __device__ __forceinline__ uint4 nothing() {   // a run of -infinity
         const uint32_t w = DT == ROW_F32 ? 0xff800000u : DT == ROW_F16 ? 0xfc00fc00u : 0xff80ff80u;
         return make_uint4(w, w, w, w);
     }
-    static __device__ __forceinline__ int first_class(int step) { return step * STEP + (int)threadIdx.x * RUN; }
+    __device__ __forceinline__ int first_class(int step) const { return step * STEP + thread * RUN; }
 
     // the run of the row's last classes, one element at a time
     __device__ __forceinline__ uint4 read_end(int c) const {
@@ -466,13 +466,28 @@ template <int DT, int W, int N> struct team_row {
         row = r;
         n_classes = classes;
         steps = (classes + STEP - 1) / STEP;
+        thread = threadIdx.x;
         if (N) {
 #pragma unroll
             for (int i = 0; i < (N ? N : 1); ++i) kept[i] = read(i);
         }
     }
+    // each_run of a kept row, and right behind each run the request for the same run of the next row
+    template <typename F> __device__ __forceinline__ void each_run_then(const T* next, F f) {
+        row = next;
+#pragma unroll
+        for (int i = 0; i < (N ? N : 1); ++i) {
+            f(i, kept[i]);
+            asm volatile("" ::: "memory");               // the load stays behind the run's last use
+            __builtin_amdgcn_sched_barrier(0);
+            kept[i] = read(i);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
     // waits for the row that `open` has requested
     __device__ __forceinline__ void arrive() {
+        // the classes of all runs would otherwise be computed once, before a loop over rows, and kept in registers
+        asm volatile("" : "+v"(thread));
         if (N) {
 #pragma unroll
             for (int i = 0; i < (N ? N : 1); ++i) kept[i] = settle(i, kept[i]);
@@ -589,8 +604,10 @@ __device__ __forceinline__ float team_groups(team_row<DT, W, N>& row, team_list<
 // a score and all present entries are collected.  `list.n` may exceed the list's size: then only some of them are there.
 // SUM: also this thread's sum of e^((x - bound) unit ln 2) over what stays below the bound, in the same pass; NaN where the
 // thread has seen one.
+// A kept row is asked for the next row, `next`, on the way.
 template <bool SUM, int DT, int W, int N, int SIZE>
-__device__ __forceinline__ float team_collect(team_row<DT, W, N>& row, int kk, team_list<W, SIZE>& list, float unit, float& below) {
+__device__ __forceinline__ float team_collect(team_row<DT, W, N>& row, int kk, team_list<W, SIZE>& list, float unit, float& below,
+                                              const typename row_type<DT>::type* next) {
     constexpr int RUN = team_row<DT, W, N>::RUN;
     const int tid = threadIdx.x;
     if (tid < 64) {                                       // the largest number that kk groups reach, bit by bit
@@ -611,7 +628,10 @@ __device__ __forceinline__ float team_collect(team_row<DT, W, N>& row, int kk, t
     team_sync<W>();
     const float bound = list.bound ? row_value(list.bound) : -3.402823466e38f;
     row.next_pass();
-    row.template each<4>([&](int, const float(&v)[RUN], int c) {
+    auto take = [&](int step, const uint4& packed) {
+        float v[RUN];
+        team_row<DT, W, N>::decode(packed, v);
+        const int c = row.first_class(step);
         bool any = false;
 #pragma unroll
         for (int j = 0; j < RUN; ++j) any |= v[j] >= bound;
@@ -628,14 +648,18 @@ __device__ __forceinline__ float team_collect(team_row<DT, W, N>& row, int kk, t
 #pragma unroll
             for (int j = 0; j < RUN; ++j) below += __builtin_amdgcn_exp2f((v[j] - bound) * unit);
         }
-    });
+    };
+    if (N)
+        row.each_run_then(next, take);
+    else
+        row.template each_run<4>(take);
     team_sync<W>();
     return bound;
 }
 template <int DT, int W, int N, int SIZE>
 __device__ __forceinline__ float team_collect(team_row<DT, W, N>& row, int kk, team_list<W, SIZE>& list) {
     float none = 0;
-    return team_collect<false>(row, kk, list, 0.0f, none);
+    return team_collect<false>(row, kk, list, 0.0f, none, row.row);
 }
 // how many of the list's first n entries are above e
 template <int W, int SIZE> __device__ __forceinline__ int team_above(const team_list<W, SIZE>& list, int n, uint64_t e) {

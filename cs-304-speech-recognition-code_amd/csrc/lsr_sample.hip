@@ -480,7 +480,7 @@ __global__ __launch_bounds__(64 * W) void lsr_sample_team_kernel(const typename 
     int step = 0;
     while (run + mass[step] <= goal) run += mass[step++];
     {
-        const int c = Row::first_class(step);
+        const int c = row.first_class(step);
         float v[RUN];
         Row::decode(row.read_any(step), v);
         uint64_t own = 0;

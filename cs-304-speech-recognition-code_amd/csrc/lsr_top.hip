@@ -45,99 +45,107 @@ __device__ __forceinline__ uint64_t top_radix(const typename row_type<DT>::type*
     return threshold;
 }
 
-// Long rows, a team of W wavefronts per row (lsr_rows.h).
+// Long rows, a team of W wavefronts per row (lsr_rows.h).  Workgroups of 16 wavefronts with kept rows fill their compute
+// unit alone; there are as many of them as compute units, and each requests its next row while it collects from this one.
 template <int DT, int W, int N, bool REST>
 __global__ __launch_bounds__(64 * W) void lsr_top_team_kernel(const typename row_type<DT>::type* __restrict__ scores,
-                                                              int n_classes, int64_t row_stride, int k, float inv_t,
-                                                              float* __restrict__ values, int32_t* __restrict__ index,
-                                                              float* __restrict__ rest) {
-    using Row = team_row<DT, W, N>;
-    constexpr int THREADS = 64 * W, RUN = Row::RUN, ROOM = W == 1 ? 512 : 2048;
+                                                              int64_t n_rows, int n_classes, int64_t row_stride, int k,
+                                                              float inv_t, float* __restrict__ values,
+                                                              int32_t* __restrict__ index, float* __restrict__ rest) {
+    constexpr int THREADS = 64 * W, RUN = team_row<DT, W, N>::RUN, ROOM = W == 1 ? 512 : 2048;
     __shared__ team_list<W, ROOM> list;
     __shared__ int hist[256];
     __shared__ uint64_t one;
     __shared__ uint64_t sorted[ROOM];                     // by place: the list itself is in the order in which it was filled
     __shared__ float part[W];
     const int tid = threadIdx.x;
-    const int64_t r = blockIdx.x;
     const int kk = k + (REST ? 1 : 0);                    // the first entry of the rest as well
-    Row row;
-    row.open(scores + r * row_stride, n_classes);
-    row.arrive();
-    team_groups(row, list);
     const float unit = inv_t * 1.44269504f;
-    float below = 0.0f;
-    float bound = team_collect<REST>(row, kk, list, unit, below);
-    int n = list.n, bound_class = -1;                     // collected: above the bound, or equal up to this class
-    bool equal = true;                                    // every score that equals the bound is collected
-    if (n > ROOM) {
-        const uint64_t least = top_radix<DT, W>(scores + r * row_stride, n_classes, kk, hist, &one);
-        bound = row_value((uint32_t)(least >> 32));
-        bound_class = (int)~(uint32_t)least;
-        equal = false;
-        if (tid == 0) list.n = 0;
-        team_sync<W>();
-        row.next_pass();
-        row.template each<4>([&](int, const float(&v)[RUN], int c) {
-#pragma unroll
-            for (int j = 0; j < RUN; ++j)
-                if (v[j] > bound || (v[j] == bound && c + j <= bound_class)) list.entry[atomicAdd(&list.n, 1)] = row_entry(row_key(v[j]), c + j);
-        });
-        team_sync<W>();
-        n = list.n;
-    }
-    team_sync<W>();
-    for (int i = tid; i < n; i += THREADS) {
-        const uint64_t e = list.entry[i];
-        sorted[team_above(list, n, e)] = e;
-    }
-    team_sync<W>();
-    for (int i = tid; i < k; i += THREADS) {              // places without an entry: -infinity, -1
-        const uint64_t e = i < n ? sorted[i] : 0;
-        values[r * k + i] = e ? row_value((uint32_t)(e >> 32)) : -INFINITY;
-        index[r * k + i] = e ? (int32_t)~(uint32_t)e : -1;
-    }
-    if (!REST) return;
-    // relative to the highest score of the rest: relative to the row's best it could underflow to nothing
-    const float from = n > k ? row_value((uint32_t)(sorted[k] >> 32)) : -INFINITY;
-    const float best = n > 0 ? row_value((uint32_t)(sorted[0] >> 32)) : 0.0f;
-    float sum = 0.0f;
-    for (int i = k + tid; i < n; i += THREADS) {
-        const float v = row_value((uint32_t)(sorted[i] >> 32));
-        sum += v == from ? 1.0f : __builtin_amdgcn_exp2f((v - from) * unit);
-    }
-    // a NaN among the scores, absent like -infinity, spoils the sum of the pass that collected: once more, one by one
-    const bool spoilt = equal && team_max<W>(below != below ? 1.0f : 0.0f, part) > 0;
-    if (from > -INFINITY) {
-        if (equal && !spoilt) {                                      // relative to the bound, which an entry of the rest reaches
-            if (below > 0) sum += below * __builtin_amdgcn_exp2f((bound - from) * unit);
-        } else {
-            row.next_pass();
-            row.template each<4>([&](int, const float(&v)[RUN], int c) {
+    team_row<DT, W, N> row;
+    row.open(scores + (int64_t)blockIdx.x * row_stride, n_classes);
+    for (int64_t r = blockIdx.x; r < n_rows; r += gridDim.x) {
+        const auto* mine = scores + r * row_stride;
+        if (N)
+            row.arrive();
+        else
+            row.open(mine, n_classes);
+        team_groups(row, list);
+        float below = 0.0f;
+        float bound = team_collect<REST>(row, kk, list, unit, below, mine + (r + gridDim.x < n_rows ? gridDim.x * row_stride : 0));
+        team_row<DT, W, 0> again;                         // for the cases that need the row once more
+        again.open(mine, n_classes);
+        int n = list.n, bound_class = -1;                 // collected: above the bound, or equal up to this class
+        bool equal = true;                                // every score that equals the bound is collected
+        if (n > ROOM) {
+            const uint64_t least = top_radix<DT, W>(mine, n_classes, kk, hist, &one);
+            bound = row_value((uint32_t)(least >> 32));
+            bound_class = (int)~(uint32_t)least;
+            equal = false;
+            if (tid == 0) list.n = 0;
+            team_sync<W>();
+            again.template each<1>([&](int, const float(&v)[RUN], int c) {
 #pragma unroll
                 for (int j = 0; j < RUN; ++j)
-                    if (v[j] < bound || (!equal && v[j] == bound && c + j > bound_class))
-                        sum += v[j] == from ? 1.0f : __builtin_amdgcn_exp2f((v[j] - from) * unit);
+                    if (v[j] > bound || (v[j] == bound && c + j <= bound_class))
+                        list.entry[atomicAdd(&list.n, 1)] = row_entry(row_key(v[j]), c + j);
             });
+            team_sync<W>();
+            n = list.n;
         }
+#pragma unroll 1
+        for (int i = tid; i < n; i += THREADS) {
+            const uint64_t e = list.entry[i];
+            sorted[team_above(list, n, e)] = e;
+        }
+        team_sync<W>();
+        for (int i = tid; i < k; i += THREADS) {          // places without an entry: -infinity, -1
+            const uint64_t e = i < n ? sorted[i] : 0;
+            values[r * k + i] = e ? row_value((uint32_t)(e >> 32)) : -INFINITY;
+            index[r * k + i] = e ? (int32_t)~(uint32_t)e : -1;
+        }
+        if (REST) {
+            // relative to the highest score of the rest: relative to the row's best it could underflow to nothing
+            const float from = n > k ? row_value((uint32_t)(sorted[k] >> 32)) : -INFINITY;
+            const float best = n > 0 ? row_value((uint32_t)(sorted[0] >> 32)) : 0.0f;
+            float sum = 0.0f;
+            for (int i = k + tid; i < n; i += THREADS) {
+                const float v = row_value((uint32_t)(sorted[i] >> 32));
+                sum += v == from ? 1.0f : __builtin_amdgcn_exp2f((v - from) * unit);
+            }
+            // a NaN among the scores, absent like -infinity, spoils the sum of the pass that collected: once more, one by one
+            const bool spoilt = equal && team_max<W>(below != below ? 1.0f : 0.0f, part) > 0;
+            if (from > -INFINITY) {
+                if (equal && !spoilt) {                   // relative to the bound, which an entry of the rest reaches
+                    if (below > 0) sum += below * __builtin_amdgcn_exp2f((bound - from) * unit);
+                } else {
+                    again.template each<1>([&](int, const float(&v)[RUN], int c) {
+#pragma unroll
+                        for (int j = 0; j < RUN; ++j)
+                            if (v[j] < bound || (!equal && v[j] == bound && c + j > bound_class))
+                                sum += v[j] == from ? 1.0f : __builtin_amdgcn_exp2f((v[j] - from) * unit);
+                    });
+                }
+            }
+            sum = team_sum<W>(sum, part);
+            if (tid == 0) rest[r] = from > -INFINITY ? (from == best ? 0.0f : (from - best) * inv_t) + logf(sum) : -INFINITY;
+        }
+        team_sync<W>();                                   // the next row's list takes this one's place
     }
-    sum = team_sum<W>(sum, part);
-    if (tid == 0) rest[r] = from > -INFINITY ? (from == best ? 0.0f : (from - best) * inv_t) + logf(sum) : -INFINITY;
 }
 
 template <int DT, int W, int N>
-static void lsr_top_team(hipStream_t stream, const void* scores_d, int64_t n_rows, int n_classes, int64_t row_stride, int k,
+static void lsr_top_team(lsr_ctx* ctx, const void* scores_d, int64_t n_rows, int n_classes, int64_t row_stride, int k,
                          float inv_t, float* values_d, int32_t* index_d, float* rest_d) {
     const auto* scores = (const typename row_type<DT>::type*)scores_d;
-    const dim3 grid((unsigned)n_rows), block(64 * W);
     // 64 registers of 32-bit scores and what the passes need do not fit together: 96 x 50001 with the rest takes 37 us kept
     // and spilling, 16.5 us read again
     constexpr int KEEP = DT == ROW_F32 && W == 16 ? 0 : N;
+    const dim3 grid((unsigned)(W == 16 && KEEP && n_rows > ctx->n_cus ? ctx->n_cus : n_rows)), block(64 * W);
     if (rest_d)
-        hipLaunchKernelGGL((lsr_top_team_kernel<DT, W, KEEP, true>), grid, block, 0, stream, scores, n_classes, row_stride, k,
+        hipLaunchKernelGGL((lsr_top_team_kernel<DT, W, KEEP, true>), grid, block, 0, ctx->stream, scores, n_rows, n_classes, row_stride, k,
                            inv_t, values_d, index_d, rest_d);
     else
-        hipLaunchKernelGGL((lsr_top_team_kernel<DT, W, KEEP, false>), grid, block, 0, stream, scores, n_classes, row_stride, k,
+        hipLaunchKernelGGL((lsr_top_team_kernel<DT, W, KEEP, false>), grid, block, 0, ctx->stream, scores, n_rows, n_classes, row_stride, k,
                            inv_t, values_d, index_d, rest_d);
 }
 
@@ -241,7 +249,7 @@ extern "C" int lsr_top_scores(lsr_ctx* ctx, const void* scores_d, int dtype, int
         LSR_LAUNCH_CHECK(ctx, "lsr_top_quad_kernel");
         return LSR_OK;
     }
-    LSR_TEAM_SWITCH(dtype, n_classes, lsr_top_team<DT, W, N>(ctx->stream, scores_d, n_rows, (int)n_classes, row_stride, k, inv_t,
+    LSR_TEAM_SWITCH(dtype, n_classes, lsr_top_team<DT, W, N>(ctx, scores_d, n_rows, (int)n_classes, row_stride, k, inv_t,
                                                              values_d, index_d, rest_d));
     lsr_prof_end(ctx);
     LSR_LAUNCH_CHECK(ctx, "lsr_top_team_kernel");
