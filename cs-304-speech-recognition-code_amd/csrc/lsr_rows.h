@@ -604,7 +604,7 @@ __device__ __forceinline__ float team_groups(team_row<DT, W, N>& row, team_list<
 // a score and all present entries are collected.  `list.n` may exceed the list's size: then only some of them are there.
 // SUM: also this thread's sum of e^((x - bound) unit ln 2) over what stays below the bound, in the same pass; NaN where the
 // thread has seen one.
-// A kept row is asked for the next row, `next`, on the way.
+// A kept row of a team of 16 is asked for the next row, `next`, on the way.
 template <bool SUM, int DT, int W, int N, int SIZE>
 __device__ __forceinline__ float team_collect(team_row<DT, W, N>& row, int kk, team_list<W, SIZE>& list, float unit, float& below,
                                               const typename row_type<DT>::type* next) {
@@ -649,7 +649,7 @@ __device__ __forceinline__ float team_collect(team_row<DT, W, N>& row, int kk, t
             for (int j = 0; j < RUN; ++j) below += __builtin_amdgcn_exp2f((v[j] - bound) * unit);
         }
     };
-    if (N)
+    if (W == 16 && N)                                     // (smaller teams take one row each)
         row.each_run_then(next, take);
     else
         row.template each_run<4>(take);

@@ -58,17 +58,18 @@ __global__ __launch_bounds__(64 * W) void lsr_top_team_kernel(const typename row
     __shared__ uint64_t one;
     __shared__ uint64_t sorted[ROOM];                     // by place: the list itself is in the order in which it was filled
     __shared__ float part[W];
-    const int tid = threadIdx.x;
+    constexpr bool ON = W == 16 && N > 0;                 // goes on to further rows
+    int tid = threadIdx.x;
     const int kk = k + (REST ? 1 : 0);                    // the first entry of the rest as well
     const float unit = inv_t * 1.44269504f;
     team_row<DT, W, N> row;
     row.open(scores + (int64_t)blockIdx.x * row_stride, n_classes);
-    for (int64_t r = blockIdx.x; r < n_rows; r += gridDim.x) {
+    int64_t r = blockIdx.x;
+    do {
+        asm volatile("" : "+v"(tid));                     // nothing that depends on it is kept from row to row in registers
         const auto* mine = scores + r * row_stride;
-        if (N)
-            row.arrive();
-        else
-            row.open(mine, n_classes);
+        row.arrive();
+        if (!N) row.open(mine, n_classes);
         team_groups(row, list);
         float below = 0.0f;
         float bound = team_collect<REST>(row, kk, list, unit, below, mine + (r + gridDim.x < n_rows ? gridDim.x * row_stride : 0));
@@ -129,8 +130,8 @@ __global__ __launch_bounds__(64 * W) void lsr_top_team_kernel(const typename row
             sum = team_sum<W>(sum, part);
             if (tid == 0) rest[r] = from > -INFINITY ? (from == best ? 0.0f : (from - best) * inv_t) + logf(sum) : -INFINITY;
         }
-        team_sync<W>();                                   // the next row's list takes this one's place
-    }
+        if (ON) team_sync<W>();                           // the next row's list takes this one's place
+    } while (ON && (r += gridDim.x) < n_rows);
 }
 
 template <int DT, int W, int N>
