@@ -189,7 +189,8 @@ __global__ __launch_bounds__(64 * W) void lsr_distill_team_kernel(
             out.e[j] = (T)(used ? (nan ? NAN : d) : 0.0f);
         }
         if (c + RUN <= n_classes) {
-            *(decltype(out)*)(g + c) = out;
+            const uint4 u = __builtin_bit_cast(uint4, out);
+            __builtin_nontemporal_store((row_words){u.x, u.y, u.z, u.w}, (row_words*)(g + c));
         } else {
 #pragma unroll
             for (int j = 0; j < RUN; ++j)
