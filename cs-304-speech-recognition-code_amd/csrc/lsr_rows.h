@@ -609,33 +609,13 @@ __device__ __forceinline__ float team_groups(team_row<DT, W, N>& row, team_list<
     const uint32_t best = (uint32_t)wave_max((uint64_t)(a > b ? a : b));
     return best ? row_value(best) : -INFINITY;
 }
-// Collects the entries that reach the bound of kk; returns the bound as a score, -FLT_MAX when there are fewer groups with
-// a score and all present entries are collected.  `list.n` may exceed the list's size: then only some of them are there.
+// Collects the entries that reach `bound`; `list.n`, 0 on entry, may exceed the list's size: then only some of them are there.
 // SUM: also this thread's sum of e^((x - bound) unit ln 2) over what stays below the bound, in the same pass; NaN where the
-// thread has seen one.
-// A kept row of a team of 16 is asked for the next row, `next`, on the way.
+// thread has seen one.  A kept row of a team of 16 is asked for the next row, `next`, on the way.
 template <bool SUM, int DT, int W, int N, int SIZE>
-__device__ __forceinline__ float team_collect(team_row<DT, W, N>& row, int kk, team_list<W, SIZE>& list, float unit, float& below,
-                                              const typename row_type<DT>::type* next) {
+__device__ __forceinline__ void team_take(team_row<DT, W, N>& row, float bound, team_list<W, SIZE>& list, float unit, float& below,
+                                          const typename row_type<DT>::type* next) {
     constexpr int RUN = team_row<DT, W, N>::RUN;
-    const int tid = threadIdx.x;
-    if (tid < 64) {                                       // the largest number that kk groups reach, bit by bit
-        const uint4 o = *(const uint4*)&list.group[tid * 4];
-        uint32_t bound = 0;
-#pragma unroll 1
-        for (uint32_t bit = 1u << 31; bit; bit >>= 1) {
-            const uint32_t b = bound | bit;
-            const int reach = __popcll(__ballot(o.x >= b)) + __popcll(__ballot(o.y >= b)) + __popcll(__ballot(o.z >= b)) +
-                              __popcll(__ballot(o.w >= b));
-            if (reach >= kk) bound = b;
-        }
-        if (tid == 0) {
-            list.bound = bound;
-            list.n = 0;
-        }
-    }
-    team_sync<W>();
-    const float bound = list.bound ? row_value(list.bound) : -3.402823466e38f;
     row.next_pass();
     auto take = [&](int step, const uint4& packed) {
         float v[RUN];
@@ -663,6 +643,31 @@ __device__ __forceinline__ float team_collect(team_row<DT, W, N>& row, int kk, t
     else
         row.template each_run<4>(take);
     team_sync<W>();
+}
+// Collects the entries that reach the bound of kk; returns the bound as a score, -FLT_MAX when there are fewer groups with
+// a score and all present entries are collected.
+template <bool SUM, int DT, int W, int N, int SIZE>
+__device__ __forceinline__ float team_collect(team_row<DT, W, N>& row, int kk, team_list<W, SIZE>& list, float unit, float& below,
+                                              const typename row_type<DT>::type* next) {
+    const int tid = threadIdx.x;
+    if (tid < 64) {                                       // the largest number that kk groups reach, bit by bit
+        const uint4 o = *(const uint4*)&list.group[tid * 4];
+        uint32_t bound = 0;
+#pragma unroll 1
+        for (uint32_t bit = 1u << 31; bit; bit >>= 1) {
+            const uint32_t b = bound | bit;
+            const int reach = __popcll(__ballot(o.x >= b)) + __popcll(__ballot(o.y >= b)) + __popcll(__ballot(o.z >= b)) +
+                              __popcll(__ballot(o.w >= b));
+            if (reach >= kk) bound = b;
+        }
+        if (tid == 0) {
+            list.bound = bound;
+            list.n = 0;
+        }
+    }
+    team_sync<W>();
+    const float bound = list.bound ? row_value(list.bound) : -3.402823466e38f;
+    team_take<SUM>(row, bound, list, unit, below, next);
     return bound;
 }
 template <int DT, int W, int N, int SIZE>

@@ -223,34 +223,52 @@ __global__ __launch_bounds__(64 * W) void lsr_sample_team_kernel(const typename 
     };
     if (best == INFINITY) return slowly();
 
-    // few: a small top_k; nucleus: top_p alone, where it looks as if a short head will do: where the best scores of the
-    // groups hold that share of the row's weight, both in 32 bits
-    const bool cut = top_k > 0 && top_k < n_classes, few = cut && top_k <= LSR_MAX_TOP;
-    bool nucleus = !cut && top_p < 1;
-    if (nucleus) {
-        const float unit_f = (float)unit;
-        float guess = 0, head = 0;
+    // Rows that are answered from a list of their first entries.  few: a small top_k.  level: min_p without top_k, when not
+    // many entries reach it.  nucleus: top_p alone, where it looks as if a short head will do: where the best scores of the
+    // groups hold that share of the row's weight.
+    const bool cut = top_k > 0 && top_k < n_classes, few = cut && top_k <= LSR_MAX_TOP, level = !cut && min_p > 0;
+    const float floor = min_p > 0 ? sample_floor(best, t, min_p) : -INFINITY, unit_f = (float)unit;
+    bool nucleus = !cut && !level && top_p < 1;
+    float guess = 0;                                      // the row's weight in 32 bits, good to 2^-12 and better
+    if (!cut && top_p < 1) {
+        float head = 0;
         row.template each<4>([&](int, const float(&v)[RUN], int) {
 #pragma unroll
             for (int j = 0; j < RUN; ++j) guess += __builtin_amdgcn_exp2f((v[j] - best) * unit_f);
         });
+        guess = team_sum<W>(guess, part_f);
         for (int i = tid; i < ROW_GROUPS; i += THREADS)
             if (list.group[i]) head += __builtin_amdgcn_exp2f((row_value(list.group[i]) - best) * unit_f);
-        nucleus = team_sum<W>(head, part_f) >= (float)top_p * team_sum<W>(guess, part_f);
+        nucleus = nucleus && team_sum<W>(head, part_f) >= (float)top_p * guess;
     }
-    if (few || nucleus) {
-        const int want = few ? top_k : NUCLEUS < n_classes ? NUCLEUS : n_classes;
-        team_collect(row, want, list);
+    if (few || level || nucleus) {
+        if (level) {
+            float none = 0;
+            if (tid == 0) list.n = 0;
+            team_sync<W>();
+            team_take<false>(row, floor, list, 0.0f, none, mine);
+        } else {
+            team_collect(row, few ? top_k : NUCLEUS < n_classes ? NUCLEUS : n_classes, list);
+        }
         const int n = list.n;
-        if (n <= ROOM) {
+        if (n <= (level ? LSR_MAX_TOP : ROOM)) {
 #pragma unroll 1
             for (int i = tid; i < n; i += THREADS) {
                 const uint64_t e = list.entry[i];
                 const int place = team_above(list, n, e);
                 if (place < LSR_MAX_TOP) sorted[place] = e;
             }
-            uint64_t all = 0;                             // weight of the row, where the list does not hold what top_p is a share of
-            if (nucleus) {
+            // weight of the row, where the list does not hold what top_p is a share of; where the level's entries weigh
+            // less than that share by more than the guess can be off, top_p takes nothing away
+            uint64_t all = 0;
+            bool open = top_p >= 1;
+            if (level && !open) {
+                float listed = 0;
+                for (int i = tid; i < n; i += THREADS)
+                    listed += __builtin_amdgcn_exp2f((row_value((uint32_t)(list.entry[i] >> 32)) - best) * unit_f);
+                open = team_sum<W>(listed, part_f) < (1 - 1.0f / 512) * (float)top_p * guess;
+            }
+            if (!few && !open) {
                 row.template each<2>([&](int, const float(&v)[RUN], int) {
 #pragma unroll
                     for (int j = 0; j < RUN; ++j)
@@ -262,7 +280,6 @@ __global__ __launch_bounds__(64 * W) void lsr_sample_team_kernel(const typename 
             team_sync<W>();
             const int most = few ? top_k : LSR_MAX_TOP, m = n < most ? n : most;     // the list is the head of the row, all of it
             if (tid < 64) {                               // lane l has the places 4 l ... 4 l + 3
-                const float floor = min_p > 0 ? sample_floor(best, t, min_p) : -INFINITY;
                 constexpr int FOUR = LSR_MAX_TOP / 64;
                 uint64_t w[FOUR], own = 0;
                 float v[FOUR];
@@ -274,7 +291,7 @@ __global__ __launch_bounds__(64 * W) void lsr_sample_team_kernel(const typename 
                     own += w[i];
                 }
                 uint64_t run = wave_running(own);
-                const uint64_t listed = wave_last(run), target = sample_target(top_p, few ? listed : all);
+                const uint64_t listed = wave_last(run), target = open ? ~0ull : sample_target(top_p, few ? listed : all);
                 run -= own;
                 uint64_t sum = 0;
                 int kept = 0;
@@ -291,7 +308,7 @@ __global__ __launch_bounds__(64 * W) void lsr_sample_team_kernel(const typename 
                 kept = wave_sum(kept);
                 if (tid == 0) {
                     kept_sum = sum;
-                    n_kept = few || listed >= target ? kept : 0;                 // 0: the list is too short for top_p
+                    n_kept = few || level || listed >= target ? kept : 0;        // 0: the list is too short for top_p
                 }
             }
             team_sync<W>();
@@ -419,12 +436,9 @@ __global__ __launch_bounds__(64 * W) void lsr_sample_team_kernel(const typename 
         last = row_value((uint32_t)(lowest >> 32));
         last_class = (int)~(uint32_t)lowest;
     }
-    if (min_p > 0) {
-        const float floor = sample_floor(best, t, min_p);
-        if (floor > last) {
-            last = floor;
-            last_class = n_classes;
-        }
+    if (floor > last) {
+        last = floor;
+        last_class = n_classes;
     }
     // weight of every step, and the step in which the goal lies
     team_sync<W>();
