@@ -4,6 +4,7 @@
 // e^((x - best) / T) are computed in 64 bits and summed as whole numbers: which class a uniform number falls on does not
 // depend on the order of the sums.
 #include <math.h>
+#include <type_traits>
 
 #include "lsr_rows.h"
 
@@ -33,14 +34,27 @@ __device__ __forceinline__ uint64_t sample_goal(float u, uint64_t sum) {
     return !(at > 0) ? 0 : at >= (double)sum ? sum - 1 : (uint64_t)at;
 }
 
-// The lowest entry of the shortest head of a list whose mass is at least `left`, eight bits at a time from a histogram of
-// the entries that still match.  The search is over as soon as a digit's whole mass is needed; then the result, with zeros
-// in the digits that are left, lies below the entry.  `hist` has 257 places.
+// The last entry of the shortest head of a list whose mass is at least `left` (1 at least, and not more than the list's).
+// Up to 256 entries: each is compared with all others.  More: eight bits at a time, from a histogram of the entries that
+// still match; where the whole mass of a digit is needed, the lowest entry of that digit that has mass is the one.  `hist`
+// has 257 places.
 template <int W>
-__device__ __forceinline__ uint64_t list_by_radix(const uint64_t* entry, const uint64_t* mass, int n, uint64_t left, uint64_t* hist) {
+__device__ __forceinline__ uint64_t list_head(const uint64_t* entry, const uint64_t* mass, int n, uint64_t left, uint64_t* hist) {
     constexpr int THREADS = 64 * W;
     const int tid = threadIdx.x;
     uint64_t found = 0;
+    if (n <= (THREADS < 256 ? THREADS : 256)) {
+        team_sync<W>();
+        if (tid < n) {
+            const uint64_t e = entry[tid], m = mass[tid];
+            uint64_t before = 0;
+#pragma unroll 4
+            for (int j = 0; j < n; ++j) before += entry[j] > e ? mass[j] : 0;
+            if (before < left && left <= before + m) hist[0] = e;
+        }
+        team_sync<W>();
+        return hist[0];
+    }
 #pragma unroll 1
     for (int shift = 56; shift >= 0; shift -= 8) {
         team_sync<W>();
@@ -73,7 +87,13 @@ __device__ __forceinline__ uint64_t list_by_radix(const uint64_t* entry, const u
         left = hist[0];
         if (hist[1]) break;
     }
-    return found;
+    team_sync<W>();
+    if (tid == 0) hist[0] = ~0ull;
+    team_sync<W>();
+    for (int i = tid; i < n; i += THREADS)
+        if (mass[i] && entry[i] >= found) atomicMin((unsigned long long*)&hist[0], (unsigned long long)entry[i]);
+    team_sync<W>();
+    return hist[0];
 }
 
 // A row in many passes over memory, by radix selection with weights: for rows that the fast form below does not take (an
@@ -179,15 +199,18 @@ __global__ __launch_bounds__(64 * W) void lsr_sample_team_kernel(const typename 
                                                                  const float* __restrict__ uniform, sample_args a,
                                                                  int32_t* __restrict__ index, float* __restrict__ logprob) {
     using Row = team_row<DT, W, 0>;
-    constexpr int THREADS = 64 * W, RUN = Row::RUN, ROOM = W == 1 ? 512 : 2048;
-    constexpr int BINS = W == 1 ? 512 : W == 4 ? 2048 : 4096, OWN = BINS / THREADS;
+    constexpr int THREADS = 64 * W, RUN = Row::RUN, ROOM = W == 1 ? 512 : W == 4 ? 2048 : 4096;
+    constexpr int BINS = W == 1 ? 512 : W == 4 ? 2048 : 8192, OWN = BINS / THREADS;
     constexpr int STEPS = (W == 1 ? 1024 : W == 4 ? 16384 : LSR_MAX_CLASSES) / Row::STEP;
     __shared__ team_list<W, ROOM> list;
-    __shared__ uint64_t mass[BINS > STEPS ? BINS : STEPS];          // of a bin, of an entry of the list, of a step
-    __shared__ int bin_n[BINS];
-    __shared__ uint64_t sorted[257], part[W], above, lowest, kept_sum;
+    static_assert(ROOM >= LSR_MAX_TOP, "weights of the few");
+    __shared__ uint64_t mass[STEPS > LSR_MAX_TOP ? STEPS : LSR_MAX_TOP];     // of a step, of one of the few
+    static_assert(2 * ROOM >= BINS, "the histogram and the weights of the list share their place, one after the other");
+    __shared__ uint64_t list_mass[ROOM];
+    int* const bin_n = (int*)list_mass;
+    __shared__ uint64_t sorted[257], part[W], above, kept_sum;
     __shared__ float part_f[W];
-    __shared__ int cut_bin, n_kept;
+    __shared__ int part_n[W], cut_bin, n_kept;
     constexpr int NUCLEUS = 128;                          // entries that a nucleus is first looked for in
     const row_exp2_t row_exp2;
     const int tid = threadIdx.x;
@@ -230,7 +253,7 @@ __global__ __launch_bounds__(64 * W) void lsr_sample_team_kernel(const typename 
     const float floor = min_p > 0 ? sample_floor(best, t, min_p) : -INFINITY, unit_f = (float)unit;
     bool nucleus = !cut && !level && top_p < 1;
     float guess = 0;                                      // the row's weight in 32 bits, good to 2^-12 and better
-    if (!cut && top_p < 1) {
+    if (!few && top_p < 1) {
         float head = 0;
         row.template each<4>([&](int, const float(&v)[RUN], int) {
 #pragma unroll
@@ -334,6 +357,7 @@ __global__ __launch_bounds__(64 * W) void lsr_sample_team_kernel(const typename 
             }
             if (kept > 0) return;
         }
+        if (few) return slowly();                         // thousands of entries are alike
     }
 
     float last = -INFINITY;                               // kept: above this score, or equal up to this class
@@ -343,133 +367,193 @@ __global__ __launch_bounds__(64 * W) void lsr_sample_team_kernel(const typename 
     const float per_bin = (float)fmin(BINS / 24.0 / t, 1e30);
     auto bin_of = [&](float v) { return (int)fminf((best - v) * per_bin, (float)(BINS - 1)); };
 
-    // cuts the row where the mass of a head first reaches the target: by number of entries, then by weight
-    for (int by_weight = 0; by_weight < 2; ++by_weight) {
-        if (by_weight ? !(top_p < 1.0) : top_k <= 0 || top_k >= n_classes) continue;
+    auto cut_at = [&](uint64_t e) {
+        last = row_value((uint32_t)(e >> 32));
+        last_class = (int)~(uint32_t)e;
+    };
+    const uint64_t zero = (uint64_t)__double_as_longlong(a.magic);
+    bool summed = false;                                  // the weights of the steps are known already
+
+    if (cut) {                                            // the first top_k entries, by a histogram of their numbers
         team_sync<W>();
-        for (int i = tid; i < BINS; i += THREADS) {
-            mass[i] = 0;
-            bin_n[i] = 0;
-        }
-        if (tid == 0) {
-            list.n = 0;
-            lowest = ~0ull;
-        }
+        for (int i = tid; i < BINS; i += THREADS) bin_n[i] = 0;
+        if (tid == 0) list.n = 0;
         team_sync<W>();
-        if (by_weight) {                                  // what is cut or absent weighs nothing
-            row.template each<2>([&](int, const float(&v)[RUN], int c) {
-                float s[RUN];
+        row.template each<4>([&](int, const float(&v)[RUN], int) {
 #pragma unroll
-                for (int j = 0; j < RUN; ++j) s[j] = keeps(v[j], c + j) ? v[j] : -INFINITY;
-#pragma unroll
-                for (int j = 0; j < RUN; ++j) {
-                    const uint64_t m = weigh(s[j]);
-                    if (m) atomicAdd((unsigned long long*)&mass[bin_of(s[j])], (unsigned long long)m);
-                }
-            });
-        } else {
-            row.template each<4>([&](int, const float(&v)[RUN], int) {
-#pragma unroll
-                for (int j = 0; j < RUN; ++j)
-                    if (v[j] > -INFINITY) atomicAdd(&bin_n[bin_of(v[j])], 1);
-            });
-        }
+            for (int j = 0; j < RUN; ++j)
+                if (v[j] > -INFINITY) atomicAdd(&bin_n[bin_of(v[j])], 1);
+        });
         team_sync<W>();
-        uint64_t own = 0;
+        int own = 0, sum = 0;
 #pragma unroll
-        for (int i = 0; i < OWN; ++i) own += by_weight ? mass[tid * OWN + i] : (uint64_t)bin_n[tid * OWN + i];
-        uint64_t run = wave_running(own);
-        if ((tid & 63) == 63) part[tid >> 6] = run;
+        for (int i = 0; i < OWN; ++i) own += bin_n[tid * OWN + i];
+        int run = wave_running(own);
+        if ((tid & 63) == 63) part_n[tid >> 6] = run;
         team_sync<W>();
-        uint64_t sum = 0;
 #pragma unroll
         for (int i = 0; i < W; ++i) {
-            if (i < (tid >> 6)) run += part[i];
-            sum += part[i];
+            if (i < (tid >> 6)) run += part_n[i];
+            sum += part_n[i];
         }
-        const uint64_t target = by_weight ? sample_target(top_p, sum) : (uint64_t)top_k;
-        if (target > sum) continue;                       // fewer entries than that: all are kept
+        if (top_k <= sum) {                               // or all are kept
+            run -= own;
+            if (run < top_k && top_k <= run + own) {
+#pragma unroll
+                for (int i = 0; i < OWN; ++i) {
+                    const int m = bin_n[tid * OWN + i];
+                    if (run < top_k && top_k <= run + m) {
+                        cut_bin = tid * OWN + i;
+                        n_kept = run;
+                    }
+                    run += m;
+                }
+            }
+            team_sync<W>();
+            const int b = cut_bin, ahead = n_kept;
+            row.template each<4>([&](int, const float(&v)[RUN], int c) {
+#pragma unroll
+                for (int j = 0; j < RUN; ++j)
+                    if (v[j] > -INFINITY && bin_of(v[j]) == b) {
+                        const int at = atomicAdd(&list.n, 1);
+                        if (at < ROOM) list.entry[at] = row_entry(row_key(v[j]), c + j);
+                    }
+            });
+            team_sync<W>();
+            const int n = list.n;
+            if (n > ROOM) return slowly();
+            for (int i = tid; i < n; i += THREADS) list_mass[i] = 1;
+            team_sync<W>();
+            cut_at(list_head<W>(list.entry, list_mass, n, (uint64_t)(top_k - ahead), sorted));
+        }
+    }
+    if (top_p < 1) {
+        // The entries that hold top_p of what is left.  A histogram of weights in 32 bits (whole numbers: adding floats in
+        // shared memory takes eight times as long) says near which bin that cut lies.  One pass in 64 bits then sums
+        // everything and, step by step, what is above the neighbours of that bin, and collects what is in the three of
+        // them: if the cut is there, everything is known that the draw needs.  It can be elsewhere where it lies as near to
+        // an edge as 32 bits are off and empty bins follow.
+        team_sync<W>();
+        for (int i = tid; i < BINS; i += THREADS) bin_n[i] = 0;
+        for (int i = tid; i < row.steps; i += THREADS) mass[i] = 0;
+        if (tid == 0) {
+            list.n = 0;
+            cut_bin = BINS - 1;
+        }
+        team_sync<W>();
+        const float scale = 1073741824.0f / guess;
+        row.template each<4>([&](int, const float(&v)[RUN], int c) {
+#pragma unroll
+            for (int j = 0; j < RUN; ++j) {
+                const float s = !cut || keeps(v[j], c + j) ? v[j] : -INFINITY;
+                const int m = (int)(__builtin_amdgcn_exp2f((s - best) * unit_f) * scale + 0.5f);
+                if (m) atomicAdd(&bin_n[bin_of(s)], m);
+            }
+        });
+        team_sync<W>();
+        uint32_t own = 0, total = 0;
+#pragma unroll
+        for (int i = 0; i < OWN; ++i) own += (uint32_t)bin_n[tid * OWN + i];
+        uint32_t run = (uint32_t)wave_running((int)own);
+        if ((tid & 63) == 63) part_n[tid >> 6] = (int)run;
+        team_sync<W>();
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+            if (i < (tid >> 6)) run += (uint32_t)part_n[i];
+            total += (uint32_t)part_n[i];
+        }
         run -= own;
-        if (run < target && target <= run + own) {
+        const uint32_t near = (uint32_t)(top_p * total);
+        if (run < near && near <= run + own) {
 #pragma unroll
             for (int i = 0; i < OWN; ++i) {
-                const uint64_t m = by_weight ? mass[tid * OWN + i] : (uint64_t)bin_n[tid * OWN + i];
-                if (run < target && target <= run + m) {
-                    cut_bin = tid * OWN + i;
-                    above = run;
-                }
-                run += m;
+                if (run < near) cut_bin = tid * OWN + i;
+                run += (uint32_t)bin_n[tid * OWN + i];
             }
         }
         team_sync<W>();
-        const int b = cut_bin;
-        const uint64_t ahead = above;
-        row.template each<4>([&](int, const float(&v)[RUN], int c) {
+        const float high = best - (cut_bin - 1) / per_bin, low = best - (cut_bin + 2) / per_bin;
+        uint64_t all = 0;
+        auto weigh_all = [&](auto some) {
+            row.template each<2>([&](int step, const float(&v)[RUN], int c) {
+                uint64_t higher = 0;
 #pragma unroll
-            for (int j = 0; j < RUN; ++j)
-                if (keeps(v[j], c + j) && bin_of(v[j]) == b) {
-                    const int at = atomicAdd(&list.n, 1);
-                    if (at < ROOM) list.entry[at] = row_entry(row_key(v[j]), c + j);
+                for (int j = 0; j < RUN; ++j) {
+                    const float s = !some.value || keeps(v[j], c + j) ? v[j] : -INFINITY;
+                    const uint64_t m = (uint64_t)__double_as_longlong(row_exp2(((double)s - best) * unit) + a.magic);
+                    all += m;
+                    higher += s > high ? m : zero;
+                    if ((s <= high) & (s >= low) & (s > -INFINITY)) {
+                        const int at = atomicAdd(&list.n, 1);
+                        if (at < ROOM) {
+                            list.entry[at] = row_entry(row_key(s), c + j);
+                            list_mass[at] = m - zero;
+                        }
+                    }
                 }
-        });
+                all -= RUN * zero;
+                higher = wave_sum(higher - RUN * zero);
+                if ((tid & 63) == 0 && higher) atomicAdd((unsigned long long*)&mass[step], (unsigned long long)higher);
+            });
+        };
+        if (cut)
+            weigh_all(std::true_type{});
+        else
+            weigh_all(std::false_type{});
+        all = team_sum<W>(all, part);
         team_sync<W>();
         const int n = list.n;
         if (n > ROOM) return slowly();
-        for (int i = tid; i < n; i += THREADS) mass[i] = by_weight ? weigh(row_value((uint32_t)(list.entry[i] >> 32))) : 1;
-        team_sync<W>();
-        if (n > (THREADS < 256 ? THREADS : 256)) {        // many: radix selection in the list
-            const uint64_t least = list_by_radix<W>(list.entry, mass, n, target - ahead, sorted);
-            // a threshold between entries rather than one of them: its class may be any number, its key below every score's
-            const uint32_t key = (uint32_t)(least >> 32), beyond = ~(uint32_t)least;
-            last = key > 0x007fffffu ? row_value(key) : -3.402823466e38f;
-            last_class = key > 0x007fffffu && beyond < (uint32_t)n_classes ? (int)beyond : n_classes;
-            continue;
-        }
-        for (int i = tid; i < n; i += THREADS) {
+        uint64_t ahead = 0, listed = 0;
+        for (int i = 0; i < row.steps; ++i) ahead += mass[i];
+        for (int i = tid; i < n; i += THREADS) listed += list_mass[i];
+        listed = team_sum<W>(listed, part);
+        const uint64_t target = sample_target(top_p, all);
+        if (ahead >= target || target > ahead + listed) return slowly();
+        cut_at(list_head<W>(list.entry, list_mass, n, target - ahead, sorted));
+        summed = floor <= last;
+        for (int i = tid; summed && i < n; i += THREADS) {
             const uint64_t e = list.entry[i];
-            uint64_t before = ahead;
-#pragma unroll 4
-            for (int j = 0; j < n; ++j) before += list.entry[j] > e ? mass[j] : 0;
-            if (before < target) atomicMin((unsigned long long*)&lowest, (unsigned long long)e);
+            const int c = (int)~(uint32_t)e;
+            if (keeps(row_value((uint32_t)(e >> 32)), c))
+                atomicAdd((unsigned long long*)&mass[c / Row::STEP], (unsigned long long)list_mass[i]);
         }
-        team_sync<W>();
-        last = row_value((uint32_t)(lowest >> 32));
-        last_class = (int)~(uint32_t)lowest;
     }
     if (floor > last) {
         last = floor;
         last_class = n_classes;
     }
     // weight of every step, and the step in which the goal lies
-    team_sync<W>();
-    for (int i = tid; i < row.steps; i += THREADS) mass[i] = 0;
-    team_sync<W>();
-    const uint64_t zero = (uint64_t)__double_as_longlong(a.magic);
-    const bool all = last == -INFINITY;
-    row.template each<2>([&](int step, const float(&v)[RUN], int c) {
-        uint64_t sum = 0;
-        if (all) {                                        // what is absent weighs nothing
-#pragma unroll
-            for (int j = 0; j < RUN; ++j)
-                sum += (uint64_t)__double_as_longlong(row_exp2(((double)v[j] - best) * unit) + a.magic);
-            sum -= RUN * zero;
-        } else {
-            float s[RUN], high = -INFINITY;
-#pragma unroll
-            for (int j = 0; j < RUN; ++j) {
-                s[j] = keeps(v[j], c + j) ? v[j] : -INFINITY;
-                high = row_max(high, s[j]);
-            }
-            if (high > -INFINITY) {
+    if (!summed) {
+        team_sync<W>();
+        for (int i = tid; i < row.steps; i += THREADS) mass[i] = 0;
+        team_sync<W>();
+        const bool all = last == -INFINITY;
+        row.template each<2>([&](int step, const float(&v)[RUN], int c) {
+            uint64_t sum = 0;
+            if (all) {                                        // what is absent weighs nothing
 #pragma unroll
                 for (int j = 0; j < RUN; ++j)
-                    sum += (uint64_t)__double_as_longlong(row_exp2(((double)s[j] - best) * unit) + a.magic);
+                    sum += (uint64_t)__double_as_longlong(row_exp2(((double)v[j] - best) * unit) + a.magic);
                 sum -= RUN * zero;
+            } else {
+                float s[RUN], high = -INFINITY;
+#pragma unroll
+                for (int j = 0; j < RUN; ++j) {
+                    s[j] = keeps(v[j], c + j) ? v[j] : -INFINITY;
+                    high = row_max(high, s[j]);
+                }
+                if (high > -INFINITY) {
+#pragma unroll
+                    for (int j = 0; j < RUN; ++j)
+                        sum += (uint64_t)__double_as_longlong(row_exp2(((double)s[j] - best) * unit) + a.magic);
+                    sum -= RUN * zero;
+                }
             }
-        }
-        sum = wave_sum(sum);
-        if ((tid & 63) == 0 && sum) atomicAdd((unsigned long long*)&mass[step], (unsigned long long)sum);
-    });
+            sum = wave_sum(sum);
+            if ((tid & 63) == 0 && sum) atomicAdd((unsigned long long*)&mass[step], (unsigned long long)sum);
+        });
+    }
     team_sync<W>();
     uint64_t sum = 0;
     for (int i = 0; i < row.steps; ++i) sum += mass[i];
