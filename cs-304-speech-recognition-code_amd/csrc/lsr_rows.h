@@ -27,26 +27,6 @@ __device__ __forceinline__ float row_value(uint32_t key) {
 }
 __device__ __forceinline__ uint64_t row_entry(uint32_t key, uint32_t cls) { return (uint64_t)key << 32 | (uint32_t)~cls; }
 
-__device__ __forceinline__ int row_wave_sum(int v) {
-    for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
-    return v;
-}
-__device__ __forceinline__ float row_wave_sum(float v) {
-    for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
-    return v;
-}
-__device__ __forceinline__ uint64_t row_wave_sum(uint64_t v) {
-    for (int d = 32; d; d >>= 1) v += (uint64_t)__shfl_xor((unsigned long long)v, d);
-    return v;
-}
-__device__ __forceinline__ uint64_t row_wave_max(uint64_t v) {
-    for (int d = 32; d; d >>= 1) {
-        const uint64_t o = (uint64_t)__shfl_xor((unsigned long long)v, d);
-        v = o > v ? o : v;
-    }
-    return v;
-}
-
 // 2^y for y <= 0 to 2^-50 of the result: the fraction in [-1/2, 1/2] goes through a polynomial of degree 10 that is 1 at 0
 // (interpolation of (2^f - 1) / f at the Chebyshev nodes, largest relative error 5.6e-16).  16 instructions, all of them of
 // the rate of 32-bit ones on this part; the library's exp takes about three times as many.  The coefficients are held in
@@ -644,11 +624,8 @@ __device__ __forceinline__ void team_take(team_row<DT, W, N>& row, float bound, 
         row.template each_run<4>(take);
     team_sync<W>();
 }
-// Collects the entries that reach the bound of kk; returns the bound as a score, -FLT_MAX when there are fewer groups with
-// a score and all present entries are collected.
-template <bool SUM, int DT, int W, int N, int SIZE>
-__device__ __forceinline__ float team_collect(team_row<DT, W, N>& row, int kk, team_list<W, SIZE>& list, float unit, float& below,
-                                              const typename row_type<DT>::type* next) {
+// The bound of kk as a score, -FLT_MAX when fewer groups than that have a score; empties the list.
+template <int W, int SIZE> __device__ __forceinline__ float team_bound(int kk, team_list<W, SIZE>& list) {
     const int tid = threadIdx.x;
     if (tid < 64) {                                       // the largest number that kk groups reach, bit by bit
         const uint4 o = *(const uint4*)&list.group[tid * 4];
@@ -666,14 +643,7 @@ __device__ __forceinline__ float team_collect(team_row<DT, W, N>& row, int kk, t
         }
     }
     team_sync<W>();
-    const float bound = list.bound ? row_value(list.bound) : -3.402823466e38f;
-    team_take<SUM>(row, bound, list, unit, below, next);
-    return bound;
-}
-template <int DT, int W, int N, int SIZE>
-__device__ __forceinline__ float team_collect(team_row<DT, W, N>& row, int kk, team_list<W, SIZE>& list) {
-    float none = 0;
-    return team_collect<false>(row, kk, list, 0.0f, none, row.row);
+    return list.bound ? row_value(list.bound) : -3.402823466e38f;
 }
 // how many of the list's first n entries are above e
 template <int W, int SIZE> __device__ __forceinline__ int team_above(const team_list<W, SIZE>& list, int n, uint64_t e) {
@@ -683,8 +653,8 @@ template <int W, int SIZE> __device__ __forceinline__ int team_above(const team_
     return above;
 }
 
-// Wavefronts per row by the row's width.  KEPT: rows that fit stay in registers, the number of runs a thread keeps is the
-// second parameter.
+// Wavefronts per row by the row's width, W, and the runs of it that a thread keeps in registers, N; LSR_WAVES_SWITCH for an
+// operator that keeps none.
 #define LSR_TEAM_SWITCH(dtype, classes, ...)                                                              \
     do {                                                                                                  \
         if ((dtype) == LSR_F32) {                                                                         \

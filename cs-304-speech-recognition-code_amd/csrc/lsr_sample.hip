@@ -22,6 +22,11 @@ __device__ __forceinline__ float sample_floor(float best, double t, double min_p
     const float f = (float)low;
     return (double)f < low ? nextafterf(f, INFINITY) : f;
 }
+// The lowest score that weighs anything in 64 bits.  What is below (masked with the type's lowest value, say) changes no sum
+// and is never drawn; leaving it out keeps thousands of equal scores out of the lists.
+__device__ __forceinline__ float sample_least(float best, double unit) {
+    return (float)fmax((double)best - 1074.0 / unit, -3.402823466e38);
+}
 // the mass that top_p asks for: the first whole number that is not below its share of the sum, 1 at least
 __device__ __forceinline__ uint64_t sample_target(double top_p, uint64_t sum) {
     if (!(top_p < 1.0)) return ~0ull;
@@ -106,7 +111,7 @@ __device__ __forceinline__ void sample_by_radix(const typename row_type<DT>::typ
     const row_exp2_t row_exp2;
     const int tid = threadIdx.x;
     const double unit = isinf(best) ? 1.0 : ROW_LOG2E / t;
-    uint64_t least = 1;
+    uint64_t least = (uint64_t)row_key(sample_least(best, unit)) << 32;
     // mass of a class: 1 or its weight, 0 below the threshold
     auto mass = [&](int c, bool count, uint64_t* e) -> uint64_t {
         const float v = (float)x[c];
@@ -226,6 +231,7 @@ __global__ __launch_bounds__(64 * W) void lsr_sample_team_kernel(const typename 
     const double unit = ROW_LOG2E / t;
 
     const float best = team_groups(row, list);
+    const float least = sample_least(best, unit);
     if (best == -INFINITY || !(t > 0)) {                  // nothing to draw from, or the best entry itself
         int at = 1 << 30;
         if (best > -INFINITY)
@@ -265,14 +271,10 @@ __global__ __launch_bounds__(64 * W) void lsr_sample_team_kernel(const typename 
         nucleus = nucleus && team_sum<W>(head, part_f) >= (float)top_p * guess;
     }
     if (few || level || nucleus) {
-        if (level) {
-            float none = 0;
-            if (tid == 0) list.n = 0;
-            team_sync<W>();
-            team_take<false>(row, floor, list, 0.0f, none, mine);
-        } else {
-            team_collect(row, few ? top_k : NUCLEUS < n_classes ? NUCLEUS : n_classes, list);
-        }
+        float none = 0, bound = few || nucleus ? team_bound(few ? top_k : NUCLEUS < n_classes ? NUCLEUS : n_classes, list) : floor;
+        if (level && tid == 0) list.n = 0;
+        if (level) team_sync<W>();
+        team_take<false>(row, row_max(bound, least), list, 0.0f, none, mine);
         const int n = list.n;
         if (n <= (level ? LSR_MAX_TOP : ROOM)) {
 #pragma unroll 1
@@ -360,8 +362,8 @@ __global__ __launch_bounds__(64 * W) void lsr_sample_team_kernel(const typename 
         if (few) return slowly();                         // thousands of entries are alike
     }
 
-    float last = -INFINITY;                               // kept: above this score, or equal up to this class
-    int last_class = -1;
+    float last = least;                                   // kept: above this score, or equal up to this class
+    int last_class = n_classes;
     auto keeps = [&](float v, int c) { return (v > last) | ((v == last) & (c <= last_class)); };
     auto weigh = [&](float v) { return row_fixed(row_exp2(((double)v - best) * unit), a.magic); };
     const float per_bin = (float)fmin(BINS / 24.0 / t, 1e30);
@@ -382,7 +384,7 @@ __global__ __launch_bounds__(64 * W) void lsr_sample_team_kernel(const typename 
         row.template each<4>([&](int, const float(&v)[RUN], int) {
 #pragma unroll
             for (int j = 0; j < RUN; ++j)
-                if (v[j] > -INFINITY) atomicAdd(&bin_n[bin_of(v[j])], 1);
+                if (v[j] >= least) atomicAdd(&bin_n[bin_of(v[j])], 1);
         });
         team_sync<W>();
         int own = 0, sum = 0;
@@ -414,7 +416,7 @@ __global__ __launch_bounds__(64 * W) void lsr_sample_team_kernel(const typename 
             row.template each<4>([&](int, const float(&v)[RUN], int c) {
 #pragma unroll
                 for (int j = 0; j < RUN; ++j)
-                    if (v[j] > -INFINITY && bin_of(v[j]) == b) {
+                    if (v[j] >= least && bin_of(v[j]) == b) {
                         const int at = atomicAdd(&list.n, 1);
                         if (at < ROOM) list.entry[at] = row_entry(row_key(v[j]), c + j);
                     }
@@ -528,10 +530,10 @@ __global__ __launch_bounds__(64 * W) void lsr_sample_team_kernel(const typename 
         team_sync<W>();
         for (int i = tid; i < row.steps; i += THREADS) mass[i] = 0;
         team_sync<W>();
-        const bool all = last == -INFINITY;
+        const bool all = last == least && last_class == n_classes;      // not cut
         row.template each<2>([&](int step, const float(&v)[RUN], int c) {
             uint64_t sum = 0;
-            if (all) {                                        // what is absent weighs nothing
+            if (all) {                                    // what is below `least` weighs nothing
 #pragma unroll
                 for (int j = 0; j < RUN; ++j)
                     sum += (uint64_t)__double_as_longlong(row_exp2(((double)v[j] - best) * unit) + a.magic);
@@ -721,7 +723,7 @@ __global__ __launch_bounds__(LSR_ROW_THREADS) void lsr_sample_quad_kernel(const 
         lane[g] = (w[4 * g] + w[4 * g + 1]) + (w[4 * g + 2] + w[4 * g + 3]);
         total += quad_sum(lane[g]);
     }
-    const double goal = (double)uniform[r] * total;
+    const double goal = (double)fmaxf(uniform[r], 0.0f) * total;         // the first class for NaN
     double base = 0;
     int at = 1 << 30, end = -1;
 #pragma unroll

@@ -72,16 +72,61 @@ __global__ __launch_bounds__(64 * W) void lsr_top_team_kernel(const typename row
         if (!N) row.open(mine, n_classes);
         team_groups(row, list);
         float below = 0.0f;
-        float bound = team_collect<REST>(row, kk, list, unit, below, mine + (r + gridDim.x < n_rows ? gridDim.x * row_stride : 0));
+        float bound = team_bound(kk, list);
+        team_take<REST>(row, bound, list, unit, below, mine + (r + gridDim.x < n_rows ? gridDim.x * row_stride : 0));
         team_row<DT, W, 0> again;                         // for the cases that need the row once more
         again.open(mine, n_classes);
         int n = list.n, bound_class = -1;                 // collected: above the bound, or equal up to this class
         bool equal = true;                                // every score that equals the bound is collected
+        if (n > ROOM) {                                   // thousands of equal scores, as a rule: first what is above them
+            equal = false;
+            if (tid == 0) list.n = 0;
+            team_sync<W>();
+            again.template each<4>([&](int, const float(&v)[RUN], int c) {
+#pragma unroll
+                for (int j = 0; j < RUN; ++j)
+                    if (v[j] > bound) {
+                        const int at = atomicAdd(&list.n, 1);
+                        if (at < ROOM) list.entry[at] = row_entry(row_key(v[j]), c + j);
+                    }
+            });
+            team_sync<W>();
+            n = list.n;
+            // then, in the order of their classes, as many of them as are missing: a masked row is done after one step
+#pragma unroll 1
+            for (int step = 0; step < again.steps && n < kk; ++step) {
+                float v[RUN];
+                again.decode(again.read_any(step), v);
+                int own = 0, sum = 0;
+#pragma unroll
+                for (int j = 0; j < RUN; ++j) own += v[j] == bound;
+                int run = wave_running(own);
+                team_sync<W>();
+                if ((tid & 63) == 63) hist[tid >> 6] = run;
+                team_sync<W>();
+#pragma unroll
+                for (int i = 0; i < W; ++i) {
+                    if (i < (tid >> 6)) run += hist[i];
+                    sum += hist[i];
+                }
+                int place = n + run - own;
+#pragma unroll
+                for (int j = 0; j < RUN; ++j)
+                    if (v[j] == bound) {
+                        if (place < kk) list.entry[place] = row_entry(row_key(v[j]), again.first_class(step) + j);
+                        ++place;
+                    }
+                n = min(n + sum, kk);
+                if (n == kk) {
+                    team_sync<W>();
+                    bound_class = (int)~(uint32_t)list.entry[kk - 1];
+                }
+            }
+        }
         if (n > ROOM) {
             const uint64_t least = top_radix<DT, W>(mine, n_classes, kk, hist, &one);
             bound = row_value((uint32_t)(least >> 32));
             bound_class = (int)~(uint32_t)least;
-            equal = false;
             if (tid == 0) list.n = 0;
             team_sync<W>();
             again.template each<1>([&](int, const float(&v)[RUN], int c) {
@@ -93,6 +138,7 @@ __global__ __launch_bounds__(64 * W) void lsr_top_team_kernel(const typename row
             team_sync<W>();
             n = list.n;
         }
+        team_sync<W>();
 #pragma unroll 1
         for (int i = tid; i < n; i += THREADS) {
             const uint64_t e = list.entry[i];

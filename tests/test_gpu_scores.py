@@ -161,6 +161,48 @@ def test_sample_scores_on_the_borders(classes):
         _check_sample(view, x, u, 1.0, top_k, top_p, 0.0)
 
 
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("classes", [11, 58, 100, 1000, 8200, 20011, 70001])
+def test_rows_masked_with_the_lowest_number(classes, dtype):
+    """Nearly all scores are the type's lowest number: it has no weight, so that not even a uniform number of 0 draws it,
+    but it is an entry of the row for top_scores."""
+    rng = np.random.default_rng(classes)
+    x = rng.normal(size=(8, classes))
+    lowest = torch.finfo(TYPES[dtype]).min
+    for r, allowed in enumerate([1, 2, 3, 5, 8, 10, 10, 0]):
+        masked = np.ones(classes, bool)
+        masked[rng.permutation(classes)[:allowed]] = False
+        masked[0] = True
+        x[r, masked] = lowest
+    x[6, classes // 2:] = -np.inf                         # and some are not there at all
+    x[6, -1] = 0.5
+    view, x = _device(x, dtype, pad=3)
+    u = np.array([0.0, 1.0, 0.0, 0.3, 0.0, 0.9, 0.0, 0.0])
+    for t, top_k, top_p, min_p in [(1.0, 0, 1.0, 0.0), (1.0, 6, 1.0, 0.0), (0.7, 9, 0.9, 0.0), (1.0, 300, 1.0, 0.0),
+                                   (2.0, 400, 0.95, 0.0), (1.0, 0, 0.95, 0.0), (1.0, 0, 0.95, 0.01), (1.5, 0, 1.0, 0.05)]:
+        _check_sample(view, x, u, t, top_k, top_p, min_p)
+    for k in sorted({1, 4, 9, min(classes, 64), min(classes, 256)}):
+        _check_top(view, x, k, 1.0)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("classes", [1000, 8200, 70001])
+def test_top_scores_of_many_equal_ones(classes, dtype):
+    """More equal scores at the last places than a list has room for: the first classes of them are taken."""
+    rng = np.random.default_rng(classes)
+    x = np.full((6, classes), 1.0)
+    x[1, rng.permutation(classes)[:30]] = 2.0
+    x[2, rng.permutation(classes)[:classes // 4]] = 0.5
+    x[3, rng.permutation(classes)[:classes // 3]] = np.nan
+    x[3, 7] = 3.0
+    x[4] = np.where(rng.random(classes) < 0.1, 4.0, 5.0)
+    x[5, ::2] = 1.5
+    x[5, :3 * classes // 4] = -np.inf
+    view, x = _device(x, dtype, pad=1)
+    for k in [1, 5, 29, 30, 31, 64, 255, 256]:
+        _check_top(view, x, k, 1.0)
+
+
 def test_sample_scores_distribution():
     """The share of each class over evenly spread uniform numbers is its probability to within one number per border."""
     from loe_speech_recognition_amd import sample_scores
