@@ -422,6 +422,19 @@ extern "C" int lsr_distill_scores(lsr_ctx* ctx, const void* scores_d, int dtype,
     if ((uintptr_t)grad_d % row_dtype_bytes(dtype))
         return lsr_fail(ctx, LSR_ERR_ARG, "lsr_distill_scores: gradient is not aligned to its element size");
     LSR_HIP_CHECK(ctx, hipSetDevice(ctx->device));
+    const int64_t most = lsr_launch_rows(n_classes);
+    if (n_rows > most) {
+        const int bytes = row_dtype_bytes(dtype);
+        for (int64_t r = 0; r < n_rows; r += most) {
+            const int failed = lsr_distill_scores(ctx, (const char*)scores_d + r * row_stride * bytes, dtype,
+                                                  n_rows - r < most ? n_rows - r : most, n_classes, row_stride,
+                                                  top_values_d + r * k, top_index_d + r * k, k, rest_d ? rest_d + r : nullptr,
+                                                  temperature, row_weight_d ? row_weight_d + r : nullptr, loss_d + r,
+                                                  grad_d ? (char*)grad_d + r * n_classes * bytes : nullptr);
+            if (failed) return failed;
+        }
+        return LSR_OK;
+    }
     lsr_prof_begin(ctx, LSR_K_DISTILL);
     if (n_classes <= LSR_QUAD_CLASSES) {
         LSR_DTYPE_SWITCH(dtype, LSR_QUAD_SWITCH(n_classes, lsr_distill_quad<DT, E>(ctx->stream, scores_d, n_rows, (int)n_classes,

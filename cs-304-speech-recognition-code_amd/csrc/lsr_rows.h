@@ -89,6 +89,9 @@ __device__ __forceinline__ uint64_t row_fixed(double w, double magic) {
 
 static inline int row_dtype_bytes(int dtype) { return dtype == LSR_F32 ? 4 : 2; }
 
+// Rows of one launch: a grid has fewer than 2^32 threads.  The entry points take more rows in several launches.
+static inline int64_t lsr_launch_rows(int64_t n_classes) { return n_classes <= 128 ? (int64_t)1 << 29 : (int64_t)1 << 21; }
+
 // argument checks common to the three entry points; 0 or an error code with its message set
 int lsr_check_rows(lsr_ctx* ctx, const char* name, const void* scores_d, int dtype, int64_t n_rows, int64_t n_classes,
                    int64_t row_stride);

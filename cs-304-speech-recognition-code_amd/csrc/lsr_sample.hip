@@ -784,6 +784,18 @@ extern "C" int lsr_sample_scores(lsr_ctx* ctx, const void* scores_d, int dtype, 
     if (n_rows == 0) return LSR_OK;
     if (!uniform_d || !index_d || !logprob_d) return lsr_fail(ctx, LSR_ERR_ARG, "lsr_sample_scores: null pointer");
     LSR_HIP_CHECK(ctx, hipSetDevice(ctx->device));
+    const int64_t most = lsr_launch_rows(n_classes);
+    if (n_rows > most) {
+        for (int64_t r = 0; r < n_rows; r += most) {
+            const int failed = lsr_sample_scores(ctx, (const char*)scores_d + r * row_stride * row_dtype_bytes(dtype), dtype,
+                                                 n_rows - r < most ? n_rows - r : most, n_classes, row_stride, uniform_d + r,
+                                                 temperature, top_k, top_p, min_p, temperature_d ? temperature_d + r : nullptr,
+                                                 top_k_d ? top_k_d + r : nullptr, top_p_d ? top_p_d + r : nullptr,
+                                                 min_p_d ? min_p_d + r : nullptr, index_d + r, logprob_d + r);
+            if (failed) return failed;
+        }
+        return LSR_OK;
+    }
     // weights of up to n_classes entries have to fit 62 bits together
     int shift = 62;
     for (int64_t n = 1; n < n_classes; n *= 2) --shift;

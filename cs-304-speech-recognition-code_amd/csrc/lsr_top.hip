@@ -287,6 +287,16 @@ extern "C" int lsr_top_scores(lsr_ctx* ctx, const void* scores_d, int dtype, int
     if (n_rows == 0) return LSR_OK;
     if (!values_d || !index_d) return lsr_fail(ctx, LSR_ERR_ARG, "lsr_top_scores: null pointer");
     LSR_HIP_CHECK(ctx, hipSetDevice(ctx->device));
+    const int64_t most = lsr_launch_rows(n_classes);
+    if (n_rows > most) {
+        for (int64_t r = 0; r < n_rows; r += most) {
+            const int failed = lsr_top_scores(ctx, (const char*)scores_d + r * row_stride * row_dtype_bytes(dtype), dtype,
+                                              n_rows - r < most ? n_rows - r : most, n_classes, row_stride, k, temperature,
+                                              values_d + r * k, index_d + r * k, rest_d ? rest_d + r : nullptr);
+            if (failed) return failed;
+        }
+        return LSR_OK;
+    }
     const float inv_t = (float)(1.0 / temperature);
     lsr_prof_begin(ctx, LSR_K_TOP);
     if (n_classes <= LSR_QUAD_CLASSES) {

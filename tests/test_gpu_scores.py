@@ -361,6 +361,46 @@ def test_offsets_beyond_32_bits():
         assert torch.equal(a, b)
 
 
+def test_more_rows_than_one_launch_takes():
+    """2^21 rows of more than 128 classes are a launch; what lies beyond is read and written at its own place."""
+    from loe_speech_recognition_amd import distill_scores, sample_scores, top_scores
+
+    rng = np.random.default_rng(21)
+    n = 2 ** 21 + 3
+    view, x = _device(_matrix(rng, 1, 130, hard=False), "f32")
+    rows = view.expand(n, -1)
+    u = torch.zeros(n, device="cuda")
+    u[-2:] = torch.tensor([0.4, 0.999], device="cuda")
+    values, index, rest = top_scores(rows, 2, want_rest=True)
+    v, i, q = R.top(x[0], 2, 1.0)
+    assert (index == torch.tensor(i, device="cuda")).all() and (values[-3:].cpu().numpy() == v).all()
+    assert (rest == rest[0]).all() and abs(rest[0].item() - q) <= _sum_error(130, _span(x[0], 1.0)) + 2.0 ** -22 * abs(q)
+    drawn, logprob = sample_scores(rows, u)
+    want = [R.sample(x[0], float(a), 1.0, 0, 1.0, 0.0)[0] for a in u[-3:].tolist()]
+    assert drawn[-3:].tolist() == want and (drawn[:-2] == want[0]).all() and (logprob[:-2] == logprob[0]).all()
+    loss, grad = distill_scores(rows, values, index, rest=rest)
+    assert (loss == loss[0]).all() and (grad[-4:] == grad[0]).all()
+    del loss, grad
+
+
+def test_rows_masked_in_a_long_batch():
+    """Workgroups that go on from row to row meet rows whose equal scores overflow the list between ordinary ones."""
+    rng = np.random.default_rng(8)
+    x = torch.tensor(rng.normal(size=(700, 66000)), dtype=torch.bfloat16)
+    for r in range(0, 700, 3):
+        x[r, rng.random(66000) > 1e-3] = torch.finfo(x.dtype).min
+    from loe_speech_recognition_amd import top_scores
+
+    for want_rest in (False, True):
+        values, index, rest = top_scores(x.cuda(), 200, want_rest=want_rest)
+        for r in [*range(0, 12), *range(253, 262), *range(508, 520), *range(690, 700)]:
+            v, i, q = R.top(x[r].double().numpy(), 200, 1.0)
+            assert np.array_equal(index[r].cpu().numpy(), i) and np.array_equal(values[r].double().cpu().numpy(), v), r
+            if want_rest:
+                tol = _sum_error(66000, _span(x[r].double().numpy(), 1.0)) + 2.0 ** -22 * abs(q)
+                assert abs(rest[r].item() - q) <= tol, (r, rest[r].item(), q)
+
+
 def test_no_rows():
     from loe_speech_recognition_amd import distill_scores, sample_scores, top_scores
 
