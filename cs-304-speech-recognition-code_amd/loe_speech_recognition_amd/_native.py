@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import threading
 from ctypes import POINTER, c_char_p, c_double, c_float, c_int, c_int32, c_int64, c_uint8, c_void_p
 from typing import List, Optional, Sequence, Tuple
 
@@ -223,6 +224,7 @@ class Engine:
         self._rotated = {}               # token -> triangularised whitening matrices (at most 8 kept)
         # models resident on the device: token -> (slot, states); slot 0 takes the uploads without a token
         self._resident = {}
+        self._turn = threading.Lock()
         self._slot = 0
         self._between = None
 
@@ -262,27 +264,29 @@ class Engine:
     def on_current_stream(self, fn, *args) -> None:
         """``fn(ctx, *args)`` on torch's current stream, after the work already queued on the engine's stream (the two are
         usually one).  For entry points that use no workspace of the context.  While the current stream is captured the
-        engine's earlier work is not waited for: a capture starts from finished work."""
-        cuda = self.torch.cuda
-        before = cuda.current_device()
-        handle = self._raw_stream(self.device_index)
-        try:
-            if handle == self._stream_handle:
-                rc = fn(self.ctx, *args)
-            else:
-                stream = cuda.current_stream(self.device)
-                if not cuda.is_current_stream_capturing():
-                    stream.wait_stream(self._stream)
-                self._check(self.lib.lsr_set_stream(self.ctx, c_void_p(handle)))
-                try:
+        engine's earlier work is not waited for: a capture starts from finished work.  Threads that call this at once take
+        turns; the engine's other calls belong to one thread, as the context does."""
+        with self._turn:
+            cuda = self.torch.cuda
+            before = cuda.current_device()
+            handle = self._raw_stream(self.device_index)
+            try:
+                if handle == self._stream_handle:
                     rc = fn(self.ctx, *args)
-                finally:
-                    self._check(self.lib.lsr_set_stream(self.ctx, c_void_p(self._stream_handle)))
-        finally:
-            if before != self.device_index:              # the library makes its own device the current one
-                cuda.set_device(before)
-        if rc:
-            self._check(rc)
+                else:
+                    stream = cuda.current_stream(self.device)
+                    if not cuda.is_current_stream_capturing():
+                        stream.wait_stream(self._stream)
+                    self._check(self.lib.lsr_set_stream(self.ctx, c_void_p(handle)))
+                    try:
+                        rc = fn(self.ctx, *args)
+                    finally:
+                        self._check(self.lib.lsr_set_stream(self.ctx, c_void_p(self._stream_handle)))
+            finally:
+                if before != self.device_index:              # the library makes its own device the current one
+                    cuda.set_device(before)
+            if rc:
+                self._check(rc)
 
     @staticmethod
     def _ptr(t) -> c_void_p:

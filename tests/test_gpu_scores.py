@@ -522,6 +522,34 @@ def test_two_captured_graphs(rows, classes, dtype):
                 assert torch.equal(a, b), turn
 
 
+def test_threads_on_streams_of_their_own():
+    import threading
+
+    from loe_speech_recognition_amd import sample_scores, top_scores
+
+    rng = np.random.default_rng(31)
+    views = [_device(_matrix(rng, 40, 1000 + 100 * i, hard=False), "f32")[0] for i in range(4)]
+    u = torch.tensor(rng.random(40), dtype=torch.float32, device="cuda")
+    want = [(top_scores(v, 9)[1], sample_scores(v, u, 0.9, 50, 0.95)[0]) for v in views]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(50):
+                x = views[i] + 0.0                        # on this thread's stream: a call on another one could overtake it
+                got = top_scores(x, 9)[1], sample_scores(x, u, 0.9, 50, 0.95)[0]
+                if not all(bool(torch.equal(a, b)) for a, b in zip(got, want[i])):
+                    wrong.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
 def test_same_bits_in_any_batch():
     """A row's results do not depend on the rows around it nor on how often it is run."""
     from loe_speech_recognition_amd import distill_scores
