@@ -109,6 +109,7 @@ int lsr_check_rows(lsr_ctx* ctx, const char* name, const void* scores_d, int dty
 template <int PERM> __device__ __forceinline__ int quad_move(int v) {
     return __builtin_amdgcn_mov_dpp(v, PERM, 0xf, 0xf, true);
 }
+template <int PERM> __device__ __forceinline__ uint32_t quad_move(uint32_t v) { return (uint32_t)quad_move<PERM>((int)v); }
 template <int PERM> __device__ __forceinline__ float quad_move(float v) {
     return __int_as_float(quad_move<PERM>(__float_as_int(v)));
 }
@@ -345,7 +346,8 @@ template <int CTRL, int ROWS> __device__ __forceinline__ double wave_shift(doubl
     } while (0)
 template <typename V> __device__ __forceinline__ V row_add(V a, V b) { return a + b; }
 __device__ __forceinline__ uint64_t row_max(uint64_t a, uint64_t b) { return a > b ? a : b; }
-__device__ __forceinline__ int row_max(int a, int b) { return max(a, b); }
+__device__ __forceinline__ uint32_t row_max(uint32_t a, uint32_t b) { return max(a, b); }
+__device__ __forceinline__ uint32_t row_min(uint32_t a, uint32_t b) { return min(a, b); }
 
 __device__ __forceinline__ float wave_last(float v) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63)); }
 __device__ __forceinline__ int wave_last(int v) { return __builtin_amdgcn_readlane(v, 63); }
@@ -654,6 +656,111 @@ template <int W, int SIZE> __device__ __forceinline__ int team_above(const team_
 #pragma unroll 8
     for (int i = 0; i < n; ++i) above += list.entry[i] > e;
     return above;
+}
+
+// Sorting 64 E numbers of a wavefront, largest first; lane l has the places l E ... l E + E - 1.  A bitonic network whose
+// merges begin with a mirrored step, so that every step keeps the larger number in the lower place.
+template <int X, typename V> __device__ __forceinline__ V wave_xor(V v) {              // of lane l ^ X
+    if constexpr (X == 1) return quad_move<QUAD_XOR1>(v);
+    else if constexpr (X == 2) return quad_move<QUAD_XOR2>(v);
+    else if constexpr (X == 3) return quad_move<QUAD_XOR3>(v);
+    else if constexpr (X == 7) return quad_move<0x141>(v);               // the halves of 16 lanes mirrored
+    else if constexpr (X == 8) return quad_move<0x128>(v);               // 16 lanes rotated by 8
+    else if constexpr (X == 15) return quad_move<0x140>(v);              // 16 lanes mirrored
+    else return __shfl_xor(v, X);
+}
+template <int E, typename V> __device__ __forceinline__ void wave_sort_own(V (&e)[E]) {
+#pragma unroll
+    for (int s = E / 2; s; s /= 2)
+#pragma unroll
+        for (int i = 0; i < E; ++i)
+            if (!(i & s)) {
+                const V a = e[i], b = e[i + s];
+                e[i] = row_max(a, b);
+                e[i + s] = row_min(a, b);
+            }
+}
+template <int X, bool MIRROR, int E, typename V> __device__ __forceinline__ void wave_sort_step(V (&e)[E]) {
+    const bool upper = threadIdx.x & (MIRROR ? (X + 1) / 2 : X);
+    V o[E];
+#pragma unroll
+    for (int i = 0; i < E; ++i) o[i] = wave_xor<X>(e[MIRROR ? E - 1 - i : i]);
+#pragma unroll
+    for (int i = 0; i < E; ++i) e[i] = upper ? row_min(e[i], o[i]) : row_max(e[i], o[i]);
+}
+template <int M, int E, typename V> __device__ __forceinline__ void wave_sort_merge(V (&e)[E]) {      // over M lanes
+    wave_sort_step<M - 1, true>(e);
+    if constexpr (M > 32) wave_sort_step<16, false>(e);
+    if constexpr (M > 16) wave_sort_step<8, false>(e);
+    if constexpr (M > 8) wave_sort_step<4, false>(e);
+    if constexpr (M > 4) wave_sort_step<2, false>(e);
+    if constexpr (M > 2) wave_sort_step<1, false>(e);
+    wave_sort_own(e);
+}
+template <int E, typename V> __device__ __forceinline__ void wave_sort(V (&e)[E]) {
+#pragma unroll
+    for (int k = 2; k <= E; k *= 2) {
+        // pairs that are mirrored in their group of k
+#pragma unroll
+        for (int i = 0; i < E; ++i)
+            if ((i & (k - 1)) < k / 2) {
+                const int j = (i & ~(k - 1)) + k - 1 - (i & (k - 1));
+                const V a = e[i], b = e[j];
+                e[i] = row_max(a, b);
+                e[j] = row_min(a, b);
+            }
+#pragma unroll
+        for (int s = k / 4; s; s /= 2)
+#pragma unroll
+            for (int i = 0; i < E; ++i)
+                if (!(i & s)) {
+                    const V a = e[i], b = e[i + s];
+                    e[i] = row_max(a, b);
+                    e[i + s] = row_min(a, b);
+                }
+    }
+    wave_sort_merge<2>(e);
+    wave_sort_merge<4>(e);
+    wave_sort_merge<8>(e);
+    wave_sort_merge<16>(e);
+    wave_sort_merge<32>(e);
+    wave_sort_merge<64>(e);
+}
+// Puts the first 64 E entries of a list of n in order, by one wavefront.  Key and class take 56 bits and are compared as
+// floating-point numbers, for which there is an instruction.
+template <int E, int W, int SIZE> __device__ __forceinline__ void team_sort(const team_list<W, SIZE>& list, int n, uint64_t* sorted, int room) {
+    double e[E];
+    const int lane = threadIdx.x;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        const uint64_t u = i * 64 + lane < n ? list.entry[i * 64 + lane] : 0;
+        e[i] = __longlong_as_double((long long)(u >> 32 << 24 | (u & 0xffffffu)));
+    }
+    wave_sort(e);
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        const uint64_t u = (uint64_t)__double_as_longlong(e[i]);
+        if (lane * E + i < room) sorted[lane * E + i] = u >> 24 << 32 | 0xff000000u | (u & 0xffffffu);
+    }
+}
+// The list's entries by place, `room` of them at most.  Up to 128 are compared with all others, more are sorted: the
+// comparisons wait for shared memory, one read for every 64 of them.
+template <int W, int SIZE> __device__ __forceinline__ void team_order(const team_list<W, SIZE>& list, int n, uint64_t* sorted, int room) {
+    if (n > 128 && n <= 512) {
+        if (threadIdx.x < 64) {
+            if (n <= 256)
+                team_sort<4>(list, n, sorted, room);
+            else
+                team_sort<8>(list, n, sorted, room);
+        }
+        return;
+    }
+#pragma unroll 1
+    for (int i = threadIdx.x; i < n; i += 64 * W) {
+        const uint64_t e = list.entry[i];
+        const int place = team_above(list, n, e);
+        if (place < room) sorted[place] = e;
+    }
 }
 
 // Wavefronts per row by the row's width, W, and the runs of it that a thread keeps in registers, N; LSR_WAVES_SWITCH for an

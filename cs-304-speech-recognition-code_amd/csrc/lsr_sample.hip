@@ -277,12 +277,7 @@ __global__ __launch_bounds__(64 * W) void lsr_sample_team_kernel(const typename 
         team_take<false>(row, row_max(bound, least), list, 0.0f, none, mine);
         const int n = list.n;
         if (n <= (level ? LSR_MAX_TOP : ROOM)) {
-#pragma unroll 1
-            for (int i = tid; i < n; i += THREADS) {
-                const uint64_t e = list.entry[i];
-                const int place = team_above(list, n, e);
-                if (place < LSR_MAX_TOP) sorted[place] = e;
-            }
+            team_order(list, n, sorted, LSR_MAX_TOP);
             // weight of the row, where the list does not hold what top_p is a share of; where the level's entries weigh
             // less than that share by more than the guess can be off, top_p takes nothing away
             uint64_t all = 0;
@@ -339,6 +334,36 @@ __global__ __launch_bounds__(64 * W) void lsr_sample_team_kernel(const typename 
             team_sync<W>();
             const int kept = n_kept;
             const uint64_t goal = sample_goal(u, kept_sum);
+            auto answer = [&](uint64_t e) {
+                index[r] = (int32_t)~(uint32_t)e;
+                logprob[r] = (float)(((double)row_value((uint32_t)(e >> 32)) - best) / t - row_log((double)kept_sum * a.unit));
+            };
+            if (kept > 64) {                              // in the order of their classes, the weights added up
+                if (tid < 64) {
+                    constexpr int FOUR = LSR_MAX_TOP / 64;
+                    static_assert(LSR_MAX_TOP <= 256 && LSR_MAX_CLASSES <= 1 << 24, "class and place in 32 bits");
+                    uint32_t c[FOUR];
+#pragma unroll
+                    for (int i = 0; i < FOUR; ++i) {
+                        const int place = i * 64 + tid;
+                        c[i] = place < kept ? (uint32_t)sorted[place] << 8 | place : 0;  // classes are complemented
+                    }
+                    wave_sort(c);
+                    uint64_t own = 0, w[FOUR];
+#pragma unroll
+                    for (int i = 0; i < FOUR; ++i) {
+                        w[i] = tid * FOUR + i < kept ? mass[c[i] & 255] : 0;
+                        own += w[i];
+                    }
+                    uint64_t run = wave_running(own) - own;
+#pragma unroll
+                    for (int i = 0; i < FOUR; ++i) {
+                        if (tid * FOUR + i < kept && (goal == 0 ? tid + i == 0 : run <= goal && goal < run + w[i])) answer(sorted[c[i] & 255]);
+                        run += w[i];
+                    }
+                }
+                return;
+            }
 #pragma unroll 1
             for (int i = tid; i < kept; i += THREADS) {
                 // weight of the kept entries of lower classes
@@ -347,15 +372,11 @@ __global__ __launch_bounds__(64 * W) void lsr_sample_team_kernel(const typename 
                 int ahead = 0;
 #pragma unroll 8
                 for (int j = 0; j < kept; ++j) {
-                    const bool lower = (uint32_t)sorted[j] > own;                // classes are complemented
+                    const bool lower = (uint32_t)sorted[j] > own;
                     before += lower ? mass[j] : 0;
                     ahead += lower;
                 }
-                if (goal == 0 ? ahead == 0 : before <= goal && goal < before + mass[i]) {
-                    const float v = row_value((uint32_t)(sorted[i] >> 32));
-                    index[r] = (int32_t)~own;
-                    logprob[r] = (float)(((double)v - best) / t - row_log((double)kept_sum * a.unit));
-                }
+                if (goal == 0 ? ahead == 0 : before <= goal && goal < before + mass[i]) answer(sorted[i]);
             }
             if (kept > 0) return;
         }

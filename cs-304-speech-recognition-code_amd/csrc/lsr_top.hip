@@ -139,11 +139,7 @@ __global__ __launch_bounds__(64 * W) void lsr_top_team_kernel(const typename row
             n = list.n;
         }
         team_sync<W>();
-#pragma unroll 1
-        for (int i = tid; i < n; i += THREADS) {
-            const uint64_t e = list.entry[i];
-            sorted[team_above(list, n, e)] = e;
-        }
+        team_order(list, n, sorted, ROOM);
         team_sync<W>();
         for (int i = tid; i < k; i += THREADS) {          // places without an entry: -infinity, -1
             const uint64_t e = i < n ? sorted[i] : 0;
