@@ -596,8 +596,8 @@ __device__ __forceinline__ float team_groups(team_row<DT, W, N>& row, team_list<
 }
 // Collects the entries that reach `bound`; `list.n`, 0 on entry, may exceed the list's size: then only some of them are there.
 // SUM: also this thread's sum of e^((x - bound) unit ln 2) over what stays below the bound, in the same pass; NaN where the
-// thread has seen one.  A kept row of a team of 16 is asked for the next row, `next`, on the way.
-template <bool SUM, int DT, int W, int N, int SIZE>
+// thread has seen one.  NEXT: a kept row is asked for the next row, `next`, on the way.
+template <bool SUM, bool NEXT, int DT, int W, int N, int SIZE>
 __device__ __forceinline__ void team_take(team_row<DT, W, N>& row, float bound, team_list<W, SIZE>& list, float unit, float& below,
                                           const typename row_type<DT>::type* next) {
     constexpr int RUN = team_row<DT, W, N>::RUN;
@@ -623,7 +623,7 @@ __device__ __forceinline__ void team_take(team_row<DT, W, N>& row, float bound, 
             for (int j = 0; j < RUN; ++j) below += __builtin_amdgcn_exp2f((v[j] - bound) * unit);
         }
     };
-    if (W == 16 && N)                                     // (smaller teams take one row each)
+    if constexpr (NEXT)
         row.each_run_then(next, take);
     else
         row.template each_run<4>(take);
@@ -743,10 +743,10 @@ template <int E, int W, int SIZE> __device__ __forceinline__ void team_sort(cons
         if (lane * E + i < room) sorted[lane * E + i] = u >> 24 << 32 | 0xff000000u | (u & 0xffffffu);
     }
 }
-// The list's entries by place, `room` of them at most.  Up to 128 are compared with all others, more are sorted: the
-// comparisons wait for shared memory, one read for every 64 of them.
-template <int W, int SIZE> __device__ __forceinline__ void team_order(const team_list<W, SIZE>& list, int n, uint64_t* sorted, int room) {
-    if (n > 128 && n <= 512) {
+// The list's entries by place, `room` of them at most.  Up to 128 are compared with all others, more are sorted if SORT: the
+// comparisons wait for shared memory, one read for every 64 of them (4096 x 1000, k = 200: 76 us, sorted 27).
+template <bool SORT, int W, int SIZE> __device__ __forceinline__ void team_order(const team_list<W, SIZE>& list, int n, uint64_t* sorted, int room) {
+    if (SORT && n > 128 && n <= 512) {
         if (threadIdx.x < 64) {
             if (n <= 256)
                 team_sort<4>(list, n, sorted, room);

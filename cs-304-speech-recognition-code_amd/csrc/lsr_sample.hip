@@ -274,10 +274,10 @@ __global__ __launch_bounds__(64 * W) void lsr_sample_team_kernel(const typename 
         float none = 0, bound = few || nucleus ? team_bound(few ? top_k : NUCLEUS < n_classes ? NUCLEUS : n_classes, list) : floor;
         if (level && tid == 0) list.n = 0;
         if (level) team_sync<W>();
-        team_take<false>(row, row_max(bound, least), list, 0.0f, none, mine);
+        team_take<false, false>(row, row_max(bound, least), list, 0.0f, none, mine);
         const int n = list.n;
         if (n <= (level ? LSR_MAX_TOP : ROOM)) {
-            team_order(list, n, sorted, LSR_MAX_TOP);
+            team_order<true>(list, n, sorted, LSR_MAX_TOP);
             // weight of the row, where the list does not hold what top_p is a share of; where the level's entries weigh
             // less than that share by more than the guess can be off, top_p takes nothing away
             uint64_t all = 0;

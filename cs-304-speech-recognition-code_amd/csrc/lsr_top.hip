@@ -45,9 +45,11 @@ __device__ __forceinline__ uint64_t top_radix(const typename row_type<DT>::type*
     return threshold;
 }
 
-// Long rows, a team of W wavefronts per row (lsr_rows.h).  Workgroups of 16 wavefronts with kept rows fill their compute
-// unit alone; there are as many of them as compute units, and each requests its next row while it collects from this one.
-template <int DT, int W, int N, bool REST>
+// Long rows, a team of W wavefronts per row (lsr_rows.h).  ON: workgroups of 16 wavefronts with kept rows fill their compute
+// unit alone; there are as many of them as compute units, and each requests its next row while it collects from this one
+// (2048 x 131072, k = 64: 168 us against 186 with a workgroup per row).  The registers that this takes are missing for the
+// sorting of longer lists, so that it is for k <= 64, whose lists have about 80 entries.
+template <int DT, int W, int N, bool ON, bool REST>
 __global__ __launch_bounds__(64 * W) void lsr_top_team_kernel(const typename row_type<DT>::type* __restrict__ scores,
                                                               int64_t n_rows, int n_classes, int64_t row_stride, int k,
                                                               float inv_t, float* __restrict__ values,
@@ -58,7 +60,6 @@ __global__ __launch_bounds__(64 * W) void lsr_top_team_kernel(const typename row
     __shared__ uint64_t one;
     __shared__ uint64_t sorted[ROOM];                     // by place: the list itself is in the order in which it was filled
     __shared__ float part[W];
-    constexpr bool ON = W == 16 && N > 0;                 // goes on to further rows
     int tid = threadIdx.x;
     const int kk = k + (REST ? 1 : 0);                    // the first entry of the rest as well
     const float unit = inv_t * 1.44269504f;
@@ -73,7 +74,7 @@ __global__ __launch_bounds__(64 * W) void lsr_top_team_kernel(const typename row
         team_groups(row, list);
         float below = 0.0f;
         float bound = team_bound(kk, list);
-        team_take<REST>(row, bound, list, unit, below, mine + (r + gridDim.x < n_rows ? gridDim.x * row_stride : 0));
+        team_take<REST, ON>(row, bound, list, unit, below, mine + (r + gridDim.x < n_rows ? gridDim.x * row_stride : 0));
         team_row<DT, W, 0> again;                         // for the cases that need the row once more
         again.open(mine, n_classes);
         int n = list.n, bound_class = -1;                 // collected: above the bound, or equal up to this class
@@ -139,7 +140,7 @@ __global__ __launch_bounds__(64 * W) void lsr_top_team_kernel(const typename row
             n = list.n;
         }
         team_sync<W>();
-        team_order(list, n, sorted, ROOM);
+        team_order<!ON>(list, n, sorted, ROOM);
         team_sync<W>();
         for (int i = tid; i < k; i += THREADS) {          // places without an entry: -infinity, -1
             const uint64_t e = i < n ? sorted[i] : 0;
@@ -183,13 +184,18 @@ static void lsr_top_team(lsr_ctx* ctx, const void* scores_d, int64_t n_rows, int
     // 64 registers of 32-bit scores and what the passes need do not fit together: 96 x 50001 with the rest takes 37 us kept
     // and spilling, 16.5 us read again
     constexpr int KEEP = DT == ROW_F32 && W == 16 ? 0 : N;
-    const dim3 grid((unsigned)(W == 16 && KEEP && n_rows > ctx->n_cus ? ctx->n_cus : n_rows)), block(64 * W);
-    if (rest_d)
-        hipLaunchKernelGGL((lsr_top_team_kernel<DT, W, KEEP, true>), grid, block, 0, ctx->stream, scores, n_rows, n_classes, row_stride, k,
-                           inv_t, values_d, index_d, rest_d);
-    else
-        hipLaunchKernelGGL((lsr_top_team_kernel<DT, W, KEEP, false>), grid, block, 0, ctx->stream, scores, n_rows, n_classes, row_stride, k,
-                           inv_t, values_d, index_d, rest_d);
+    const dim3 all((unsigned)n_rows), some((unsigned)ctx->n_cus), block(64 * W);
+#define LAUNCH(ON, REST)                                                                                                    \
+    hipLaunchKernelGGL((lsr_top_team_kernel<DT, W, KEEP, ON, REST>), ON ? some : all, block, 0, ctx->stream, scores, n_rows, \
+                       n_classes, row_stride, k, inv_t, values_d, index_d, rest_d)
+    if constexpr (W == 16 && KEEP > 0) {
+        if (n_rows > ctx->n_cus && k <= 64) {
+            if (rest_d) LAUNCH(true, true); else LAUNCH(true, false);
+            return;
+        }
+    }
+    if (rest_d) LAUNCH(false, true); else LAUNCH(false, false);
+#undef LAUNCH
 }
 
 // Short rows (at most LSR_QUAD_CLASSES classes), a quad per row: the entries are sorted by a network over the quad's
