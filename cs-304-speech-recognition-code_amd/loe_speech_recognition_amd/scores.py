@@ -110,7 +110,8 @@ def sample_scores(scores, uniform, temperature: Union[float, "torch.Tensor"] = 1
     ``w >= min_p`` (0: all); at least its best.  The result is the first class in ascending order at which the running
     weight of the kept classes exceeds ``uniform`` times their total, and the log of its share of that total.
     ``temperature`` 0 takes the best class.  Every setting is a number or a tensor [rows] (float32; int32 for ``top_k``)
-    with a number for each row.  Scores of -inf and NaN are never drawn; a row without others gives -1 and -inf."""
+    with a number for each row.  Scores of -inf and NaN are never drawn, nor are scores masked with a type's lowest number (or
+    others without weight in 64 bits, beyond 745 temperatures below the best); a row without others gives -1 and -inf."""
     import torch
 
     rows, classes, code = _check_scores(scores)

@@ -396,7 +396,9 @@ int lsr_top_scores(lsr_ctx* ctx, const void* scores_d, int dtype, int64_t n_rows
  * the log of its share of the total.  temperature <= 0 (or NaN in temperature_d): the row's first entry, log share 0.  A
  * row without entries: -1, -infinity.  If the row holds +infinity only those entries have weight.  Each setting is one
  * number for all rows or, where its pointer is not NULL, float32 / int32[n_rows].  Weights are computed in 64 bits and
- * summed as whole multiples of 2^-52 (up to 1 024 classes) ... 2^-38 (2^24 classes) of the best one's. */
+ * summed as whole multiples of 2^-52 (up to 1 024 classes) ... 2^-38 (2^24 classes) of the best one's.  A class whose
+ * weight is 0 in 64 bits (more than about 745 temperatures below the best, such as one masked with the type's lowest
+ * number) is never drawn. */
 int lsr_sample_scores(lsr_ctx* ctx, const void* scores_d, int dtype, int64_t n_rows, int64_t n_classes, int64_t row_stride,
                       const float* uniform_d, double temperature, int top_k, double top_p, double min_p,
                       const float* temperature_d, const int32_t* top_k_d, const float* top_p_d, const float* min_p_d,
