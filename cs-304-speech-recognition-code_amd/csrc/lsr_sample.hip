@@ -254,6 +254,30 @@ __global__ __launch_bounds__(64 * W) void lsr_sample_team_kernel(const typename 
     };
     if (best == INFINITY) return slowly();
 
+    float last = least;                                   // kept: above this score, or equal up to this class
+    int last_class = n_classes;
+    auto keeps = [&](float v, int c) { return (v > last) | ((v == last) & (c <= last_class)); };
+    auto weigh = [&](float v) { return row_fixed(row_exp2(((double)v - best) * unit), a.magic); };
+    const float per_bin = (float)fmin(BINS / 24.0 / t, 1e30);
+    auto bin_of = [&](float v) { return (int)fminf((best - v) * per_bin, (float)(BINS - 1)); };
+
+    auto cut_at = [&](uint64_t e) {
+        last = row_value((uint32_t)(e >> 32));
+        last_class = (int)~(uint32_t)e;
+    };
+    const uint64_t zero = (uint64_t)__double_as_longlong(a.magic);
+    bool summed = false;                                  // the weights of the steps are known already
+    // adds the weights of the list's entries that are kept to those of their steps
+    auto tally = [&](int n) {
+        for (int i = tid; i < n; i += THREADS) {
+            const uint64_t e = list.entry[i];
+            const int c = (int)~(uint32_t)e;
+            if (keeps(row_value((uint32_t)(e >> 32)), c))
+                atomicAdd((unsigned long long*)&mass[c / Row::STEP], (unsigned long long)list_mass[i]);
+        }
+        summed = true;
+    };
+
     // Rows that are answered from a list of their first entries.  few: a small top_k.  level: min_p without top_k, when not
     // many entries reach it.  nucleus: top_p alone, where it looks as if a short head will do: where the best scores of the
     // groups hold that share of the row's weight.
@@ -278,8 +302,7 @@ __global__ __launch_bounds__(64 * W) void lsr_sample_team_kernel(const typename 
         if (level) team_sync<W>();
         team_take<false, false>(row, row_max(bound, least), list, 0.0f, none, mine);
         const int n = list.n;
-        if (n <= (level ? LSR_MAX_TOP : ROOM)) {
-            team_order<true>(list, n, sorted, LSR_MAX_TOP);
+        if (n <= ROOM) {
             // weight of the row, where the list does not hold what top_p is a share of; where the level's entries weigh
             // less than that share by more than the guess can be off, top_p takes nothing away
             uint64_t all = 0;
@@ -299,105 +322,105 @@ __global__ __launch_bounds__(64 * W) void lsr_sample_team_kernel(const typename 
                 });
                 all = team_sum<W>(all, part);
             }
-            team_sync<W>();
-            const int most = few ? top_k : LSR_MAX_TOP, m = n < most ? n : most;     // the list is the head of the row, all of it
-            if (tid < 64) {                               // lane l has the places 4 l ... 4 l + 3
-                constexpr int FOUR = LSR_MAX_TOP / 64;
-                uint64_t w[FOUR], own = 0;
-                float v[FOUR];
-#pragma unroll
-                for (int i = 0; i < FOUR; ++i) {
-                    const int place = tid * FOUR + i;
-                    v[i] = place < m ? row_value((uint32_t)(sorted[place] >> 32)) : -INFINITY;
-                    w[i] = row_fixed(row_exp2(((double)v[i] - best) * unit), a.magic);
-                    own += w[i];
-                }
-                uint64_t run = wave_running(own);
-                const uint64_t listed = wave_last(run), target = open ? ~0ull : sample_target(top_p, few ? listed : all);
-                run -= own;
+            if (level && n > LSR_MAX_TOP) {               // too many to put in order
+                for (int i = tid; i < n; i += THREADS) list_mass[i] = weigh(row_value((uint32_t)(list.entry[i] >> 32)));
+                for (int i = tid; i < row.steps; i += THREADS) mass[i] = 0;
+                team_sync<W>();
                 uint64_t sum = 0;
-                int kept = 0;
-#pragma unroll
-                for (int i = 0; i < FOUR; ++i) {          // kept: the weight ahead of it is short of the target
-                    const int place = tid * FOUR + i;
-                    const bool in = (place < m) & ((place == 0) | (run < target)) & (v[i] >= floor);
-                    run += w[i];
-                    sum += in ? w[i] : 0;
-                    kept += in;
-                    mass[place] = w[i];
-                }
-                sum = wave_sum(sum);
-                kept = wave_sum(kept);
-                if (tid == 0) {
-                    kept_sum = sum;
-                    n_kept = few || level || listed >= target ? kept : 0;        // 0: the list is too short for top_p
-                }
-            }
-            team_sync<W>();
-            const int kept = n_kept;
-            const uint64_t goal = sample_goal(u, kept_sum);
-            auto answer = [&](uint64_t e) {
-                index[r] = (int32_t)~(uint32_t)e;
-                logprob[r] = (float)(((double)row_value((uint32_t)(e >> 32)) - best) / t - row_log((double)kept_sum * a.unit));
-            };
-            if (kept > 64) {                              // in the order of their classes, the weights added up
-                if (tid < 64) {
+                for (int i = tid; i < n; i += THREADS) sum += list_mass[i];
+                sum = team_sum<W>(sum, part);
+                last = row_max(floor, least);
+                const uint64_t target = open ? ~0ull : sample_target(top_p, all);
+                if (target <= sum) cut_at(list_head<W>(list.entry, list_mass, n, target, sorted));
+                tally(n);
+            } else {
+                team_order<true>(list, n, sorted, LSR_MAX_TOP);
+                team_sync<W>();
+                const int most = few ? top_k : LSR_MAX_TOP, m = n < most ? n : most;     // the list is the head of the row, all of it
+                if (tid < 64) {                               // lane l has the places 4 l ... 4 l + 3
                     constexpr int FOUR = LSR_MAX_TOP / 64;
-                    static_assert(LSR_MAX_TOP <= 256 && LSR_MAX_CLASSES <= 1 << 24, "class and place in 32 bits");
-                    uint32_t c[FOUR];
+                    uint64_t w[FOUR], own = 0;
+                    float v[FOUR];
 #pragma unroll
                     for (int i = 0; i < FOUR; ++i) {
-                        const int place = i * 64 + tid;
-                        c[i] = place < kept ? (uint32_t)sorted[place] << 8 | place : 0;  // classes are complemented
-                    }
-                    wave_sort(c);
-                    uint64_t own = 0, w[FOUR];
-#pragma unroll
-                    for (int i = 0; i < FOUR; ++i) {
-                        w[i] = tid * FOUR + i < kept ? mass[c[i] & 255] : 0;
+                        const int place = tid * FOUR + i;
+                        v[i] = place < m ? row_value((uint32_t)(sorted[place] >> 32)) : -INFINITY;
+                        w[i] = row_fixed(row_exp2(((double)v[i] - best) * unit), a.magic);
                         own += w[i];
                     }
-                    uint64_t run = wave_running(own) - own;
+                    uint64_t run = wave_running(own);
+                    const uint64_t listed = wave_last(run), target = open ? ~0ull : sample_target(top_p, few ? listed : all);
+                    run -= own;
+                    uint64_t sum = 0;
+                    int kept = 0;
 #pragma unroll
-                    for (int i = 0; i < FOUR; ++i) {
-                        if (tid * FOUR + i < kept && (goal == 0 ? tid + i == 0 : run <= goal && goal < run + w[i])) answer(sorted[c[i] & 255]);
+                    for (int i = 0; i < FOUR; ++i) {          // kept: the weight ahead of it is short of the target
+                        const int place = tid * FOUR + i;
+                        const bool in = (place < m) & ((place == 0) | (run < target)) & (v[i] >= floor);
                         run += w[i];
+                        sum += in ? w[i] : 0;
+                        kept += in;
+                        mass[place] = w[i];
+                    }
+                    sum = wave_sum(sum);
+                    kept = wave_sum(kept);
+                    if (tid == 0) {
+                        kept_sum = sum;
+                        n_kept = few || level || listed >= target ? kept : 0;        // 0: the list is too short for top_p
                     }
                 }
-                return;
-            }
-#pragma unroll 1
-            for (int i = tid; i < kept; i += THREADS) {
-                // weight of the kept entries of lower classes
-                const uint32_t own = (uint32_t)sorted[i];
-                uint64_t before = 0;
-                int ahead = 0;
-#pragma unroll 8
-                for (int j = 0; j < kept; ++j) {
-                    const bool lower = (uint32_t)sorted[j] > own;
-                    before += lower ? mass[j] : 0;
-                    ahead += lower;
+                team_sync<W>();
+                const int kept = n_kept;
+                const uint64_t goal = sample_goal(u, kept_sum);
+                auto answer = [&](uint64_t e) {
+                    index[r] = (int32_t)~(uint32_t)e;
+                    logprob[r] = (float)(((double)row_value((uint32_t)(e >> 32)) - best) / t - row_log((double)kept_sum * a.unit));
+                };
+                if (kept > 64) {                              // in the order of their classes, the weights added up
+                    if (tid < 64) {
+                        constexpr int FOUR = LSR_MAX_TOP / 64;
+                        static_assert(LSR_MAX_TOP <= 256 && LSR_MAX_CLASSES <= 1 << 24, "class and place in 32 bits");
+                        uint32_t c[FOUR];
+#pragma unroll
+                        for (int i = 0; i < FOUR; ++i) {
+                            const int place = i * 64 + tid;
+                            c[i] = place < kept ? (uint32_t)sorted[place] << 8 | place : 0;  // classes are complemented
+                        }
+                        wave_sort(c);
+                        uint64_t own = 0, w[FOUR];
+#pragma unroll
+                        for (int i = 0; i < FOUR; ++i) {
+                            w[i] = tid * FOUR + i < kept ? mass[c[i] & 255] : 0;
+                            own += w[i];
+                        }
+                        uint64_t run = wave_running(own) - own;
+#pragma unroll
+                        for (int i = 0; i < FOUR; ++i) {
+                            if (tid * FOUR + i < kept && (goal == 0 ? tid + i == 0 : run <= goal && goal < run + w[i])) answer(sorted[c[i] & 255]);
+                            run += w[i];
+                        }
+                    }
+                    return;
                 }
-                if (goal == 0 ? ahead == 0 : before <= goal && goal < before + mass[i]) answer(sorted[i]);
+#pragma unroll 1
+                for (int i = tid; i < kept; i += THREADS) {
+                    // weight of the kept entries of lower classes
+                    const uint32_t own = (uint32_t)sorted[i];
+                    uint64_t before = 0;
+                    int ahead = 0;
+#pragma unroll 8
+                    for (int j = 0; j < kept; ++j) {
+                        const bool lower = (uint32_t)sorted[j] > own;
+                        before += lower ? mass[j] : 0;
+                        ahead += lower;
+                    }
+                    if (goal == 0 ? ahead == 0 : before <= goal && goal < before + mass[i]) answer(sorted[i]);
+                }
+                if (kept > 0) return;
             }
-            if (kept > 0) return;
         }
         if (few) return slowly();                         // thousands of entries are alike
     }
-
-    float last = least;                                   // kept: above this score, or equal up to this class
-    int last_class = n_classes;
-    auto keeps = [&](float v, int c) { return (v > last) | ((v == last) & (c <= last_class)); };
-    auto weigh = [&](float v) { return row_fixed(row_exp2(((double)v - best) * unit), a.magic); };
-    const float per_bin = (float)fmin(BINS / 24.0 / t, 1e30);
-    auto bin_of = [&](float v) { return (int)fminf((best - v) * per_bin, (float)(BINS - 1)); };
-
-    auto cut_at = [&](uint64_t e) {
-        last = row_value((uint32_t)(e >> 32));
-        last_class = (int)~(uint32_t)e;
-    };
-    const uint64_t zero = (uint64_t)__double_as_longlong(a.magic);
-    bool summed = false;                                  // the weights of the steps are known already
 
     if (cut) {                                            // the first top_k entries, by a histogram of their numbers
         team_sync<W>();
@@ -452,7 +475,7 @@ __global__ __launch_bounds__(64 * W) void lsr_sample_team_kernel(const typename 
             cut_at(list_head<W>(list.entry, list_mass, n, (uint64_t)(top_k - ahead), sorted));
         }
     }
-    if (top_p < 1) {
+    if (top_p < 1 && !summed) {
         // The entries that hold top_p of what is left.  A histogram of weights in 32 bits (whole numbers: adding floats in
         // shared memory takes eight times as long) says near which bin that cut lies.  One pass in 64 bits then sums
         // everything and, step by step, what is above the neighbours of that bin, and collects what is in the three of
@@ -536,13 +559,7 @@ __global__ __launch_bounds__(64 * W) void lsr_sample_team_kernel(const typename 
         const uint64_t target = sample_target(top_p, all);
         if (ahead >= target || target > ahead + listed) return slowly();
         cut_at(list_head<W>(list.entry, list_mass, n, target - ahead, sorted));
-        summed = floor <= last;
-        for (int i = tid; summed && i < n; i += THREADS) {
-            const uint64_t e = list.entry[i];
-            const int c = (int)~(uint32_t)e;
-            if (keeps(row_value((uint32_t)(e >> 32)), c))
-                atomicAdd((unsigned long long*)&mass[c / Row::STEP], (unsigned long long)list_mass[i]);
-        }
+        if (floor <= last) tally(n);
     }
     if (floor > last) {
         last = floor;

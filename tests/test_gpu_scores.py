@@ -645,3 +645,18 @@ def test_a_student_of_the_word_models(digits):
     for r in range(0, fb.total_frames, 11):
         assert drawn[r].item() == R.sample(x[r], float(u[r].item()), t, 0, 0.9, 0.0)[0]
     assert torch.equal(sample_scores(state_scores, u, t, 0, 0.9)[0], drawn)
+
+
+@pytest.mark.parametrize("classes,dtype", [(1000, "f32"), (9001, "f16"), (131072, "bf16"), (50001, "f32")])
+def test_sample_scores_of_hundreds_of_entries(classes, dtype):
+    """min_p that hundreds or thousands of entries reach, with and without a cut by top_p among them."""
+    rng = np.random.default_rng(classes + 5)
+    view, x = _device(rng.normal(size=(24, classes)) * 2.0, dtype)
+    best = x.max(axis=1)
+    order = np.sort(x, axis=1)[:, ::-1]
+    reach = np.array([260, 300, 400, 480, 511, 513, 900, 2000, 2049, 4000, 4100, 5000] * 2) % classes
+    min_p = np.exp(order[np.arange(24), reach] - best)
+    top_p = np.where(np.arange(24) < 12, 1.0, rng.uniform(0.02, 0.9, 24))
+    u = rng.random(24)
+    u[3], u[20] = 0.0, 1.0 - 2.0 ** -24
+    _check_sample(view, x, u, np.ones(24), np.zeros(24, int), top_p, min_p, as_tensor=True)
