@@ -420,6 +420,8 @@ extern "C" int lsr_distill_scores(lsr_ctx* ctx, const void* scores_d, int dtype,
     if (k > LSR_MAX_TOP) return lsr_fail(ctx, LSR_ERR_LIMIT, "lsr_distill_scores: k = %d > %d", k, LSR_MAX_TOP);
     if (!(temperature > 0) || !isfinite(temperature))
         return lsr_fail(ctx, LSR_ERR_ARG, "lsr_distill_scores: temperature must be positive and finite");
+    if (temperature < 1e-30 || temperature > 1e30)        // its reciprocal is used in 32 bits
+        return lsr_fail(ctx, LSR_ERR_LIMIT, "lsr_distill_scores: temperature %g outside 1e-30..1e30", temperature);
     if (n_rows == 0) return LSR_OK;
     if (!top_values_d || !top_index_d || !loss_d) return lsr_fail(ctx, LSR_ERR_ARG, "lsr_distill_scores: null pointer");
     if ((uintptr_t)grad_d % row_dtype_bytes(dtype))

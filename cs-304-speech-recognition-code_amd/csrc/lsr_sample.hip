@@ -525,17 +525,25 @@ __global__ __launch_bounds__(64 * W) void lsr_sample_team_kernel(const typename 
         auto weigh_all = [&](auto some) {
             row.template each<2>([&](int step, const float(&v)[RUN], int c) {
                 uint64_t higher = 0;
+                bool any = false;
 #pragma unroll
                 for (int j = 0; j < RUN; ++j) {
                     const float s = !some.value || keeps(v[j], c + j) ? v[j] : -INFINITY;
                     const uint64_t m = (uint64_t)__double_as_longlong(row_exp2(((double)s - best) * unit) + a.magic);
                     all += m;
                     higher += s > high ? m : zero;
-                    if ((s <= high) & (s >= low) & (s > -INFINITY)) {
-                        const int at = atomicAdd(&list.n, 1);
-                        if (at < ROOM) {
-                            list.entry[at] = row_entry(row_key(s), c + j);
-                            list_mass[at] = m - zero;
+                    any |= (s >= low) & !(s > high);
+                }
+                if (any) {
+#pragma unroll
+                    for (int j = 0; j < RUN; ++j) {
+                        const float s = !some.value || keeps(v[j], c + j) ? v[j] : -INFINITY;
+                        if ((s >= low) & !(s > high) & (s > -INFINITY)) {
+                            const int at = atomicAdd(&list.n, 1);
+                            if (at < ROOM) {
+                                list.entry[at] = row_entry(row_key(s), c + j);
+                                list_mass[at] = weigh(s);
+                            }
                         }
                     }
                 }
@@ -822,6 +830,8 @@ extern "C" int lsr_sample_scores(lsr_ctx* ctx, const void* scores_d, int dtype, 
     if (rc) return rc;
     if (isnan(temperature) || isnan(top_p) || isnan(min_p))
         return lsr_fail(ctx, LSR_ERR_ARG, "lsr_sample_scores: a setting is not a number");
+    if (temperature > 0 && (temperature < 1e-45 || temperature > 1e38))           // what float32 settings per row can be
+        return lsr_fail(ctx, LSR_ERR_LIMIT, "lsr_sample_scores: temperature %g outside 1e-45..1e38", temperature);
     if (n_rows == 0) return LSR_OK;
     if (!uniform_d || !index_d || !logprob_d) return lsr_fail(ctx, LSR_ERR_ARG, "lsr_sample_scores: null pointer");
     LSR_HIP_CHECK(ctx, hipSetDevice(ctx->device));

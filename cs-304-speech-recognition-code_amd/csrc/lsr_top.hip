@@ -288,6 +288,8 @@ extern "C" int lsr_top_scores(lsr_ctx* ctx, const void* scores_d, int dtype, int
     if (k < 1 || k > n_classes) return lsr_fail(ctx, LSR_ERR_ARG, "lsr_top_scores: k = %d outside 1..%lld", k, (long long)n_classes);
     if (k > LSR_MAX_TOP) return lsr_fail(ctx, LSR_ERR_LIMIT, "lsr_top_scores: k = %d > %d", k, LSR_MAX_TOP);
     if (!(temperature > 0) || !isfinite(temperature)) return lsr_fail(ctx, LSR_ERR_ARG, "lsr_top_scores: temperature must be positive and finite");
+    if (temperature < 1e-30 || temperature > 1e30)        // its reciprocal is used in 32 bits
+        return lsr_fail(ctx, LSR_ERR_LIMIT, "lsr_top_scores: temperature %g outside 1e-30..1e30", temperature);
     if (n_rows == 0) return LSR_OK;
     if (!values_d || !index_d) return lsr_fail(ctx, LSR_ERR_ARG, "lsr_top_scores: null pointer");
     LSR_HIP_CHECK(ctx, hipSetDevice(ctx->device));

@@ -67,8 +67,8 @@ def _check_like(name: str, t, shape: Tuple[int, ...], dtype: str, device) -> Non
 
 def _check_temperature(temperature) -> float:
     temperature = float(temperature)
-    if not 0.0 < temperature < float("inf"):
-        raise ValueError("temperature must be positive and finite")
+    if not 1e-30 <= temperature <= 1e30:
+        raise ValueError(f"temperature must be in 1e-30..1e30, got {temperature}")
     return temperature
 
 
@@ -128,8 +128,8 @@ def sample_scores(scores, uniform, temperature: Union[float, "torch.Tensor"] = 1
             if isinstance(v, bool) or int(v) != v or v < 0:
                 raise ValueError(f"top_k must be an integer >= 0, got {v}")
             v = min(int(v), classes)
-        elif not 0.0 <= float(v) < float("inf") or (name != "temperature" and float(v) > 1.0):
-            raise ValueError(f"{name} must be {'>= 0 and finite' if name == 'temperature' else 'in [0, 1]'}, got {v}")
+        elif not 0.0 <= float(v) <= (1e38 if name == "temperature" else 1.0) or (name == "temperature" and 0 < float(v) < 1e-45):
+            raise ValueError(f"{name} must be {'0 or in 1e-45..1e38' if name == 'temperature' else 'in [0, 1]'}, got {v}")
         numbers.append(v if name == "top_k" else float(v))
         tensors.append(None)
     eng = _engine(scores)

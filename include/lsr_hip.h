@@ -384,7 +384,7 @@ int lsr_unpack_label_records(lsr_ctx* ctx, const uint8_t* records_d, int world, 
 /* The first k (1..min(n_classes, LSR_MAX_TOP)) entries of every row: values_d float32[n_rows][k], index_d
  * int32[n_rows][k]; a row with fewer entries is filled with -infinity / -1.  rest_d float32[n_rows] (may be NULL): log of
  * the sum of e^((x - x_best) / temperature) over the other entries of the row, -infinity if there are none - the log
- * weight of "any other class" relative to the row's best. */
+ * weight of "any other class" relative to the row's best.  temperature: 1e-30..1e30. */
 int lsr_top_scores(lsr_ctx* ctx, const void* scores_d, int dtype, int64_t n_rows, int64_t n_classes, int64_t row_stride,
                    int k, double temperature, float* values_d, int32_t* index_d, float* rest_d);
 
@@ -393,8 +393,8 @@ int lsr_top_scores(lsr_ctx* ctx, const void* scores_d, int dtype, int64_t n_rows
  * those the shortest head that holds top_p of their weight (>= 1: all, <= 0: the first); the entries with
  * x >= x_best + temperature ln(min_p) (<= 0: all, values above 1 count as 1).  index_d[n_rows] is the first class, in
  * ascending class order, at which the running weight of the kept classes exceeds uniform * their total, logprob_d[n_rows]
- * the log of its share of the total.  temperature <= 0 (or NaN in temperature_d): the row's first entry, log share 0.  A
- * row without entries: -1, -infinity.  If the row holds +infinity only those entries have weight.  Each setting is one
+ * the log of its share of the total.  temperature (1e-45..1e38) <= 0, or NaN in temperature_d: the row's first entry, log
+ * share 0.  A row without entries: -1, -infinity.  If the row holds +infinity only those entries have weight.  Each setting is one
  * number for all rows or, where its pointer is not NULL, float32 / int32[n_rows].  Weights are computed in 64 bits and
  * summed as whole multiples of 2^-52 (up to 1 024 classes) ... 2^-38 (2^24 classes) of the best one's.  A class whose
  * weight is 0 in 64 bits (more than about 745 temperatures below the best, such as one masked with the type's lowest

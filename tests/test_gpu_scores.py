@@ -203,6 +203,21 @@ def test_top_scores_of_many_equal_ones(classes, dtype):
         _check_top(view, x, k, 1.0)
 
 
+@pytest.mark.parametrize("classes,dtype", [(58, "f32"), (1000, "f16"), (20011, "f32"), (70001, "bf16")])
+def test_extreme_temperatures(classes, dtype):
+    rng = np.random.default_rng(classes + 9)
+    n = 12
+    x = rng.normal(size=(n, classes))
+    x[:, 3] = -np.inf
+    x[1::2, 5] = x[1::2].max(axis=1)                      # two best ones
+    view, x = _device(x, dtype)
+    t = np.array([1e-45, 1e-45, 1e-38, 1e-38, 1e-30, 1e-20, 1e20, 1e30, 1e38, 3e38, 1e-3, 1e3])
+    for top_k, top_p, min_p in [(0, 1.0, 0.0), (7, 1.0, 0.0), (400, 0.9, 0.0), (0, 0.8, 0.0), (0, 0.8, 0.5)]:
+        _check_sample(view, x, rng.random(n), t, np.full(n, top_k), np.full(n, top_p), np.full(n, min_p), as_tensor=True)
+    for one in (1e-30, 1e30):
+        _check_top(view, x, 6, one)
+
+
 def test_sample_scores_distribution():
     """The share of each class over evenly spread uniform numbers is its probability to within one number per border."""
     from loe_speech_recognition_amd import sample_scores
@@ -455,7 +470,8 @@ def test_c_entry_points_refuse():
     top = lambda s=p(x), d=0, n=4, v=9, st=9, k=2, t=1.0, o=p(out): code(eng.lib.lsr_top_scores, s, d, n, v, st, k, t, o, o, None)
     for kw, want in (({"d": 3}, -1), ({"n": -1}, -1), ({"v": 0}, -1), ({"st": -1}, -1), ({"k": 0}, -1), ({"k": 10}, -1),
                      ({"t": 0.0}, -1), ({"t": float("nan")}, -1), ({"s": None}, -1), ({"o": None}, -1),
-                     ({"s": ctypes.c_void_p(x.data_ptr() + 2)}, -1), ({"v": (1 << 24) + 1}, -3), ({"v": 1000, "k": 257}, -3)):
+                     ({"s": ctypes.c_void_p(x.data_ptr() + 2)}, -1), ({"v": (1 << 24) + 1}, -3), ({"v": 1000, "k": 257}, -3),
+                     ({"t": 1e-31}, -3), ({"t": 1e31}, -3)):
         rc, text = top(**kw)
         assert rc == want and "lsr_top_scores" in text, (kw, rc, text)
     for args in ((None, 1.0, 0, 1.0, 0.0), (p(out), float("nan"), 0, 1.0, 0.0), (p(out), 1.0, 0, float("nan"), 0.0)):

@@ -24,6 +24,10 @@ def _rows(n=4, v=9, dtype=torch.float32):
     (lambda: top_scores(_rows(2, 1000), _native.MAX_TOP + 1), ValueError),
     (lambda: top_scores(_rows(), 2, temperature=0.0), ValueError),
     (lambda: top_scores(_rows(), 2, temperature=float("inf")), ValueError),
+    (lambda: top_scores(_rows(), 2, temperature=1e-39), ValueError),
+    (lambda: top_scores(_rows(), 2, temperature=1e39), ValueError),
+    (lambda: sample_scores(_rows(), torch.zeros(4), temperature=1e-310), ValueError),
+    (lambda: distill_scores(_rows(), *_teacher(), temperature=1e-39), ValueError),
     (lambda: top_scores(_rows(), 2), ValueError),                                     # not on the GPU
 ])
 def test_top_scores_refuses(call, error):
