@@ -249,414 +249,415 @@ __global__ __launch_bounds__(64 * W) void lsr_sample_team_kernel(const typename 
         }
         return;
     }
-    auto slowly = [&]() {
-        sample_by_radix<DT, W>(mine, n_classes, best, t, top_k, top_p, min_p, u, a, mass, &above, index + r, logprob + r);
-    };
-    if (best == INFINITY) return slowly();
+    // false: not for here
+    auto fast = [&]() -> bool {
+        float last = least;                                   // kept: above this score, or equal up to this class
+        int last_class = n_classes;
+        auto keeps = [&](float v, int c) { return (v > last) | ((v == last) & (c <= last_class)); };
+        auto weigh = [&](float v) { return row_fixed(row_exp2(((double)v - best) * unit), a.magic); };
+        const float per_bin = (float)fmin(BINS / 24.0 / t, 1e30);
+        auto bin_of = [&](float v) { return (int)fminf((best - v) * per_bin, (float)(BINS - 1)); };
 
-    float last = least;                                   // kept: above this score, or equal up to this class
-    int last_class = n_classes;
-    auto keeps = [&](float v, int c) { return (v > last) | ((v == last) & (c <= last_class)); };
-    auto weigh = [&](float v) { return row_fixed(row_exp2(((double)v - best) * unit), a.magic); };
-    const float per_bin = (float)fmin(BINS / 24.0 / t, 1e30);
-    auto bin_of = [&](float v) { return (int)fminf((best - v) * per_bin, (float)(BINS - 1)); };
+        auto cut_at = [&](uint64_t e) {
+            last = row_value((uint32_t)(e >> 32));
+            last_class = (int)~(uint32_t)e;
+        };
+        const uint64_t zero = (uint64_t)__double_as_longlong(a.magic);
+        bool summed = false;                                  // the weights of the steps are known already
+        // adds the weights of the list's entries that are kept to those of their steps
+        auto tally = [&](int n) {
+            for (int i = tid; i < n; i += THREADS) {
+                const uint64_t e = list.entry[i];
+                const int c = (int)~(uint32_t)e;
+                if (keeps(row_value((uint32_t)(e >> 32)), c))
+                    atomicAdd((unsigned long long*)&mass[c / Row::STEP], (unsigned long long)list_mass[i]);
+            }
+            summed = true;
+        };
 
-    auto cut_at = [&](uint64_t e) {
-        last = row_value((uint32_t)(e >> 32));
-        last_class = (int)~(uint32_t)e;
-    };
-    const uint64_t zero = (uint64_t)__double_as_longlong(a.magic);
-    bool summed = false;                                  // the weights of the steps are known already
-    // adds the weights of the list's entries that are kept to those of their steps
-    auto tally = [&](int n) {
-        for (int i = tid; i < n; i += THREADS) {
-            const uint64_t e = list.entry[i];
-            const int c = (int)~(uint32_t)e;
-            if (keeps(row_value((uint32_t)(e >> 32)), c))
-                atomicAdd((unsigned long long*)&mass[c / Row::STEP], (unsigned long long)list_mass[i]);
+        // Rows that are answered from a list of their first entries.  few: a small top_k.  level: min_p without top_k, when not
+        // many entries reach it.  nucleus: top_p alone, where it looks as if a short head will do: where the best scores of the
+        // groups hold that share of the row's weight.
+        const bool cut = top_k > 0 && top_k < n_classes, few = cut && top_k <= LSR_MAX_TOP, level = !cut && min_p > 0;
+        const float floor = min_p > 0 ? sample_floor(best, t, min_p) : -INFINITY, unit_f = (float)unit;
+        bool nucleus = !cut && !level && top_p < 1;
+        float guess = 0;                                      // the row's weight in 32 bits, good to 2^-12 and better
+        if (!few && top_p < 1) {
+            float head = 0;
+            row.template each<4>([&](int, const float(&v)[RUN], int) {
+#pragma unroll
+                for (int j = 0; j < RUN; ++j) guess += __builtin_amdgcn_exp2f((v[j] - best) * unit_f);
+            });
+            guess = team_sum<W>(guess, part_f);
+            for (int i = tid; i < ROW_GROUPS; i += THREADS)
+                if (list.group[i]) head += __builtin_amdgcn_exp2f((row_value(list.group[i]) - best) * unit_f);
+            nucleus = nucleus && team_sum<W>(head, part_f) >= (float)top_p * guess;
         }
-        summed = true;
-    };
-
-    // Rows that are answered from a list of their first entries.  few: a small top_k.  level: min_p without top_k, when not
-    // many entries reach it.  nucleus: top_p alone, where it looks as if a short head will do: where the best scores of the
-    // groups hold that share of the row's weight.
-    const bool cut = top_k > 0 && top_k < n_classes, few = cut && top_k <= LSR_MAX_TOP, level = !cut && min_p > 0;
-    const float floor = min_p > 0 ? sample_floor(best, t, min_p) : -INFINITY, unit_f = (float)unit;
-    bool nucleus = !cut && !level && top_p < 1;
-    float guess = 0;                                      // the row's weight in 32 bits, good to 2^-12 and better
-    if (!few && top_p < 1) {
-        float head = 0;
-        row.template each<4>([&](int, const float(&v)[RUN], int) {
-#pragma unroll
-            for (int j = 0; j < RUN; ++j) guess += __builtin_amdgcn_exp2f((v[j] - best) * unit_f);
-        });
-        guess = team_sum<W>(guess, part_f);
-        for (int i = tid; i < ROW_GROUPS; i += THREADS)
-            if (list.group[i]) head += __builtin_amdgcn_exp2f((row_value(list.group[i]) - best) * unit_f);
-        nucleus = nucleus && team_sum<W>(head, part_f) >= (float)top_p * guess;
-    }
-    if (few || level || nucleus) {
-        float none = 0, bound = few || nucleus ? team_bound(few ? top_k : NUCLEUS < n_classes ? NUCLEUS : n_classes, list) : floor;
-        if (level && tid == 0) list.n = 0;
-        if (level) team_sync<W>();
-        team_take<false, false>(row, row_max(bound, least), list, 0.0f, none, mine);
-        const int n = list.n;
-        if (n <= ROOM) {
-            // weight of the row, where the list does not hold what top_p is a share of; where the level's entries weigh
-            // less than that share by more than the guess can be off, top_p takes nothing away
-            uint64_t all = 0;
-            bool open = top_p >= 1;
-            if (level && !open) {
-                float listed = 0;
-                for (int i = tid; i < n; i += THREADS)
-                    listed += __builtin_amdgcn_exp2f((row_value((uint32_t)(list.entry[i] >> 32)) - best) * unit_f);
-                open = team_sum<W>(listed, part_f) < (1 - 1.0f / 512) * (float)top_p * guess;
-            }
-            if (!few && !open) {
-                row.template each<2>([&](int, const float(&v)[RUN], int) {
-#pragma unroll
-                    for (int j = 0; j < RUN; ++j)
-                        all += (uint64_t)__double_as_longlong(row_exp2(((double)v[j] - best) * unit) + a.magic);
-                    all -= RUN * (uint64_t)__double_as_longlong(a.magic);
-                });
-                all = team_sum<W>(all, part);
-            }
-            if (level && n > LSR_MAX_TOP) {               // too many to put in order
-                for (int i = tid; i < n; i += THREADS) list_mass[i] = weigh(row_value((uint32_t)(list.entry[i] >> 32)));
-                for (int i = tid; i < row.steps; i += THREADS) mass[i] = 0;
-                team_sync<W>();
-                uint64_t sum = 0;
-                for (int i = tid; i < n; i += THREADS) sum += list_mass[i];
-                sum = team_sum<W>(sum, part);
-                last = row_max(floor, least);
-                const uint64_t target = open ? ~0ull : sample_target(top_p, all);
-                if (target <= sum) cut_at(list_head<W>(list.entry, list_mass, n, target, sorted));
-                tally(n);
-            } else {
-                team_order<true>(list, n, sorted, LSR_MAX_TOP);
-                team_sync<W>();
-                const int most = few ? top_k : LSR_MAX_TOP, m = n < most ? n : most;     // the list is the head of the row, all of it
-                if (tid < 64) {                               // lane l has the places 4 l ... 4 l + 3
-                    constexpr int FOUR = LSR_MAX_TOP / 64;
-                    uint64_t w[FOUR], own = 0;
-                    float v[FOUR];
-#pragma unroll
-                    for (int i = 0; i < FOUR; ++i) {
-                        const int place = tid * FOUR + i;
-                        v[i] = place < m ? row_value((uint32_t)(sorted[place] >> 32)) : -INFINITY;
-                        w[i] = row_fixed(row_exp2(((double)v[i] - best) * unit), a.magic);
-                        own += w[i];
-                    }
-                    uint64_t run = wave_running(own);
-                    const uint64_t listed = wave_last(run), target = open ? ~0ull : sample_target(top_p, few ? listed : all);
-                    run -= own;
-                    uint64_t sum = 0;
-                    int kept = 0;
-#pragma unroll
-                    for (int i = 0; i < FOUR; ++i) {          // kept: the weight ahead of it is short of the target
-                        const int place = tid * FOUR + i;
-                        const bool in = (place < m) & ((place == 0) | (run < target)) & (v[i] >= floor);
-                        run += w[i];
-                        sum += in ? w[i] : 0;
-                        kept += in;
-                        mass[place] = w[i];
-                    }
-                    sum = wave_sum(sum);
-                    kept = wave_sum(kept);
-                    if (tid == 0) {
-                        kept_sum = sum;
-                        n_kept = few || level || listed >= target ? kept : 0;        // 0: the list is too short for top_p
-                    }
+        if (few || level || nucleus) {
+            float none = 0, bound = few || nucleus ? team_bound(few ? top_k : NUCLEUS < n_classes ? NUCLEUS : n_classes, list) : floor;
+            if (level && tid == 0) list.n = 0;
+            if (level) team_sync<W>();
+            team_take<false, false>(row, row_max(bound, least), list, 0.0f, none, mine);
+            const int n = list.n;
+            if (n <= ROOM) {
+                // weight of the row, where the list does not hold what top_p is a share of; where the level's entries weigh
+                // less than that share by more than the guess can be off, top_p takes nothing away
+                uint64_t all = 0;
+                bool open = top_p >= 1;
+                if (level && !open) {
+                    float listed = 0;
+                    for (int i = tid; i < n; i += THREADS)
+                        listed += __builtin_amdgcn_exp2f((row_value((uint32_t)(list.entry[i] >> 32)) - best) * unit_f);
+                    open = team_sum<W>(listed, part_f) < (1 - 1.0f / 512) * (float)top_p * guess;
                 }
-                team_sync<W>();
-                const int kept = n_kept;
-                const uint64_t goal = sample_goal(u, kept_sum);
-                auto answer = [&](uint64_t e) {
-                    index[r] = (int32_t)~(uint32_t)e;
-                    logprob[r] = (float)(((double)row_value((uint32_t)(e >> 32)) - best) / t - row_log((double)kept_sum * a.unit));
-                };
-                if (kept > 64) {                              // in the order of their classes, the weights added up
-                    if (tid < 64) {
+                if (!few && !open) {
+                    row.template each<2>([&](int, const float(&v)[RUN], int) {
+#pragma unroll
+                        for (int j = 0; j < RUN; ++j)
+                            all += (uint64_t)__double_as_longlong(row_exp2(((double)v[j] - best) * unit) + a.magic);
+                        all -= RUN * (uint64_t)__double_as_longlong(a.magic);
+                    });
+                    all = team_sum<W>(all, part);
+                }
+                if (level && n > LSR_MAX_TOP) {               // too many to put in order
+                    for (int i = tid; i < n; i += THREADS) list_mass[i] = weigh(row_value((uint32_t)(list.entry[i] >> 32)));
+                    for (int i = tid; i < row.steps; i += THREADS) mass[i] = 0;
+                    team_sync<W>();
+                    uint64_t sum = 0;
+                    for (int i = tid; i < n; i += THREADS) sum += list_mass[i];
+                    sum = team_sum<W>(sum, part);
+                    last = row_max(floor, least);
+                    const uint64_t target = open ? ~0ull : sample_target(top_p, all);
+                    if (target <= sum) cut_at(list_head<W>(list.entry, list_mass, n, target, sorted));
+                    tally(n);
+                } else {
+                    team_order<true>(list, n, sorted, LSR_MAX_TOP);
+                    team_sync<W>();
+                    const int most = few ? top_k : LSR_MAX_TOP, m = n < most ? n : most;     // the list is the head of the row, all of it
+                    if (tid < 64) {                               // lane l has the places 4 l ... 4 l + 3
                         constexpr int FOUR = LSR_MAX_TOP / 64;
-                        static_assert(LSR_MAX_TOP <= 256 && LSR_MAX_CLASSES <= 1 << 24, "class and place in 32 bits");
-                        uint32_t c[FOUR];
+                        uint64_t w[FOUR], own = 0;
+                        float v[FOUR];
 #pragma unroll
                         for (int i = 0; i < FOUR; ++i) {
-                            const int place = i * 64 + tid;
-                            c[i] = place < kept ? (uint32_t)sorted[place] << 8 | place : 0;  // classes are complemented
-                        }
-                        wave_sort(c);
-                        uint64_t own = 0, w[FOUR];
-#pragma unroll
-                        for (int i = 0; i < FOUR; ++i) {
-                            w[i] = tid * FOUR + i < kept ? mass[c[i] & 255] : 0;
+                            const int place = tid * FOUR + i;
+                            v[i] = place < m ? row_value((uint32_t)(sorted[place] >> 32)) : -INFINITY;
+                            w[i] = row_fixed(row_exp2(((double)v[i] - best) * unit), a.magic);
                             own += w[i];
                         }
-                        uint64_t run = wave_running(own) - own;
+                        uint64_t run = wave_running(own);
+                        const uint64_t listed = wave_last(run), target = open ? ~0ull : sample_target(top_p, few ? listed : all);
+                        run -= own;
+                        uint64_t sum = 0;
+                        int kept = 0;
 #pragma unroll
-                        for (int i = 0; i < FOUR; ++i) {
-                            if (tid * FOUR + i < kept && (goal == 0 ? tid + i == 0 : run <= goal && goal < run + w[i])) answer(sorted[c[i] & 255]);
+                        for (int i = 0; i < FOUR; ++i) {          // kept: the weight ahead of it is short of the target
+                            const int place = tid * FOUR + i;
+                            const bool in = (place < m) & ((place == 0) | (run < target)) & (v[i] >= floor);
                             run += w[i];
+                            sum += in ? w[i] : 0;
+                            kept += in;
+                            mass[place] = w[i];
+                        }
+                        sum = wave_sum(sum);
+                        kept = wave_sum(kept);
+                        if (tid == 0) {
+                            kept_sum = sum;
+                            n_kept = few || level || listed >= target ? kept : 0;        // 0: the list is too short for top_p
                         }
                     }
-                    return;
-                }
+                    team_sync<W>();
+                    const int kept = n_kept;
+                    const uint64_t goal = sample_goal(u, kept_sum);
+                    auto answer = [&](uint64_t e) {
+                        index[r] = (int32_t)~(uint32_t)e;
+                        logprob[r] = (float)(((double)row_value((uint32_t)(e >> 32)) - best) / t - row_log((double)kept_sum * a.unit));
+                    };
+                    if (kept > 64) {                              // in the order of their classes, the weights added up
+                        if (tid < 64) {
+                            constexpr int FOUR = LSR_MAX_TOP / 64;
+                            static_assert(LSR_MAX_TOP <= 256 && LSR_MAX_CLASSES <= 1 << 24, "class and place in 32 bits");
+                            uint32_t c[FOUR];
+#pragma unroll
+                            for (int i = 0; i < FOUR; ++i) {
+                                const int place = i * 64 + tid;
+                                c[i] = place < kept ? (uint32_t)sorted[place] << 8 | place : 0;  // classes are complemented
+                            }
+                            wave_sort(c);
+                            uint64_t own = 0, w[FOUR];
+#pragma unroll
+                            for (int i = 0; i < FOUR; ++i) {
+                                w[i] = tid * FOUR + i < kept ? mass[c[i] & 255] : 0;
+                                own += w[i];
+                            }
+                            uint64_t run = wave_running(own) - own;
+#pragma unroll
+                            for (int i = 0; i < FOUR; ++i) {
+                                if (tid * FOUR + i < kept && (goal == 0 ? tid + i == 0 : run <= goal && goal < run + w[i])) answer(sorted[c[i] & 255]);
+                                run += w[i];
+                            }
+                        }
+                        return true;
+                    }
 #pragma unroll 1
-                for (int i = tid; i < kept; i += THREADS) {
-                    // weight of the kept entries of lower classes
-                    const uint32_t own = (uint32_t)sorted[i];
-                    uint64_t before = 0;
-                    int ahead = 0;
+                    for (int i = tid; i < kept; i += THREADS) {
+                        // weight of the kept entries of lower classes
+                        const uint32_t own = (uint32_t)sorted[i];
+                        uint64_t before = 0;
+                        int ahead = 0;
 #pragma unroll 8
-                    for (int j = 0; j < kept; ++j) {
-                        const bool lower = (uint32_t)sorted[j] > own;
-                        before += lower ? mass[j] : 0;
-                        ahead += lower;
+                        for (int j = 0; j < kept; ++j) {
+                            const bool lower = (uint32_t)sorted[j] > own;
+                            before += lower ? mass[j] : 0;
+                            ahead += lower;
+                        }
+                        if (goal == 0 ? ahead == 0 : before <= goal && goal < before + mass[i]) answer(sorted[i]);
                     }
-                    if (goal == 0 ? ahead == 0 : before <= goal && goal < before + mass[i]) answer(sorted[i]);
+                    if (kept > 0) return true;
                 }
-                if (kept > 0) return;
             }
+            if (few) return false;                         // thousands of entries are alike
         }
-        if (few) return slowly();                         // thousands of entries are alike
-    }
 
-    if (cut) {                                            // the first top_k entries, by a histogram of their numbers
-        team_sync<W>();
-        for (int i = tid; i < BINS; i += THREADS) bin_n[i] = 0;
-        if (tid == 0) list.n = 0;
-        team_sync<W>();
-        row.template each<4>([&](int, const float(&v)[RUN], int) {
-#pragma unroll
-            for (int j = 0; j < RUN; ++j)
-                if (v[j] >= least) atomicAdd(&bin_n[bin_of(v[j])], 1);
-        });
-        team_sync<W>();
-        int own = 0, sum = 0;
-#pragma unroll
-        for (int i = 0; i < OWN; ++i) own += bin_n[tid * OWN + i];
-        int run = wave_running(own);
-        if ((tid & 63) == 63) part_n[tid >> 6] = run;
-        team_sync<W>();
-#pragma unroll
-        for (int i = 0; i < W; ++i) {
-            if (i < (tid >> 6)) run += part_n[i];
-            sum += part_n[i];
-        }
-        if (top_k <= sum) {                               // or all are kept
-            run -= own;
-            if (run < top_k && top_k <= run + own) {
-#pragma unroll
-                for (int i = 0; i < OWN; ++i) {
-                    const int m = bin_n[tid * OWN + i];
-                    if (run < top_k && top_k <= run + m) {
-                        cut_bin = tid * OWN + i;
-                        n_kept = run;
-                    }
-                    run += m;
-                }
-            }
+        if (cut) {                                            // the first top_k entries, by a histogram of their numbers
             team_sync<W>();
-            const int b = cut_bin, ahead = n_kept;
-            row.template each<4>([&](int, const float(&v)[RUN], int c) {
+            for (int i = tid; i < BINS; i += THREADS) bin_n[i] = 0;
+            if (tid == 0) list.n = 0;
+            team_sync<W>();
+            row.template each<4>([&](int, const float(&v)[RUN], int) {
 #pragma unroll
                 for (int j = 0; j < RUN; ++j)
-                    if (v[j] >= least && bin_of(v[j]) == b) {
-                        const int at = atomicAdd(&list.n, 1);
-                        if (at < ROOM) list.entry[at] = row_entry(row_key(v[j]), c + j);
-                    }
+                    if (v[j] >= least) atomicAdd(&bin_n[bin_of(v[j])], 1);
             });
             team_sync<W>();
-            const int n = list.n;
-            if (n > ROOM) return slowly();
-            for (int i = tid; i < n; i += THREADS) list_mass[i] = 1;
+            int own = 0, sum = 0;
+#pragma unroll
+            for (int i = 0; i < OWN; ++i) own += bin_n[tid * OWN + i];
+            int run = wave_running(own);
+            if ((tid & 63) == 63) part_n[tid >> 6] = run;
             team_sync<W>();
-            cut_at(list_head<W>(list.entry, list_mass, n, (uint64_t)(top_k - ahead), sorted));
-        }
-    }
-    if (top_p < 1 && !summed) {
-        // The entries that hold top_p of what is left.  A histogram of weights in 32 bits (whole numbers: adding floats in
-        // shared memory takes eight times as long) says near which bin that cut lies.  One pass in 64 bits then sums
-        // everything and, step by step, what is above the neighbours of that bin, and collects what is in the three of
-        // them: if the cut is there, everything is known that the draw needs.  It can be elsewhere where it lies as near to
-        // an edge as 32 bits are off and empty bins follow.
-        team_sync<W>();
-        for (int i = tid; i < BINS; i += THREADS) bin_n[i] = 0;
-        for (int i = tid; i < row.steps; i += THREADS) mass[i] = 0;
-        if (tid == 0) {
-            list.n = 0;
-            cut_bin = BINS - 1;
-        }
-        team_sync<W>();
-        const float scale = 1073741824.0f / guess;
-        row.template each<4>([&](int, const float(&v)[RUN], int c) {
 #pragma unroll
-            for (int j = 0; j < RUN; ++j) {
-                const float s = !cut || keeps(v[j], c + j) ? v[j] : -INFINITY;
-                const int m = (int)(__builtin_amdgcn_exp2f((s - best) * unit_f) * scale + 0.5f);
-                if (m) atomicAdd(&bin_n[bin_of(s)], m);
+            for (int i = 0; i < W; ++i) {
+                if (i < (tid >> 6)) run += part_n[i];
+                sum += part_n[i];
             }
-        });
-        team_sync<W>();
-        uint32_t own = 0, total = 0;
+            if (top_k <= sum) {                               // or all are kept
+                run -= own;
+                if (run < top_k && top_k <= run + own) {
 #pragma unroll
-        for (int i = 0; i < OWN; ++i) own += (uint32_t)bin_n[tid * OWN + i];
-        uint32_t run = (uint32_t)wave_running((int)own);
-        if ((tid & 63) == 63) part_n[tid >> 6] = (int)run;
-        team_sync<W>();
+                    for (int i = 0; i < OWN; ++i) {
+                        const int m = bin_n[tid * OWN + i];
+                        if (run < top_k && top_k <= run + m) {
+                            cut_bin = tid * OWN + i;
+                            n_kept = run;
+                        }
+                        run += m;
+                    }
+                }
+                team_sync<W>();
+                const int b = cut_bin, ahead = n_kept;
+                row.template each<4>([&](int, const float(&v)[RUN], int c) {
 #pragma unroll
-        for (int i = 0; i < W; ++i) {
-            if (i < (tid >> 6)) run += (uint32_t)part_n[i];
-            total += (uint32_t)part_n[i];
-        }
-        run -= own;
-        const uint32_t near = (uint32_t)(top_p * total);
-        if (run < near && near <= run + own) {
-#pragma unroll
-            for (int i = 0; i < OWN; ++i) {
-                if (run < near) cut_bin = tid * OWN + i;
-                run += (uint32_t)bin_n[tid * OWN + i];
+                    for (int j = 0; j < RUN; ++j)
+                        if (v[j] >= least && bin_of(v[j]) == b) {
+                            const int at = atomicAdd(&list.n, 1);
+                            if (at < ROOM) list.entry[at] = row_entry(row_key(v[j]), c + j);
+                        }
+                });
+                team_sync<W>();
+                const int n = list.n;
+                if (n > ROOM) return false;
+                for (int i = tid; i < n; i += THREADS) list_mass[i] = 1;
+                team_sync<W>();
+                cut_at(list_head<W>(list.entry, list_mass, n, (uint64_t)(top_k - ahead), sorted));
             }
         }
-        team_sync<W>();
-        const float high = best - (cut_bin - 1) / per_bin, low = best - (cut_bin + 2) / per_bin;
-        uint64_t all = 0;
-        auto weigh_all = [&](auto some) {
-            row.template each<2>([&](int step, const float(&v)[RUN], int c) {
-                uint64_t higher = 0;
-                bool any = false;
+        if (top_p < 1 && !summed) {
+            // The entries that hold top_p of what is left.  A histogram of weights in 32 bits (whole numbers: adding floats in
+            // shared memory takes eight times as long) says near which bin that cut lies.  One pass in 64 bits then sums
+            // everything and, step by step, what is above the neighbours of that bin, and collects what is in the three of
+            // them: if the cut is there, everything is known that the draw needs.  It can be elsewhere where it lies as near to
+            // an edge as 32 bits are off and empty bins follow.
+            team_sync<W>();
+            for (int i = tid; i < BINS; i += THREADS) bin_n[i] = 0;
+            for (int i = tid; i < row.steps; i += THREADS) mass[i] = 0;
+            if (tid == 0) {
+                list.n = 0;
+                cut_bin = BINS - 1;
+            }
+            team_sync<W>();
+            const float scale = 1073741824.0f / guess;
+            row.template each<4>([&](int, const float(&v)[RUN], int c) {
 #pragma unroll
                 for (int j = 0; j < RUN; ++j) {
-                    const float s = !some.value || keeps(v[j], c + j) ? v[j] : -INFINITY;
-                    const uint64_t m = (uint64_t)__double_as_longlong(row_exp2(((double)s - best) * unit) + a.magic);
-                    all += m;
-                    higher += s > high ? m : zero;
-                    any |= (s >= low) & !(s > high);
+                    const float s = !cut || keeps(v[j], c + j) ? v[j] : -INFINITY;
+                    const int m = (int)(__builtin_amdgcn_exp2f((s - best) * unit_f) * scale + 0.5f);
+                    if (m) atomicAdd(&bin_n[bin_of(s)], m);
                 }
-                if (any) {
+            });
+            team_sync<W>();
+            uint32_t own = 0, total = 0;
+#pragma unroll
+            for (int i = 0; i < OWN; ++i) own += (uint32_t)bin_n[tid * OWN + i];
+            uint32_t run = (uint32_t)wave_running((int)own);
+            if ((tid & 63) == 63) part_n[tid >> 6] = (int)run;
+            team_sync<W>();
+#pragma unroll
+            for (int i = 0; i < W; ++i) {
+                if (i < (tid >> 6)) run += (uint32_t)part_n[i];
+                total += (uint32_t)part_n[i];
+            }
+            run -= own;
+            const uint32_t near = (uint32_t)(top_p * total);
+            if (run < near && near <= run + own) {
+#pragma unroll
+                for (int i = 0; i < OWN; ++i) {
+                    if (run < near) cut_bin = tid * OWN + i;
+                    run += (uint32_t)bin_n[tid * OWN + i];
+                }
+            }
+            team_sync<W>();
+            const float high = best - (cut_bin - 1) / per_bin, low = best - (cut_bin + 2) / per_bin;
+            uint64_t all = 0;
+            auto weigh_all = [&](auto some) {
+                row.template each<2>([&](int step, const float(&v)[RUN], int c) {
+                    uint64_t higher = 0;
+                    bool any = false;
 #pragma unroll
                     for (int j = 0; j < RUN; ++j) {
                         const float s = !some.value || keeps(v[j], c + j) ? v[j] : -INFINITY;
-                        if ((s >= low) & !(s > high) & (s > -INFINITY)) {
-                            const int at = atomicAdd(&list.n, 1);
-                            if (at < ROOM) {
-                                list.entry[at] = row_entry(row_key(s), c + j);
-                                list_mass[at] = weigh(s);
+                        const uint64_t m = (uint64_t)__double_as_longlong(row_exp2(((double)s - best) * unit) + a.magic);
+                        all += m;
+                        higher += s > high ? m : zero;
+                        any |= (s >= low) & !(s > high);
+                    }
+                    if (any) {
+#pragma unroll
+                        for (int j = 0; j < RUN; ++j) {
+                            const float s = !some.value || keeps(v[j], c + j) ? v[j] : -INFINITY;
+                            if ((s >= low) & !(s > high) & (s > -INFINITY)) {
+                                const int at = atomicAdd(&list.n, 1);
+                                if (at < ROOM) {
+                                    list.entry[at] = row_entry(row_key(s), c + j);
+                                    list_mass[at] = weigh(s);
+                                }
                             }
                         }
                     }
-                }
-                all -= RUN * zero;
-                higher = wave_sum(higher - RUN * zero);
-                if ((tid & 63) == 0 && higher) atomicAdd((unsigned long long*)&mass[step], (unsigned long long)higher);
-            });
-        };
-        if (cut)
-            weigh_all(std::true_type{});
-        else
-            weigh_all(std::false_type{});
-        all = team_sum<W>(all, part);
-        team_sync<W>();
-        const int n = list.n;
-        if (n > ROOM) return slowly();
-        uint64_t ahead = 0, listed = 0;
-        for (int i = 0; i < row.steps; ++i) ahead += mass[i];
-        for (int i = tid; i < n; i += THREADS) listed += list_mass[i];
-        listed = team_sum<W>(listed, part);
-        const uint64_t target = sample_target(top_p, all);
-        if (ahead >= target || target > ahead + listed) return slowly();
-        cut_at(list_head<W>(list.entry, list_mass, n, target - ahead, sorted));
-        if (floor <= last) tally(n);
-    }
-    if (floor > last) {
-        last = floor;
-        last_class = n_classes;
-    }
-    // weight of every step, and the step in which the goal lies
-    if (!summed) {
-        team_sync<W>();
-        for (int i = tid; i < row.steps; i += THREADS) mass[i] = 0;
-        team_sync<W>();
-        const bool all = last == least && last_class == n_classes;      // not cut
-        row.template each<2>([&](int step, const float(&v)[RUN], int c) {
-            uint64_t sum = 0;
-            if (all) {                                    // what is below `least` weighs nothing
-#pragma unroll
-                for (int j = 0; j < RUN; ++j)
-                    sum += (uint64_t)__double_as_longlong(row_exp2(((double)v[j] - best) * unit) + a.magic);
-                sum -= RUN * zero;
-            } else {
-                float s[RUN], high = -INFINITY;
-#pragma unroll
-                for (int j = 0; j < RUN; ++j) {
-                    s[j] = keeps(v[j], c + j) ? v[j] : -INFINITY;
-                    high = row_max(high, s[j]);
-                }
-                if (high > -INFINITY) {
+                    all -= RUN * zero;
+                    higher = wave_sum(higher - RUN * zero);
+                    if ((tid & 63) == 0 && higher) atomicAdd((unsigned long long*)&mass[step], (unsigned long long)higher);
+                });
+            };
+            if (cut)
+                weigh_all(std::true_type{});
+            else
+                weigh_all(std::false_type{});
+            all = team_sum<W>(all, part);
+            team_sync<W>();
+            const int n = list.n;
+            if (n > ROOM) return false;
+            uint64_t ahead = 0, listed = 0;
+            for (int i = 0; i < row.steps; ++i) ahead += mass[i];
+            for (int i = tid; i < n; i += THREADS) listed += list_mass[i];
+            listed = team_sum<W>(listed, part);
+            const uint64_t target = sample_target(top_p, all);
+            if (ahead >= target || target > ahead + listed) return false;
+            cut_at(list_head<W>(list.entry, list_mass, n, target - ahead, sorted));
+            if (floor <= last) tally(n);
+        }
+        if (floor > last) {
+            last = floor;
+            last_class = n_classes;
+        }
+        // weight of every step, and the step in which the goal lies
+        if (!summed) {
+            team_sync<W>();
+            for (int i = tid; i < row.steps; i += THREADS) mass[i] = 0;
+            team_sync<W>();
+            const bool all = last == least && last_class == n_classes;      // not cut
+            row.template each<2>([&](int step, const float(&v)[RUN], int c) {
+                uint64_t sum = 0;
+                if (all) {                                    // what is below `least` weighs nothing
 #pragma unroll
                     for (int j = 0; j < RUN; ++j)
-                        sum += (uint64_t)__double_as_longlong(row_exp2(((double)s[j] - best) * unit) + a.magic);
+                        sum += (uint64_t)__double_as_longlong(row_exp2(((double)v[j] - best) * unit) + a.magic);
                     sum -= RUN * zero;
+                } else {
+                    float s[RUN], high = -INFINITY;
+#pragma unroll
+                    for (int j = 0; j < RUN; ++j) {
+                        s[j] = keeps(v[j], c + j) ? v[j] : -INFINITY;
+                        high = row_max(high, s[j]);
+                    }
+                    if (high > -INFINITY) {
+#pragma unroll
+                        for (int j = 0; j < RUN; ++j)
+                            sum += (uint64_t)__double_as_longlong(row_exp2(((double)s[j] - best) * unit) + a.magic);
+                        sum -= RUN * zero;
+                    }
                 }
-            }
-            sum = wave_sum(sum);
-            if ((tid & 63) == 0 && sum) atomicAdd((unsigned long long*)&mass[step], (unsigned long long)sum);
-        });
-    }
-    team_sync<W>();
-    uint64_t sum = 0;
-    for (int i = 0; i < row.steps; ++i) sum += mass[i];
-    const uint64_t goal = sample_goal(u, sum);
-    const double log_sum = row_log((double)sum * a.unit);
-    auto answer = [&](float v, int c) {
-        index[r] = c;
-        logprob[r] = (float)(((double)v - best) / t - log_sum);
-    };
-    if (goal == 0) {                                      // below one unit: the first entry that is kept
-        int at = 1 << 30;
-        row.template each<4>([&](int, const float(&v)[RUN], int c) {
+                sum = wave_sum(sum);
+                if ((tid & 63) == 0 && sum) atomicAdd((unsigned long long*)&mass[step], (unsigned long long)sum);
+            });
+        }
+        team_sync<W>();
+        uint64_t sum = 0;
+        for (int i = 0; i < row.steps; ++i) sum += mass[i];
+        const uint64_t goal = sample_goal(u, sum);
+        const double log_sum = row_log((double)sum * a.unit);
+        auto answer = [&](float v, int c) {
+            index[r] = c;
+            logprob[r] = (float)(((double)v - best) / t - log_sum);
+        };
+        if (goal == 0) {                                      // below one unit: the first entry that is kept
+            int at = 1 << 30;
+            row.template each<4>([&](int, const float(&v)[RUN], int c) {
+#pragma unroll
+                for (int j = 0; j < RUN; ++j)
+                    if (keeps(v[j], c + j)) at = min(at, c + j);
+            });
+            at = (int)~(uint32_t)team_max<W>((uint64_t)(uint32_t)~at, part);
+            if (tid == 0) answer((float)mine[at], at);
+            return true;
+        }
+        uint64_t run = 0;
+        int step = 0;
+        while (run + mass[step] <= goal) run += mass[step++];
+        {
+            const int c = row.first_class(step);
+            float v[RUN];
+            Row::decode(row.read_any(step), v);
+            uint64_t own = 0;
 #pragma unroll
             for (int j = 0; j < RUN; ++j)
-                if (keeps(v[j], c + j)) at = min(at, c + j);
-        });
-        at = (int)~(uint32_t)team_max<W>((uint64_t)(uint32_t)~at, part);
-        if (tid == 0) answer((float)mine[at], at);
-        return;
-    }
-    uint64_t run = 0;
-    int step = 0;
-    while (run + mass[step] <= goal) run += mass[step++];
-    {
-        const int c = row.first_class(step);
-        float v[RUN];
-        Row::decode(row.read_any(step), v);
-        uint64_t own = 0;
+                if (keeps(v[j], c + j)) own += weigh(v[j]);
+            uint64_t before = wave_running(own);
+            if (W > 1) {
+                if ((tid & 63) == 63) part[tid >> 6] = before;
+                team_sync<W>();
 #pragma unroll
-        for (int j = 0; j < RUN; ++j)
-            if (keeps(v[j], c + j)) own += weigh(v[j]);
-        uint64_t before = wave_running(own);
-        if (W > 1) {
-            if ((tid & 63) == 63) part[tid >> 6] = before;
-            team_sync<W>();
+                for (int k = 0; k < W; ++k)
+                    if (k < (tid >> 6)) before += part[k];
+            }
+            before += run - own;
+            if (before <= goal && goal < before + own) {
+                bool found = false;
 #pragma unroll
-            for (int k = 0; k < W; ++k)
-                if (k < (tid >> 6)) before += part[k];
-        }
-        before += run - own;
-        if (before <= goal && goal < before + own) {
-            bool found = false;
-#pragma unroll
-            for (int j = 0; j < RUN; ++j) {
-                const uint64_t m = keeps(v[j], c + j) ? weigh(v[j]) : 0;
-                if (!found && goal < before + m) {
-                    found = true;
-                    answer(v[j], c + j);
+                for (int j = 0; j < RUN; ++j) {
+                    const uint64_t m = keeps(v[j], c + j) ? weigh(v[j]) : 0;
+                    if (!found && goal < before + m) {
+                        found = true;
+                        answer(v[j], c + j);
+                    }
+                    before += m;
                 }
-                before += m;
             }
         }
-    }
+        return true;
+    };
+    if (best == INFINITY || !fast())
+        sample_by_radix<DT, W>(mine, n_classes, best, t, top_k, top_p, min_p, u, a, mass, &above, index + r, logprob + r);
 }
 
 template <int DT, int W>
