@@ -224,16 +224,27 @@ __global__ __launch_bounds__(LSR_ROW_THREADS) void lsr_top_quad_kernel(const typ
     else
         quad_sort<E>(e, q);
     double least = 3.9;                                   // entry at place k - 1
+    if (REST) {
 #pragma unroll
-    for (int i = 0; i < (HEAD ? HEAD : E); ++i) {
-        const int place = HEAD ? i : q * E + i;
-        if (REST) least = place == k - 1 ? e[i] : least;
-        // with HEAD all lanes hold the same places: lane q writes the places that are q modulo 4
-        if (live && place < k && (!HEAD || (place & 3) == q)) {
-            const float v = quad_entry_value(e[i]);
+        for (int i = 0; i < (HEAD ? HEAD : E); ++i) least = (HEAD ? i : q * E + i) == k - 1 ? e[i] : least;
+    }
+    auto write = [&](int place, double entry) {
+        if (live && place < k) {
+            const float v = quad_entry_value(entry);
             values[r * k + place] = v;
-            index[r * k + place] = v > -INFINITY ? quad_entry_class(e[i]) : -1;
+            index[r * k + place] = v > -INFINITY ? quad_entry_class(entry) : -1;
         }
+    };
+    if constexpr (HEAD > 0) {                             // all lanes hold the same places: four at a time, a lane each
+#pragma unroll
+        for (int i = 0; i < HEAD; i += 4) {
+            const double one = e[i], two = e[i + 1], three = e[i + 2], four = e[i + 3];
+            const double even = q & 2 ? three : one, odd = q & 2 ? four : two;
+            write(i + q, q & 1 ? odd : even);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < E; ++i) write(q * E + i, e[i]);
     }
     if (!REST) return;
     if (!HEAD) least = quad_min(least);
