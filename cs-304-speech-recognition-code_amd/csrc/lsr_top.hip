@@ -200,8 +200,8 @@ static void lsr_top_team(lsr_ctx* ctx, const void* scores_d, int64_t n_rows, int
 
 // Short rows (at most LSR_QUAD_CLASSES classes), a quad per row: the entries are sorted by a network over the quad's
 // registers.  HEAD: the number of places that are put in order, 0 for all (k > E).  2.2 M x 58 with k = 8 and the rest takes
-// 182 us, 3.6 TB/s read and written: 742 vector instructions per 16 rows are two thirds of that, and overlap only in part
-// with the loads.
+// 164 us, 4.1 TB/s read and written, and is bound by 686 vector instructions per 16 rows as much as by memory.  Writing the
+// eight places one by one, each by one lane of the quad, took 182 us.
 template <int DT, int E, int HEAD, bool REST>
 __global__ __launch_bounds__(LSR_ROW_THREADS) void lsr_top_quad_kernel(const typename row_type<DT>::type* __restrict__ scores,
                                                                        int64_t n_rows, int n_classes, int64_t row_stride, int k,
