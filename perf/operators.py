@@ -230,8 +230,7 @@ def _plain_distill(s, values, index, rest, temperature, weight, grad):
     loss = terms.sum(dim=1, keepdim=True)
     q = e / total
     if rest is not None:
-        beyond = torch.where(there, at, q.shape[1])         # absent entries list no class
-        outside = torch.ones((q.shape[0], q.shape[1] + 1), device=q.device).scatter_(1, beyond, 0.0)[:, :-1]
+        outside = torch.ones_like(q).scatter_(1, at, 0.0)
         q_rest = (q * outside).sum(dim=1, keepdim=True)
         loss = loss + torch.where(p_rest > 0, p_rest * (torch.log(torch.where(p_rest > 0, p_rest, 1.0)) - torch.log(q_rest)), 0.0)
     out = {"loss": (weight[:, None] * temperature ** 2 * loss)[:, 0]}
