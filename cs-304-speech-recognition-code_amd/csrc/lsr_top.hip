@@ -81,6 +81,7 @@ __global__ __launch_bounds__(64 * W) void lsr_top_team_kernel(const typename row
         bool equal = true;                                // every score that equals the bound is collected
         if (n > ROOM) {                                   // thousands of equal scores, as a rule: first what is above them
             equal = false;
+            team_sync<W>();                               // every wavefront has read the count before it is cleared
             if (tid == 0) list.n = 0;
             team_sync<W>();
             again.template each<4>([&](int, const float(&v)[RUN], int c) {

@@ -1,0 +1,110 @@
+"""Score-row operators on the GPU: the paths that only rows of particular sizes, counts or contents take, against plain
+64-bit forms (scores_reference.py) and against the same rows in calls that take another path."""
+import numpy as np
+import pytest
+import torch
+
+import scores_reference as R
+
+pytestmark = pytest.mark.gpu
+
+TYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+
+
+def _chain(classes, dtype):
+    """Most additions in 32 bits that a term of a long row's sum goes through: the classes of one thread of its team, the
+    entries of a list that a thread adds, six steps over the lanes, one per wavefront and the last ones."""
+    run, four = (4, 8192) if dtype == "f32" else (8, 16384)
+    least = 64 * (1 if classes <= 1024 else 4 if classes <= four else 8 if classes <= 4 * four else 16)
+    return -(-classes // (least * run)) * run + 8 + 6 + 16 + 4
+
+
+def _rest_error(x, dtype, t, q):
+    """Bound of the error of ``rest``: arguments of the exponentials off by five roundings (difference, reciprocal of t, its
+    product with log2 e, that constant, product) of at most the row's range, two exponentials of one step each and their
+    product, the additions; the logarithm, the distance to the best and their sum four roundings of what they add up to."""
+    there = x[np.isfinite(x)]
+    span = min(104.0, (there.max() - there.min()) / t) if len(there) else 0.0
+    gap = (there.max() - there.min()) / t if len(there) > 1 else 0.0
+    return 2.0 ** -24 * (5 * span + 8 + _chain(len(x), dtype)) + 2.0 ** -24 * 4 * (abs(q) + min(gap, abs(q) + 17))
+
+
+def _check_rows_of_top(got, x, rows, k, t, dtype):
+    values, index, rest = got
+    for r in rows:
+        row = x[r].double().cpu().numpy()
+        v, i, q = R.top(row, k, t)
+        assert np.array_equal(index[r].cpu().numpy(), i) and np.array_equal(values[r].double().cpu().numpy(), v), r
+        if rest is not None:
+            assert rest[r].item() == q or abs(rest[r].item() - q) <= _rest_error(row, dtype, t, q), (r, rest[r].item(), q)
+
+
+def _all_kinds(rng, rows, classes, dtype):
+    """Ordinary rows with, every few rows, one that a list of the first entries cannot answer at once: nearly all classes masked
+    with the type's lowest number; half of them equal to the best; high scores in a few places that lie 8192 classes apart, so
+    that thousands of them are above what a bound from groups of classes finds; NaN among the scores; no score; a few."""
+    x = torch.tensor(rng.normal(size=(rows, classes)).astype(np.float32)).to(TYPES[dtype])
+    place = np.arange(classes) % 8192 // 32
+    for r in range(0, rows):
+        kind = r % 13
+        if kind == 1:
+            x[r, rng.random(classes) > 1e-3] = torch.finfo(x.dtype).min
+        elif kind == 3:
+            x[r, rng.random(classes) < 0.5] = 9.0
+        elif kind == 5:
+            x[r] -= 100.0
+            x[r, place < 20] += 100.0
+        elif kind == 7:
+            x[r, rng.integers(0, classes, 50)] = float("nan")
+        elif kind == 9:
+            x[r] = float("-inf")
+        elif kind == 10:
+            x[r] = float("-inf")
+            x[r, rng.integers(0, classes, 5)] = 1.0
+        elif kind == 12:
+            x[r, -3:] = torch.tensor([30.0, 31.0, 32.0])  # in the run that is cut short, where the width has one
+    return x
+
+
+@pytest.mark.parametrize("k", [1, 31, 64, 65])
+@pytest.mark.parametrize("classes,dtype", [(65537, "bf16"), (66000, "f16"), (70003, "bf16"), (131072, "bf16"), (131071, "f16")])
+def test_top_scores_of_workgroups_that_go_on(classes, dtype, k):
+    """More rows of 16 wavefronts than compute units: for k of at most 64 a workgroup goes on to its next rows.  The results are
+    those of calls of a few rows, which have a workgroup for each row, and those of the plain form."""
+    from loe_speech_recognition_amd import top_scores
+
+    rng = np.random.default_rng(classes + k)
+    units = torch.cuda.get_device_properties(0).multi_processor_count
+    rows = 2 * units + 77
+    base = _all_kinds(rng, 130, classes, dtype)
+    buf = torch.full((rows, classes + 3), 7.0, dtype=base.dtype, device="cuda")
+    x = buf[:, :classes]
+    pick = torch.arange(rows) * 37 % 130                  # a row's predecessors in its workgroup are of other kinds
+    x.copy_(base.cuda()[pick.cuda()])
+    for t in (1.0, 3.0):
+        got = top_scores(x, k, temperature=t, want_rest=True)
+        for lo in range(0, 130, 65):
+            few = top_scores(base[lo:lo + 65].cuda(), k, temperature=t, want_rest=True)
+            for a, b in zip(got, few):
+                for r in range(rows):
+                    if lo <= pick[r] < lo + 65:
+                        assert torch.equal(a[r], b[pick[r] - lo]), (t, r, int(pick[r]) % 13)
+        _check_rows_of_top(got, x, range(rows - 26, rows), k, t, dtype)
+        only = top_scores(x, k, temperature=t)
+        assert only[2] is None and torch.equal(only[0], got[0]) and torch.equal(only[1], got[1])
+
+
+@pytest.mark.parametrize("classes,dtype", [(600, "bf16"), (1000, "f16"), (3000, "f32"), (9000, "f32"), (9000, "bf16"), (40000, "f32"),
+                                           (40000, "f16"), (200000, "f32")])
+def test_top_scores_when_the_list_overflows(classes, dtype):
+    """Teams of 1, 4, 8 and 16 wavefronts: rows whose list is cleared and filled again, eight times over the same rows."""
+    from loe_speech_recognition_amd import top_scores
+
+    rng = np.random.default_rng(classes)
+    x = _all_kinds(rng, 39, classes, dtype).cuda()
+    for k in (7, 64, 200, 256):
+        first = top_scores(x, k, want_rest=True)
+        _check_rows_of_top(first, x, range(39), k, 1.0, dtype)
+        for _ in range(7):
+            for a, b in zip(top_scores(x, k, want_rest=True), first):
+                assert torch.equal(a, b)
