@@ -105,6 +105,7 @@ __global__ __launch_bounds__(64 * W) void lsr_distill_team_kernel(
             list_z = z_l;
         }
     }
+    if (W == 1) team_sync<W>();                           // larger teams meet in team_max before they read what is above
     row.arrive();
     // the runs of the row without the listed classes
     auto blank = [&](int step, uint4& u) {

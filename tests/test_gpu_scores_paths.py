@@ -108,3 +108,28 @@ def test_top_scores_when_the_list_overflows(classes, dtype):
         for _ in range(7):
             for a, b in zip(top_scores(x, k, want_rest=True), first):
                 assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("classes,dtype", [(129, "f32"), (600, "bf16"), (1000, "f32"), (1024, "f16")])
+def test_distill_scores_of_one_wavefront(classes, dtype):
+    """A wavefront hands what its list adds up to from one lane to all: entries given several times and lists that end in every
+    lane, the same bits as for the row alone, and the loss of the formula."""
+    from loe_speech_recognition_amd import distill_scores
+
+    rng = np.random.default_rng(classes)
+    rows = 300
+    x = torch.tensor(rng.normal(size=(rows, classes)) * 2).to(TYPES[dtype]).cuda()
+    for k in (1, 63, 64, 65, 128, 200):
+        k = min(k, classes)
+        values = torch.tensor(rng.normal(size=(rows, k)), dtype=torch.float32, device="cuda")
+        index = torch.tensor(rng.integers(-1, classes, (rows, k)), dtype=torch.int32, device="cuda")
+        rest = torch.tensor(rng.normal(size=rows), dtype=torch.float32, device="cuda")
+        loss, grad = distill_scores(x, values, index, rest=rest)
+        for r in range(0, rows, 23):
+            one = distill_scores(x[r:r + 1], values[r:r + 1], index[r:r + 1], rest=rest[r:r + 1])
+            assert torch.equal(one[0][0], loss[r]) and torch.equal(one[1][0], grad[r])
+            row = x[r].double().cpu().numpy()
+            want, _ = R.distill(row, values[r].cpu().numpy(), index[r].cpu().numpy(), rest[r].item(), 1.0)
+            # the sum over the others in 32 bits, with the weight of the rest; all else in 64 bits; one rounding at the end
+            span = row.max() - row.min()
+            assert abs(loss[r].item() - want) <= 2.0 ** -24 * (5 * span + 4 + _chain(classes, dtype) + abs(want)), (r, k)
