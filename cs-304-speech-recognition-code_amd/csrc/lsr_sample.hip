@@ -279,18 +279,24 @@ __global__ __launch_bounds__(64 * W) void lsr_sample_team_kernel(const typename 
         // many entries reach it.  nucleus: top_p alone, where it looks as if a short head will do: where the best scores of the
         // groups hold that share of the row's weight.
         const bool cut = top_k > 0 && top_k < n_classes, few = cut && top_k <= LSR_MAX_TOP, level = !cut && min_p > 0;
-        const float floor = min_p > 0 ? sample_floor(best, t, min_p) : -INFINITY, unit_f = (float)unit;
+        const float floor = min_p > 0 ? sample_floor(best, t, min_p) : -INFINITY;
+        if (!few && top_p < 1 && unit > 3e38) return false;   // a temperature whose reciprocal 32 bits do not hold
+        // weights in 32 bits, always a number in [0, 1]: 0 for NaN
+        const float unit_f = (float)unit;
+        auto weigh_f = [&](float v) { return __builtin_amdgcn_exp2f(row_max((v - best) * unit_f, -INFINITY)); };
         bool nucleus = !cut && !level && top_p < 1;
-        float guess = 0;                                      // the row's weight in 32 bits, good to 2^-12 and better
+        // the row's weight in 32 bits: at most 2^14 additions per thread, 22 over the team, and exponentials off by 2^-17, so
+        // that it is good to 2^-9
+        float guess = 0;
         if (!few && top_p < 1) {
             float head = 0;
             row.template each<4>([&](int, const float(&v)[RUN], int) {
 #pragma unroll
-                for (int j = 0; j < RUN; ++j) guess += __builtin_amdgcn_exp2f((v[j] - best) * unit_f);
+                for (int j = 0; j < RUN; ++j) guess += weigh_f(v[j]);
             });
             guess = team_sum<W>(guess, part_f);
             for (int i = tid; i < ROW_GROUPS; i += THREADS)
-                if (list.group[i]) head += __builtin_amdgcn_exp2f((row_value(list.group[i]) - best) * unit_f);
+                if (list.group[i]) head += weigh_f(row_value(list.group[i]));
             nucleus = nucleus && team_sum<W>(head, part_f) >= (float)top_p * guess;
         }
         if (few || level || nucleus) {
@@ -307,7 +313,7 @@ __global__ __launch_bounds__(64 * W) void lsr_sample_team_kernel(const typename 
                 if (level && !open) {
                     float listed = 0;
                     for (int i = tid; i < n; i += THREADS)
-                        listed += __builtin_amdgcn_exp2f((row_value((uint32_t)(list.entry[i] >> 32)) - best) * unit_f);
+                        listed += weigh_f(row_value((uint32_t)(list.entry[i] >> 32)));
                     open = team_sum<W>(listed, part_f) < (1 - 1.0f / 512) * (float)top_p * guess;
                 }
                 if (!few && !open) {
@@ -491,7 +497,7 @@ __global__ __launch_bounds__(64 * W) void lsr_sample_team_kernel(const typename 
 #pragma unroll
                 for (int j = 0; j < RUN; ++j) {
                     const float s = !cut || keeps(v[j], c + j) ? v[j] : -INFINITY;
-                    const int m = (int)(__builtin_amdgcn_exp2f((s - best) * unit_f) * scale + 0.5f);
+                    const int m = (int)(weigh_f(s) * scale + 0.5f);
                     if (m) atomicAdd(&bin_n[bin_of(s)], m);
                 }
             });
