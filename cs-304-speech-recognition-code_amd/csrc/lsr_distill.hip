@@ -152,10 +152,12 @@ __global__ __launch_bounds__(64 * W) void lsr_distill_team_kernel(
     });
     const float m_r = team_max<W>(high, part_f);
     const float unit_f = (float)unit, from = m_r > -INFINITY ? m_r : 0.0f;
-    float part = 0;
+    typename Row::sum_t part = 0;
     each([&](const float(&v)[RUN], int) {
+        float sum = N ? part : 0.0f;
 #pragma unroll
-        for (int j = 0; j < RUN; ++j) part += __builtin_amdgcn_exp2f((v[j] - from) * unit_f);
+        for (int j = 0; j < RUN; ++j) sum += __builtin_amdgcn_exp2f((v[j] - from) * unit_f);
+        part = N ? sum : part + sum;
     });
     const double z_r = team_sum<W>((double)part, part_d);
 

@@ -6,6 +6,8 @@
 // m entries" is always "the entries whose number is at least some threshold".
 #pragma once
 
+#include <type_traits>
+
 #include "lsr_internal.h"
 
 #define LSR_ROW_THREADS 256
@@ -405,6 +407,9 @@ template <int W, typename V> __device__ __forceinline__ V team_max(V v, V* share
 
 template <int DT, int W, int N> struct team_row {
     using T = typename row_type<DT>::type;
+    // A thread's sum over a row: a kept row has at most 128 terms per thread, one that is read again up to 2^14 (of equal
+    // size, as a rule, so that 32-bit sums would be off to one side): those are added up in 64 bits, run by run.
+    using sum_t = std::conditional_t<(N > 0), float, double>;
     static constexpr int RUN = 16 / (int)sizeof(T), THREADS = 64 * W, STEP = THREADS * RUN;   // classes of a run, of a step
 
     const T* row;
@@ -595,11 +600,11 @@ __device__ __forceinline__ float team_groups(team_row<DT, W, N>& row, team_list<
     return best ? row_value(best) : -INFINITY;
 }
 // Collects the entries that reach `bound`; `list.n`, 0 on entry, may exceed the list's size: then only some of them are there.
-// SUM: also this thread's sum of e^((x - bound) unit ln 2) over what stays below the bound, in the same pass; NaN where the
-// thread has seen one.  NEXT: a kept row is asked for the next row, `next`, on the way.
+// SUM: also this thread's sum of e^((x - bound) unit ln 2) over what stays below the bound, in the same pass, added to
+// `below`; NaN where the thread has seen one.  NEXT: a kept row is asked for the next row, `next`, on the way.
 template <bool SUM, bool NEXT, int DT, int W, int N, int SIZE>
-__device__ __forceinline__ void team_take(team_row<DT, W, N>& row, float bound, team_list<W, SIZE>& list, float unit, float& below,
-                                          const typename row_type<DT>::type* next) {
+__device__ __forceinline__ void team_take(team_row<DT, W, N>& row, float bound, team_list<W, SIZE>& list, float unit,
+                                          typename team_row<DT, W, N>::sum_t& below, const typename row_type<DT>::type* next) {
     constexpr int RUN = team_row<DT, W, N>::RUN;
     row.next_pass();
     auto take = [&](int step, const uint4& packed) {
@@ -607,6 +612,7 @@ __device__ __forceinline__ void team_take(team_row<DT, W, N>& row, float bound, 
         team_row<DT, W, N>::decode(packed, v);
         const int c = row.first_class(step);
         bool any = false;
+        float sum = N ? below : 0.0f;
 #pragma unroll
         for (int j = 0; j < RUN; ++j) any |= v[j] >= bound;
         if (any) {
@@ -616,12 +622,13 @@ __device__ __forceinline__ void team_take(team_row<DT, W, N>& row, float bound, 
                     const int at = atomicAdd(&list.n, 1);
                     if (at < SIZE) list.entry[at] = row_entry(row_key(v[j]), c + j);
                 }
-                if (SUM) below += v[j] < bound ? __builtin_amdgcn_exp2f((v[j] - bound) * unit) : 0.0f;
+                if (SUM) sum += v[j] < bound ? __builtin_amdgcn_exp2f((v[j] - bound) * unit) : 0.0f;
             }
         } else if (SUM) {
 #pragma unroll
-            for (int j = 0; j < RUN; ++j) below += __builtin_amdgcn_exp2f((v[j] - bound) * unit);
+            for (int j = 0; j < RUN; ++j) sum += __builtin_amdgcn_exp2f((v[j] - bound) * unit);
         }
+        if (SUM) below = N ? sum : below + sum;
     };
     if constexpr (NEXT)
         row.each_run_then(next, take);

@@ -300,7 +300,8 @@ __global__ __launch_bounds__(64 * W) void lsr_sample_team_kernel(const typename 
             nucleus = nucleus && team_sum<W>(head, part_f) >= (float)top_p * guess;
         }
         if (few || level || nucleus) {
-            float none = 0, bound = few || nucleus ? team_bound(few ? top_k : NUCLEUS < n_classes ? NUCLEUS : n_classes, list) : floor;
+            double none = 0;
+            float bound = few || nucleus ? team_bound(few ? top_k : NUCLEUS < n_classes ? NUCLEUS : n_classes, list) : floor;
             if (level && tid == 0) list.n = 0;
             if (level) team_sync<W>();
             team_take<false, false>(row, row_max(bound, least), list, 0.0f, none, mine);

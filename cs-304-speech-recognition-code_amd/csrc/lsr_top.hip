@@ -72,7 +72,7 @@ __global__ __launch_bounds__(64 * W) void lsr_top_team_kernel(const typename row
         row.arrive();
         if (!N) row.open(mine, n_classes);
         team_groups(row, list);
-        float below = 0.0f;
+        typename team_row<DT, W, N>::sum_t below = 0;
         float bound = team_bound(kk, list);
         team_take<REST, ON>(row, bound, list, unit, below, mine + (r + gridDim.x < n_rows ? gridDim.x * row_stride : 0));
         team_row<DT, W, 0> again;                         // for the cases that need the row once more
@@ -161,14 +161,18 @@ __global__ __launch_bounds__(64 * W) void lsr_top_team_kernel(const typename row
             const bool spoilt = equal && team_max<W>(below != below ? 1.0f : 0.0f, part) > 0;
             if (from > -INFINITY) {
                 if (equal && !spoilt) {                   // relative to the bound, which an entry of the rest reaches
-                    if (below > 0) sum += below * __builtin_amdgcn_exp2f((bound - from) * unit);
+                    if (below > 0) sum += (float)below * __builtin_amdgcn_exp2f((bound - from) * unit);
                 } else {
+                    double far = 0;
                     again.template each<1>([&](int, const float(&v)[RUN], int c) {
+                        float run = 0;
 #pragma unroll
                         for (int j = 0; j < RUN; ++j)
                             if (v[j] < bound || (!equal && v[j] == bound && c + j > bound_class))
-                                sum += v[j] == from ? 1.0f : __builtin_amdgcn_exp2f((v[j] - from) * unit);
+                                run += v[j] == from ? 1.0f : __builtin_amdgcn_exp2f((v[j] - from) * unit);
+                        far += run;
                     });
+                    sum += (float)far;
                 }
             }
             sum = team_sum<W>(sum, part);

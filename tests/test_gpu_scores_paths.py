@@ -175,3 +175,58 @@ def test_sample_scores_next_to_zero_at_the_lowest_temperatures():
         for r in range(rows):
             i, lp = R.sample(x[r].double().numpy(), float(u[r]), float(t[r]), 0, top_p, min_p)
             assert index[r].item() == i and abs(share[r].item() - lp) <= 2.0 ** -24 * abs(lp) + 1e-10, (r, top_p, min_p)
+
+
+@pytest.mark.parametrize("classes,dtype", [(1 << 21, "f32"), (1 << 24, "bf16"), ((1 << 24) - 5, "f16")])
+def test_sums_over_rows_that_are_not_kept(classes, dtype):
+    """Millions of equal scores, the widest rows: adding them one after the other in 32 bits is off by 2^-12 to one side.  Bounds:
+    five roundings of the arguments, the exponentials and their products, eight additions of a run, the list's and the
+    team's."""
+    from loe_speech_recognition_amd import distill_scores, top_scores
+
+    rng = np.random.default_rng(classes)
+    for gap in (2.9, 3.6):
+        row = np.full((1, classes), -gap)
+        row[0, rng.integers(0, classes, 3000)] = rng.uniform(0.0, 1.0, 3000)
+        row[0, -2:] = -gap / 2
+        x = torch.tensor(row).to(TYPES[dtype])
+        exact = x[0].double().numpy()
+        view = x.cuda()
+        v, i, q = R.top(exact, 50, 1.0)
+        values, index, rest = top_scores(view, 50, want_rest=True)
+        assert np.array_equal(index[0].cpu().numpy(), i) and np.array_equal(values[0].double().cpu().numpy(), v)
+        error = 2.0 ** -24 * (5 * (gap + 1) + 8 + 8 + 8 + 6 + 16 + 4)
+        assert abs(rest[0].item() - q) <= error + 2.0 ** -24 * 4 * (2 * abs(q) + 1), (gap, rest[0].item(), q)
+        teacher = values.flip(1).contiguous(), index
+        for r in (rest, None):
+            loss, grad = distill_scores(view, *teacher, rest=r)
+            want, g = R.distill(exact, teacher[0][0].cpu().numpy(), i, None if r is None else r[0].item(), 1.0)
+            assert abs(loss[0].item() - want) <= error + 2.0 ** -24 * abs(want), (gap, loss[0].item(), want)
+            # a term of the gradient is off by the sum's error, its own exponential's and its rounding, and is no larger than this
+            size = np.abs(g) + np.exp(exact - exact.max()) * (1 if r is None else 2) / np.exp(exact - exact.max()).sum()
+            step = torch.finfo(TYPES[dtype]).eps / 2
+            tiny = 2.0 ** -25 if dtype == "f16" else 0.0
+            assert np.all(np.abs(grad[0].double().cpu().numpy() - g) <= (3 * error + step * (1 + 2.0 ** -8)) * size + tiny + 2.0 ** -120)
+
+
+@pytest.mark.parametrize("classes,dtype", [(300007, "f32"), (300007, "bf16"), (70001, "f16"), (50001, "f32"), (1001, "f16"), (4099, "f32")])
+def test_the_last_classes_carry_the_rest(classes, dtype):
+    """The run of a row that is cut short holds nearly all of the weight that is not listed: leaving any of it out shows."""
+    from loe_speech_recognition_amd import distill_scores, sample_scores, top_scores
+
+    rng = np.random.default_rng(classes)
+    x = rng.normal(size=(4, classes)) - 30.0
+    x[:, :7] = 20.0 + np.arange(7)
+    last = classes % (4 if dtype == "f32" else 8)
+    x[:, -last:] = rng.uniform(5.0, 8.0, (4, last))
+    x = torch.tensor(x).to(TYPES[dtype])
+    values, index, rest = top_scores(x.cuda(), 7, want_rest=True)
+    loss, grad = distill_scores(x.cuda(), values - 1.0, index, rest=rest + 3.0)
+    index2, share = sample_scores(x.cuda(), torch.full((4,), 1.0 - 2.0 ** -24, device="cuda"), temperature=40.0)
+    for r in range(4):
+        row = x[r].double().numpy()
+        v, i, q = R.top(row, 7, 1.0)
+        assert np.array_equal(index[r].cpu().numpy(), i) and abs(rest[r].item() - q) <= 2.0 ** -24 * (5 * 60 + 100) + 2.0 ** -22 * 40
+        want, g = R.distill(row, v - 1.0, i, rest[r].item() + 3.0, 1.0)
+        assert abs(loss[r].item() - want) <= 2.0 ** -24 * (5 * 60 + 100 + abs(want) + 8 * 40)
+        assert index2[r].item() == R.sample(row, 1.0 - 2.0 ** -24, 40.0, 0, 1.0, 0.0)[0]
