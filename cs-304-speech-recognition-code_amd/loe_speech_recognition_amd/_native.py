@@ -208,17 +208,17 @@ class Engine:
         _hip_pid = os.getpid()
         torch.cuda.set_device(device)
         self.device = torch.device("cuda", device)
-        ctx = c_void_p()
-        rc = self.lib.lsr_ctx_create(device, ctypes.byref(ctx))
-        if rc != 0 or not ctx.value:
-            raise NativeError(f"lsr_ctx_create({device}) failed with code {rc}")
-        self.ctx = ctx
+        self.ctx = self._create_context()
+        # The operators on rows of scores have a context of their own: any thread may call them, on any stream, while the
+        # thread that decodes uses ``ctx``, and a context's stream, error text and event lists belong to one call at a time.
+        self.rows_ctx = self._create_context()
         self._stream = torch.cuda.current_stream(self.device)
         self._stream_handle = self._stream.cuda_stream
         # the raw handle of the current stream without making a Stream object of it (a sixth of the time), where torch has it
         self._raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
             lambda index: torch.cuda.current_stream(index).cuda_stream)
-        self._check(self.lib.lsr_set_stream(self.ctx, c_void_p(self._stream.cuda_stream)))
+        for ctx in (self.ctx, self.rows_ctx):
+            self._check(self.lib.lsr_set_stream(ctx, c_void_p(self._stream.cuda_stream)), ctx)
         self._model_token = None
         self._graph_token = None
         self._rotated = {}               # token -> triangularised whitening matrices (at most 8 kept)
@@ -229,9 +229,16 @@ class Engine:
         self._between = None
 
     # -- helpers ----------------------------------------------------------------------------------
-    def _check(self, rc: int) -> None:
+    def _create_context(self) -> c_void_p:
+        ctx = c_void_p()
+        rc = self.lib.lsr_ctx_create(self.device_index, ctypes.byref(ctx))
+        if rc != 0 or not ctx.value:
+            raise NativeError(f"lsr_ctx_create({self.device_index}) failed with code {rc}")
+        return ctx
+
+    def _check(self, rc: int, ctx: Optional[c_void_p] = None) -> None:
         if rc != 0:
-            msg = self.lib.lsr_last_error(self.ctx)
+            msg = self.lib.lsr_last_error(self.ctx if ctx is None else ctx)
             raise NativeError(f"liblsr_hip error {rc}: {msg.decode() if msg else ''}")
 
     def _check_audio(self, rc: int) -> None:
@@ -245,9 +252,11 @@ class Engine:
         self._check(rc)
 
     def close(self) -> None:
-        if getattr(self, "ctx", None) is not None and self.ctx.value:
-            self.lib.lsr_ctx_destroy(self.ctx)
-            self.ctx = c_void_p()
+        for name in ("ctx", "rows_ctx"):
+            ctx = getattr(self, name, None)
+            if ctx is not None and ctx.value:
+                self.lib.lsr_ctx_destroy(ctx)
+                setattr(self, name, c_void_p())
 
     def synchronize(self) -> None:
         self._check(self.lib.lsr_synchronize(self.ctx))
@@ -257,36 +266,38 @@ class Engine:
         on.  Ordering against work already queued on the previous stream is the caller's business (events)."""
         if stream is None:
             stream = self.torch.cuda.current_stream(self.device)
-        self._check(self.lib.lsr_set_stream(self.ctx, c_void_p(stream.cuda_stream)))
-        self._stream = stream
-        self._stream_handle = stream.cuda_stream
+        with self._turn:
+            for ctx in (self.ctx, self.rows_ctx):
+                self._check(self.lib.lsr_set_stream(ctx, c_void_p(stream.cuda_stream)), ctx)
+            self._stream = stream
+            self._stream_handle = stream.cuda_stream
 
     def on_current_stream(self, fn, *args) -> None:
-        """``fn(ctx, *args)`` on torch's current stream, after the work already queued on the engine's stream (the two are
-        usually one).  For entry points that use no workspace of the context.  While the current stream is captured the
+        """``fn(rows_ctx, *args)`` on torch's current stream, after the work already queued on the engine's stream (the two
+        are usually one).  For entry points that use no workspace of the context.  While the current stream is captured the
         engine's earlier work is not waited for: a capture starts from finished work.  Threads that call this at once take
-        turns; the engine's other calls belong to one thread, as the context does."""
+        turns; the engine's other calls, which one thread at a time may make, are not touched by it."""
         with self._turn:
-            cuda = self.torch.cuda
+            cuda, ctx = self.torch.cuda, self.rows_ctx
             before = cuda.current_device()
             handle = self._raw_stream(self.device_index)
             try:
                 if handle == self._stream_handle:
-                    rc = fn(self.ctx, *args)
+                    rc = fn(ctx, *args)
                 else:
                     stream = cuda.current_stream(self.device)
                     if not cuda.is_current_stream_capturing():
                         stream.wait_stream(self._stream)
-                    self._check(self.lib.lsr_set_stream(self.ctx, c_void_p(handle)))
+                    self._check(self.lib.lsr_set_stream(ctx, c_void_p(handle)), ctx)
                     try:
-                        rc = fn(self.ctx, *args)
+                        rc = fn(ctx, *args)
                     finally:
-                        self._check(self.lib.lsr_set_stream(self.ctx, c_void_p(self._stream_handle)))
+                        self._check(self.lib.lsr_set_stream(ctx, c_void_p(self._stream_handle)), ctx)
             finally:
                 if before != self.device_index:              # the library makes its own device the current one
                     cuda.set_device(before)
             if rc:
-                self._check(rc)
+                self._check(rc, ctx)
 
     @staticmethod
     def _ptr(t) -> c_void_p:
@@ -304,15 +315,23 @@ class Engine:
         mode = 0
         if on:
             mode = 1 if only is None else sum(2 << KERNEL_IDS[k] for k in set(only))
-        self._check(self.lib.lsr_profile_enable(self.ctx, mode))
+        with self._turn:
+            for ctx in (self.ctx, self.rows_ctx):
+                self._check(self.lib.lsr_profile_enable(ctx, mode), ctx)
 
     def profile_reset(self) -> None:
-        self._check(self.lib.lsr_profile_reset(self.ctx))
+        with self._turn:
+            for ctx in (self.ctx, self.rows_ctx):
+                self._check(self.lib.lsr_profile_reset(ctx), ctx)
 
     def profile_get(self, kernel: str) -> Tuple[float, int]:
-        ms, n = c_double(0), c_int64(0)
-        self._check(self.lib.lsr_profile_get(self.ctx, KERNEL_IDS[kernel], ctypes.byref(ms), ctypes.byref(n)))
-        return ms.value, n.value
+        total, launches = 0.0, 0
+        with self._turn:
+            for ctx in (self.ctx, self.rows_ctx):
+                ms, n = c_double(0), c_int64(0)
+                self._check(self.lib.lsr_profile_get(ctx, KERNEL_IDS[kernel], ctypes.byref(ms), ctypes.byref(n)), ctx)
+                total, launches = total + ms.value, launches + n.value
+        return total, launches
 
     # -- batches ----------------------------------------------------------------------------------
     UPLOAD_PIPELINE_BYTES = 16 << 20      # lists of host arrays of at least this size go through lsr_upload_host

@@ -13,7 +13,7 @@ Scores are CUDA tensors [rows, classes] of float32, float16 or bfloat16 on the d
 of a row have to be adjacent, rows may have any stride (a slice of the emission matrix is taken as it is).  The kernels run
 on torch's current stream, after what the engine has queued on its own; nothing is allocated besides the results, so
 calls can be captured into a graph.  Results are the same bits whatever the launch.  Threads may call the three at once,
-each on its own stream.
+each on its own stream, also while another thread decodes with the engine.
 """
 from __future__ import annotations
 

@@ -373,8 +373,9 @@ int lsr_unpack_label_records(lsr_ctx* ctx, const uint8_t* records_d, int world, 
  * from row to row (any value >= 0; 0 gives every row the same scores).  Order of a row: score descending, equal scores
  * (-0 and +0 are equal) by ascending class; a score of -infinity or NaN is absent from lsr_top_scores and
  * lsr_sample_scores.  n_rows = 0 is valid and does nothing.  The calls only enqueue kernels: no allocation, no copy and no
- * memset, so they can be captured into a graph, and calls on different streams share nothing.  Results do not depend on
- * the launch: the same inputs give the same bits. */
+ * memset, so they can be captured into a graph; calls on different streams share no device memory.  The context's stream,
+ * error text and event lists are shared by its calls: threads that call at once use a context each (lsr_ctx_create), or
+ * take turns.  Results do not depend on the launch: the same inputs give the same bits. */
 #define LSR_F32 0
 #define LSR_F16 1
 #define LSR_BF16 2

@@ -1,0 +1,123 @@
+"""Score-row operators and the engine's own calls on different streams and in different threads."""
+import ctypes
+import threading
+
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+A_WHILE = 200_000_000              # clock cycles that a stream is kept busy for: tenths of a second
+
+
+@pytest.fixture(scope="module")
+def digits():
+    from loe_speech_recognition_amd import MFCC, HiddenMarkovModelInference, ModelCollection, synthetic
+
+    models = synthetic.load_word_models()
+    inf = HiddenMarkovModelInference.from_models([models[lab] for lab in synthetic.LOOP_ORDER])
+    mc = ModelCollection()
+    mc._models = [models[lab] for lab in synthetic.LOOP_ORDER if lab != "S"]
+    feats = [MFCC.batch(synthetic.batch(seed, 12, 1)[0], 16000) for seed in (31, 32)]
+    return inf, mc, feats
+
+
+def test_a_call_on_a_side_stream_leaves_the_engines_stream_alone(digits):
+    """While one thread is inside an operator's call on a busy side stream, another thread's emission scores are computed on the
+    engine's stream, not behind what the side stream does."""
+    from loe_speech_recognition_amd import _native
+
+    inf, _, feats = digits
+    eng = inf._bind()
+    fb = eng.feature_batch(feats[0])
+    want = eng.emission(fb)[:fb.total_frames].clone()
+    torch.cuda.synchronize()
+    side, out = torch.cuda.Stream(), []
+
+    def decode():
+        got = eng.emission(fb)[:fb.total_frames]
+        eng._stream.synchronize()
+        out.append((bool(torch.equal(got, want)), side.query()))
+
+    def inside(ctx, *args):
+        thread = threading.Thread(target=decode)
+        thread.start()
+        thread.join()
+        return 0
+
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(A_WHILE)
+        eng.on_current_stream(inside)
+    torch.cuda.synchronize()
+    assert out == [(True, False)]                         # the scores were there while the side stream was still busy
+    assert _native.get_engine() is eng
+
+
+def test_errors_of_the_two_contexts_are_their_own():
+    from loe_speech_recognition_amd import _native
+
+    eng = _native.get_engine()
+    p = ctypes.c_void_p(0)
+    with pytest.raises(_native.NativeError, match="lsr_emission_batch: null"):
+        eng._check(eng.lib.lsr_emission_batch(eng.ctx, p, 1, p))
+    with pytest.raises(_native.NativeError, match="lsr_top_scores: unknown element type 9"):
+        eng.on_current_stream(eng.lib.lsr_top_scores, p, 9, 1, 1, 1, 1, 1.0, p, p, p)
+    assert "lsr_emission_batch" in eng.lib.lsr_last_error(eng.ctx).decode()
+
+
+def test_times_of_the_operators_kernels():
+    from loe_speech_recognition_amd import _native, sample_scores, top_scores
+
+    eng = _native.get_engine()
+    x, u = torch.randn((200, 58), device="cuda"), torch.rand(200, device="cuda")
+    try:
+        eng.profile_reset()
+        eng.profile_enable(True, only=("top",))
+        for _ in range(3):
+            top_scores(x, 4)
+        sample_scores(x, u)
+        ms, n = eng.profile_get("top")
+        assert n == 3 and ms > 0 and eng.profile_get("sample") == (0.0, 0)
+    finally:
+        eng.profile_enable(False)
+        eng.profile_reset()
+    assert eng.profile_get("top") == (0.0, 0)
+
+
+def test_threads_while_another_one_decodes(digits):
+    """Four threads with rows on streams of their own, and one that decodes batch after batch: everybody's results are right."""
+    from loe_speech_recognition_amd import sample_scores, top_scores
+
+    inf, mc, feats = digits
+    want_scores = [mc.scores_batch(f) for f in feats]
+    want_words = [inf.predict_batch(f) for f in feats]
+    rng = np.random.default_rng(4)
+    views = [torch.tensor(rng.normal(size=(50, 700 + 300 * i)), dtype=torch.float32, device="cuda") for i in range(4)]
+    u = torch.tensor(rng.random(50), dtype=torch.float32, device="cuda")
+    want = [(top_scores(v, 9)[1], sample_scores(v, u, 0.9, 50, 0.95)[0]) for v in views]
+    torch.cuda.synchronize()
+    wrong, done = [], threading.Event()
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            while not done.is_set():
+                x = views[i] + 0.0
+                got = top_scores(x, 9)[1], sample_scores(x, u, 0.9, 50, 0.95)[0]
+                if not all(bool(torch.equal(a, b)) for a, b in zip(got, want[i])):
+                    wrong.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    try:
+        for turn in range(40):
+            if not np.array_equal(mc.scores_batch(feats[turn % 2]), want_scores[turn % 2]):
+                wrong.append("scores")
+            if inf.predict_batch(feats[turn % 2]) != want_words[turn % 2]:
+                wrong.append("words")
+    finally:
+        done.set()
+        for t in threads:
+            t.join()
+    assert not wrong
