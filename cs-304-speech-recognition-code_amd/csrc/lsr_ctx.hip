@@ -45,6 +45,11 @@ static hipEvent_t take_event(lsr_ctx* ctx) {
 void lsr_prof_begin(lsr_ctx* ctx, int kernel) {
     ctx->prof_open = false;
     if (!ctx->profiling || !(ctx->profile_mask & (1 | LSR_PROFILE_ONLY(kernel)))) return;
+    hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(ctx->stream, &capture) != hipSuccess || capture != hipStreamCaptureStatusNone) {
+        (void)hipGetLastError();
+        return;                                            // a replay would record events that are other launches' by then
+    }
     lsr_ctx::pending p;
     p.kernel = kernel;
     p.start = take_event(ctx);
@@ -64,9 +69,12 @@ void lsr_prof_end(lsr_ctx* ctx) {
 static void drain_profile(lsr_ctx* ctx) {
     for (auto& p : ctx->pend) {
         float ms = 0.f;
-        if (hipEventElapsedTime(&ms, p.start, p.stop) == hipSuccess) {
+        // the launch may have been on another stream than the context has now
+        if (hipEventSynchronize(p.stop) == hipSuccess && hipEventElapsedTime(&ms, p.start, p.stop) == hipSuccess) {
             ctx->prof_ms[p.kernel] += ms;
             ctx->prof_n[p.kernel] += 1;
+        } else {
+            (void)hipGetLastError();                       // not to be taken for the error of the next launch
         }
         ctx->event_pool.push_back(p.start);
         ctx->event_pool.push_back(p.stop);

@@ -121,3 +121,52 @@ def test_threads_while_another_one_decodes(digits):
         for t in threads:
             t.join()
     assert not wrong
+
+
+def test_times_of_calls_on_another_stream():
+    """A kernel that is still waiting on a busy side stream when its time is asked for is waited for, and counted."""
+    from loe_speech_recognition_amd import _native, top_scores
+
+    eng = _native.get_engine()
+    x = torch.randn((200, 58), device="cuda")
+    want = top_scores(x, 4)[1].clone()
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    try:
+        eng.profile_reset()
+        eng.profile_enable(True)
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(A_WHILE)
+            index = top_scores(x, 4)[1]
+        ms, n = eng.profile_get("top")
+        assert n == 1 and ms > 0
+        side.synchronize()
+        assert torch.equal(index, want) and torch.equal(top_scores(x, 4)[1], want)
+    finally:
+        eng.profile_enable(False)
+        eng.profile_reset()
+
+
+def test_captured_calls_are_not_timed():
+    """With timing on, a captured call records no event into its graph: replays leave the times of eager calls alone, and what
+    follows works."""
+    from loe_speech_recognition_amd import _native, top_scores
+
+    eng = _native.get_engine()
+    x = torch.randn((200, 58), device="cuda")
+    want = top_scores(x, 4)[1].clone()
+    torch.cuda.synchronize()
+    try:
+        eng.profile_reset()
+        eng.profile_enable(True)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            index = top_scores(x, 4)[1]
+        for turn in range(3):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(index, want)
+            assert torch.equal(top_scores(x, 4)[1], want) and eng.profile_get("top")[1] == turn + 1
+    finally:
+        eng.profile_enable(False)
+        eng.profile_reset()
