@@ -826,6 +826,7 @@ class Engine:
 _engine: Optional[Engine] = None
 _engine_pid: Optional[int] = None
 _hip_pid: Optional[int] = None          # pid of the process in which an Engine first touched the GPU
+_engine_turn = threading.Lock()
 
 
 def get_engine() -> Engine:
@@ -833,8 +834,10 @@ def get_engine() -> Engine:
     its own; a worker forked AFTER the parent used the GPU gets a NativeError (HIP does not survive fork)."""
     global _engine, _engine_pid
     if _engine is None or _engine_pid != os.getpid():
-        _engine = Engine()                # raises in a child forked from a process that initialised the GPU
-        _engine_pid = os.getpid()
+        with _engine_turn:                # threads whose first calls come at once share one engine
+            if _engine is None or _engine_pid != os.getpid():
+                _engine = Engine()        # raises in a child forked from a process that initialised the GPU
+                _engine_pid = os.getpid()
     return _engine
 
 
