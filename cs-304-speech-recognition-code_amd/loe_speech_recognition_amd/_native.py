@@ -7,6 +7,7 @@ buffers, the stream handle and (in the distributed helpers) torch.distributed on
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import threading
@@ -272,6 +273,23 @@ class Engine:
             self._stream = stream
             self._stream_handle = stream.cuda_stream
 
+    @contextlib.contextmanager
+    def in_order(self):
+        """Engine calls inside come after what torch's current stream has queued and before what it queues next (the two
+        streams are usually one).  For calls whose results are torch's to read: their memory comes from the current stream's
+        pool, where earlier work on that stream may still be using it."""
+        if self._raw_stream(self.device_index) == self._stream_handle:
+            yield
+            return
+        current = self.torch.cuda.current_stream(self.device)
+        if self.torch.cuda.is_current_stream_capturing():
+            raise NativeError("the engine's calls can only be captured on the engine's own stream (Engine.use_stream)")
+        self._stream.wait_stream(current)
+        try:
+            yield
+        finally:
+            current.wait_stream(self._stream)
+
     def on_current_stream(self, fn, *args) -> None:
         """``fn(rows_ctx, *args)`` on torch's current stream, after the work already queued on the engine's stream (the two
         are usually one).  For entry points that use no workspace of the context.  While the current stream is captured the
@@ -433,8 +451,9 @@ class Engine:
         """float32 device tensor [total_frames, 39] (time-major)."""
         out = self.empty((batch.total_frames, DIM), self.torch.float32)
         fn = self.lib.lsr_mfcc_batch_i16 if batch.audio.dtype == self.torch.int16 else self.lib.lsr_mfcc_batch
-        self._check(fn(self.ctx, self._ptr(batch.audio), self._ptr(batch.sample_off),
-                                            self._ptr(batch.frame_off), batch.n, batch.total_frames, self._ptr(out)))
+        with self.in_order():
+            self._check(fn(self.ctx, self._ptr(batch.audio), self._ptr(batch.sample_off),
+                           self._ptr(batch.frame_off), batch.n, batch.total_frames, self._ptr(out)))
         return FeatureBatch(out, batch.frame_off, batch.lengths)
 
     # -- model / graph ----------------------------------------------------------------------------
@@ -537,7 +556,8 @@ class Engine:
     def emission(self, fb: FeatureBatch):
         rows = (fb.total_frames + 63) // 64 * 64
         out = self.empty((rows, int(self.lib.lsr_ll_stride(self.ctx))), self.torch.float32)
-        self._check(self.lib.lsr_emission_batch(self.ctx, self._ptr(fb.feats), fb.total_frames, self._ptr(out)))
+        with self.in_order():
+            self._check(self.lib.lsr_emission_batch(self.ctx, self._ptr(fb.feats), fb.total_frames, self._ptr(out)))
         return out
 
     def decode_loop(self, fb: FeatureBatch, want_paths: bool = False, label_cap: int = 32):
@@ -679,17 +699,18 @@ class Engine:
         scores = self.empty((fb.n,), t.float32)
         paths = self.empty((fb.total_frames,), t.int8) if want_paths else None
         final = self.empty((fb.n, 64), t.float32) if want_final else None
-        if wide:
-            self._check(self.lib.lsr_decode_chain_batch_wide(self.ctx, self._ptr(fb.feats), self._ptr(fb.frame_off), fb.n,
-                                                             fb.total_frames, fb.max_frames, self._ptr(d_off), total_chain,
-                                                             self._ptr(d_state), self._ptr(d_band), self._ptr(d_start),
-                                                             self._ptr(scores), self._ptr(paths)))
-        else:
-            self._check(self.lib.lsr_decode_chain_batch(self.ctx, self._ptr(fb.feats), self._ptr(fb.frame_off), fb.n,
-                                                        fb.total_frames, fb.max_frames, self._ptr(d_off), total_chain,
-                                                        self._ptr(d_state), self._ptr(d_band), self._ptr(d_start),
-                                                        self._ptr(scores), self._ptr(paths), self._ptr(final)))
-        # The chain arrays must outlive the kernels.  They were allocated on the stream the kernels run on, so the
+        with self.in_order():
+            if wide:
+                self._check(self.lib.lsr_decode_chain_batch_wide(self.ctx, self._ptr(fb.feats), self._ptr(fb.frame_off), fb.n,
+                                                                 fb.total_frames, fb.max_frames, self._ptr(d_off), total_chain,
+                                                                 self._ptr(d_state), self._ptr(d_band), self._ptr(d_start),
+                                                                 self._ptr(scores), self._ptr(paths)))
+            else:
+                self._check(self.lib.lsr_decode_chain_batch(self.ctx, self._ptr(fb.feats), self._ptr(fb.frame_off), fb.n,
+                                                            fb.total_frames, fb.max_frames, self._ptr(d_off), total_chain,
+                                                            self._ptr(d_state), self._ptr(d_band), self._ptr(d_start),
+                                                            self._ptr(scores), self._ptr(paths), self._ptr(final)))
+        # The chain arrays must outlive the kernels.  They were allocated on the stream that waits for the kernels, so the
         # caching allocator can only hand their memory to work that is ordered after those kernels; holding the
         # references until the next call keeps that true even if the caller switches torch streams in between.
         self._chain_keepalive = (d_off, d_state, d_band, d_start)
@@ -717,7 +738,8 @@ class Engine:
                 total_chain, self._ptr(d_state), self._ptr(d_band), self._ptr(d_start), self._ptr(scores), self._ptr(paths)]
         if not wide:
             args.append(self._ptr(final))
-        self._check(fn(*args))
+        with self.in_order():
+            self._check(fn(*args))
         self.last_chain = (d_off, d_state)
         self._chain_keepalive = (d_off, d_state, d_band, d_start)
         return (scores, paths, final) if want_final else (scores, paths)
@@ -745,6 +767,9 @@ class Engine:
         d_off = t.arange(n_utts + 1, dtype=t.int64, device=self.device) * n
         out = (d_off, n * n_utts, self.to_device(ids).repeat(n_utts), self.to_device(band).repeat(1, n_utts).contiguous(),
                self.to_device(np.ascontiguousarray(start, dtype=np.uint8)).repeat(n_utts))
+        if self._raw_stream(self.device_index) != self._stream_handle:
+            for a in (out[0], *out[2:]):                 # kept beyond this stream's work: not to be reused under the engine's
+                a.record_stream(self._stream)
         if len(cache) >= 8:
             cache.pop(next(iter(cache)))
         cache[(key, n_utts)] = out

@@ -170,3 +170,84 @@ def test_captured_calls_are_not_timed():
     finally:
         eng.profile_enable(False)
         eng.profile_reset()
+
+
+def test_the_frameworks_rows_on_a_side_stream(digits):
+    """The models' own entry points under another stream than the engine's, while the engine's is busy: they wait for what the
+    engine computes, and give what they give without all that."""
+    inf, mc, feats = digits
+    rng = np.random.default_rng(7)
+    u = rng.random(len(feats[0])).astype(np.float32)
+    fb = inf._bind().feature_batch(feats[0])
+    frames = torch.tensor(rng.random(fb.total_frames), dtype=torch.float32, device="cuda")
+
+    def results():
+        _, *targets = inf.state_targets(fb, 8, temperature=6.0)
+        _, *drawn = inf.sample_states(fb, frames, temperature=6.0, top_p=0.9)
+        return mc.nbest_batch(feats[0], 3), mc.sample_batch(feats[0], u, 100.0, top_p=0.9), [*targets, *drawn]
+
+    want = results()
+    torch.cuda.synchronize()
+    for turn in range(3):
+        torch.cuda._sleep(A_WHILE)                        # on the engine's stream
+        side = torch.cuda.Stream()
+        with torch.cuda.stream(side):
+            got = results()
+            side.synchronize()
+        assert got[0] == want[0] and got[1] == want[1]
+        assert all(torch.equal(a, b) for a, b in zip(got[2], want[2]))
+
+
+def test_rows_are_not_overwritten_under_a_side_stream(digits):
+    """Emission scores that an operator on a busy side stream has still to read: the next batch's do not take their place."""
+    from loe_speech_recognition_amd import top_scores
+
+    inf, _, feats = digits
+    eng = inf._bind()
+    batches = [eng.feature_batch(feats[0]), eng.feature_batch(feats[0][::-1])]
+    want = [[v.clone() for v in inf.state_targets(fb, 5)[1:]] for fb in batches]
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        got = []
+        for turn in range(6):
+            scores = eng.emission(batches[turn % 2])
+            torch.cuda._sleep(A_WHILE // 10)
+            got.append(top_scores(scores[:batches[0].total_frames, :len(inf._multivariate_normals)], 5, want_rest=True))
+            del scores
+        side.synchronize()
+    for turn, out in enumerate(got):
+        assert all(torch.equal(a, b) for a, b in zip(out, want[turn % 2])), turn
+    torch.cuda.synchronize()
+
+
+def test_capturing_the_engines_calls(digits):
+    """On the engine's own stream state scores and their targets can be captured together; under another one the capture is
+    refused, not left without them."""
+    from loe_speech_recognition_amd import _native
+
+    inf, _, feats = digits
+    eng = inf._bind()
+    fb, other = eng.feature_batch(feats[0]), eng.feature_batch(feats[0][::-1])
+    want = [[v.clone() for v in inf.state_targets(b, 5)[1:]] for b in (fb, other)]
+    torch.cuda.synchronize()
+    before, stream = eng._stream, torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(_native.NativeError, match="own stream"):
+        with torch.cuda.graph(graph, stream=stream):
+            inf.state_targets(fb, 5)
+    torch.cuda.synchronize()
+    eng.use_stream(stream)
+    try:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            _, *out = inf.state_targets(fb, 5)
+        first = fb.feats.clone()
+        for turn in range(4):
+            fb.feats.copy_(other.feats if turn % 2 else first)
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(out, want[turn % 2])), turn
+    finally:
+        eng.use_stream(before)
