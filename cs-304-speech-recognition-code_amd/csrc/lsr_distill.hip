@@ -168,7 +168,9 @@ __global__ __launch_bounds__(64 * W) void lsr_distill_team_kernel(
     const double shift = !REST ? 1.0 : z_r == 0 ? 0.0 : row_exp2(((double)m_r - m) * unit);
     const double shift_l = high_l > -INFINITY ? row_exp2(((double)high_l - m) * unit) : 1.0;
     const double z = (REST ? shift_l * list_z : 0.0) + (z_r == 0 ? 0.0 : shift * z_r);
-    const double p_r = REST ? row_exp2(rest_log * ROW_LOG2E) : 0.0, sum = list_sum + p_r;
+    // a rest so heavy that its weight relative to the list's best leaves 64 bits: everything relative to the rest instead
+    const double lift = rest_log > 500 ? rest_log : 0.0, down = lift > 0 ? row_exp2(-lift * ROW_LOG2E) : 1.0;
+    const double p_r = REST ? row_exp2((rest_log - lift) * ROW_LOG2E) : 0.0, sum = list_sum * down + p_r;
     const bool nan = z != z, used = w != 0 && list_best > -INFINITY && (m > -INFINITY || nan);
     const double scale = w * temperature;
     if (tid == 0) {
@@ -176,8 +178,8 @@ __global__ __launch_bounds__(64 * W) void lsr_distill_team_kernel(
         if (used && !nan) {
             // the list's scores were taken relative to its own highest
             const double ln_z = row_log(z), gap = (high_l > -INFINITY ? (double)high_l - m : 0.0) * inv_t;
-            l = (list_cross - list_sum * gap) / sum + ln_z - row_log(sum);
-            if (REST && p_r > 0) l += p_r / sum * (z_r > 0 ? rest_log - row_log(z_r) - ((double)m_r - m) * inv_t : INFINITY);
+            l = (list_cross - list_sum * gap) * down / sum + ln_z - row_log(sum) - lift * (list_sum * down / sum);
+            if (REST && p_r > 0) l += p_r / sum * (z_r > 0 ? rest_log - lift - row_log(z_r) - ((double)m_r - m) * inv_t : INFINITY);
         }
         loss[r] = used ? (nan ? NAN : (float)(w * temperature * temperature * l)) : 0.0f;
     }
@@ -212,7 +214,7 @@ __global__ __launch_bounds__(64 * W) void lsr_distill_team_kernel(
 #pragma unroll 1
             for (int i = 0; i < k; ++i) p += cls[i] == cls[j] ? teacher[i] : 0.0f;
         }
-        g[cls[j]] = (T)(float)(scale * (row_exp2(((double)student[j] - m) * unit) / z - p / sum));
+        g[cls[j]] = (T)(float)(scale * (row_exp2(((double)student[j] - m) * unit) / z - p * down / sum));
     }
 }
 
@@ -332,22 +334,28 @@ __global__ __launch_bounds__(LSR_ROW_THREADS) void lsr_distill_quad_kernel(
     const double z = z_l + (z_r == 0 ? 0.0 : shift * z_r);
     // NaN or +infinity among the scores: their exponentials, and with them the sum, are NaN
     const bool nan = z != z, used = (w != 0) & (best > -INFINITY) & ((m > -INFINITY) | nan);
-    double p_r = 0, rest_log = 0;
+    double p_r = 0, rest_log = 0, down = 1, lifted = 0;
     if (REST) {
         rest_log = (double)rest[r];
+        if (__any(rest_log > 500)) {                      // the rest's weight relative to the list's best may leave 64 bits:
+            const double lift = rest_log > 500 ? rest_log : 0.0;          // everything relative to the rest instead
+            down = row_exp2(-lift * ROW_LOG2E);
+            lifted = lift * (sum * down);
+            rest_log -= lift;
+        }
         p_r = row_exp2(rest_log * ROW_LOG2E);
-        sum += p_r;
+        sum = sum * down + p_r;
     }
     const double ln = row_log(q == 0 ? z : q == 1 ? sum : z_r);
     const double ln_z = quad_move<0x00>(ln), ln_s = quad_move<0x55>(ln), ln_r = quad_move<0xAA>(ln);
     if (live && q == 0) {
-        double l = cross / sum + ln_z - ln_s;
+        double l = cross * down / sum + ln_z - ln_s - lifted / sum;
         if (REST && p_r > 0) l += p_r / sum * (z_r > 0 ? rest_log - ln_r - ((double)m_r - m) * inv_t : INFINITY);
         loss[r] = used ? (nan ? NAN : (float)(w * temperature * temperature * l)) : 0.0f;
     }
     if (!GRAD) return;
     const double scale = w * temperature;
-    const float c_l = (float)(scale / z), c_p = (float)(scale / sum);
+    const float c_l = (float)(scale / z), c_p = (float)(scale * down / sum);
     const float c_r = REST ? (z_r > 0 ? (float)(scale * (shift / z - p_r / sum / z_r)) : 0.0f) : c_l;
     if (REST) {
         // the student's weights of the listed classes take the place of the teacher's, which are in registers now

@@ -230,3 +230,30 @@ def test_the_last_classes_carry_the_rest(classes, dtype):
         want, g = R.distill(row, v - 1.0, i, rest[r].item() + 3.0, 1.0)
         assert abs(loss[r].item() - want) <= 2.0 ** -24 * (5 * 60 + 100 + abs(want) + 8 * 40)
         assert index2[r].item() == R.sample(row, 1.0 - 2.0 ** -24, 40.0, 0, 1.0, 0.0)[0]
+
+
+@pytest.mark.parametrize("classes,dtype", [(11, "f32"), (58, "f32"), (100, "f16"), (300, "f32"), (5000, "bf16"), (20011, "f32"), (150001, "bf16")])
+def test_distill_scores_with_a_rest_that_outweighs_the_list(classes, dtype):
+    """Entries of the teacher that are far below its best classes, which are in the rest: weights e^rest that 64 bits do not
+    hold, next to ordinary rows."""
+    from loe_speech_recognition_amd import distill_scores
+
+    rng = np.random.default_rng(classes)
+    heavy = np.array([0.5, 16.0, 499.0, 501.0, 709.0, 710.0, 800.0, 1e4, 1e30, 3e38, -np.inf, np.nan, 3.0], np.float32)
+    rows, k = len(heavy), 3
+    x = torch.tensor(rng.normal(size=(rows, classes)) * 2).to(TYPES[dtype])
+    values = torch.tensor(rng.normal(size=(rows, k)), dtype=torch.float32)
+    index = torch.tensor(np.stack([rng.permutation(classes)[:k] for _ in range(rows)]), dtype=torch.int32)
+    loss, grad = distill_scores(x.cuda(), values.cuda(), index.cuda(), rest=torch.tensor(heavy).cuda(), temperature=2.0)
+    for r in range(rows):
+        row = x[r].double().numpy()
+        rest = -np.inf if np.isnan(heavy[r]) else float(heavy[r])          # a rest that is no number has no weight
+        want, g = R.distill(row, values[r].numpy(), index[r].numpy(), rest, 2.0)
+        span = (row.max() - row.min()) / 2
+        # sum over the others and its exponentials in 32 bits, their errors in units of the loss (temperature^2) and of the
+        # gradient's terms (temperature), which are at most 2
+        error = 2.0 ** -24 * (5 * span + 8 + 8 + _chain(classes, dtype))
+        assert abs(loss[r].item() - want) <= 4 * error + 2.0 ** -24 * abs(want), (heavy[r], loss[r].item(), want)
+        step = torch.finfo(TYPES[dtype]).eps / 2
+        tiny = 2.0 ** -25 if dtype == "f16" else 0.0
+        assert np.all(np.abs(grad[r].double().numpy(force=True) - g) <= 4 * error + step * (1 + 2.0 ** -8) * np.abs(g) + tiny), heavy[r]
