@@ -31,7 +31,7 @@ __global__ __launch_bounds__(64 * W) void lsr_distill_team_kernel(
     __shared__ float student[LSR_MAX_TOP];                // scores of the listed classes
     __shared__ bool first[LSR_MAX_TOP];                   // the class has not been listed before
     __shared__ float part_f[W], list_best, list_high;
-    __shared__ double part_d[W], list_sum, list_cross, list_z;
+    __shared__ double part_d[W], list_sum, list_cross, list_z, list_rest, list_lift;
     __shared__ int again;
     const int tid = threadIdx.x;
     const int64_t r = blockIdx.x;
@@ -82,6 +82,9 @@ __global__ __launch_bounds__(64 * W) void lsr_distill_team_kernel(
         }
         best = wave_max(best);
         high = wave_max(high);
+        // a rest so heavy that its weight relative to the list's best leaves 64 bits: everything relative to the rest instead
+        const double rest_log = REST ? (double)rest[r] : 0.0, lift = rest_log > 500 ? rest_log : 0.0;
+        const double down = lift > 0 ? row_exp2(-lift * ROW_LOG2E) : 1.0;
         // sum of the teacher's weights e^y, of e^y (y - z), of the student's e^z; z relative to the list's highest score
         double sum = 0, cross = 0, z_l = 0;
 #pragma unroll 1
@@ -92,7 +95,7 @@ __global__ __launch_bounds__(64 * W) void lsr_distill_team_kernel(
             sum += p;
             if (p > 0) cross += p * (y - z);
             if (REST && first[j]) z_l += student[j] < INFINITY ? row_exp2(z) : NAN;
-            teacher[j] = (float)p;
+            teacher[j] = (float)(p * down);
         }
         sum = wave_sum(sum);
         cross = wave_sum(cross);
@@ -100,9 +103,11 @@ __global__ __launch_bounds__(64 * W) void lsr_distill_team_kernel(
         if (tid == 0) {
             list_best = best;
             list_high = high;
-            list_sum = sum;
-            list_cross = cross * (1.0 / ROW_LOG2E);
+            list_sum = sum * down;
+            list_cross = cross * (1.0 / ROW_LOG2E) * down;
             list_z = z_l;
+            list_rest = rest_log - lift;
+            list_lift = lift;
         }
     }
     if (W == 1) team_sync<W>();                           // larger teams meet in team_max before they read what is above
@@ -162,15 +167,13 @@ __global__ __launch_bounds__(64 * W) void lsr_distill_team_kernel(
     const double z_r = team_sum<W>((double)part, part_d);
 
     // every thread for itself: no barrier between the sum and the gradient
-    const double w = weight ? (double)weight[r] : 1.0, rest_log = REST ? (double)rest[r] : 0.0;
+    const double w = weight ? (double)weight[r] : 1.0, rest_log = REST ? list_rest : 0.0;
     const float high_l = list_high, m = REST ? row_max(m_r, high_l) : m_r;
     // NaN or +infinity among the scores: their exponentials, and with them the sum, are NaN
     const double shift = !REST ? 1.0 : z_r == 0 ? 0.0 : row_exp2(((double)m_r - m) * unit);
     const double shift_l = high_l > -INFINITY ? row_exp2(((double)high_l - m) * unit) : 1.0;
     const double z = (REST ? shift_l * list_z : 0.0) + (z_r == 0 ? 0.0 : shift * z_r);
-    // a rest so heavy that its weight relative to the list's best leaves 64 bits: everything relative to the rest instead
-    const double lift = rest_log > 500 ? rest_log : 0.0, down = lift > 0 ? row_exp2(-lift * ROW_LOG2E) : 1.0;
-    const double p_r = REST ? row_exp2((rest_log - lift) * ROW_LOG2E) : 0.0, sum = list_sum * down + p_r;
+    const double p_r = REST ? row_exp2(rest_log * ROW_LOG2E) : 0.0, sum = list_sum + p_r;
     const bool nan = z != z, used = w != 0 && list_best > -INFINITY && (m > -INFINITY || nan);
     const double scale = w * temperature;
     if (tid == 0) {
@@ -178,8 +181,8 @@ __global__ __launch_bounds__(64 * W) void lsr_distill_team_kernel(
         if (used && !nan) {
             // the list's scores were taken relative to its own highest
             const double ln_z = row_log(z), gap = (high_l > -INFINITY ? (double)high_l - m : 0.0) * inv_t;
-            l = (list_cross - list_sum * gap) * down / sum + ln_z - row_log(sum) - lift * (list_sum * down / sum);
-            if (REST && p_r > 0) l += p_r / sum * (z_r > 0 ? rest_log - lift - row_log(z_r) - ((double)m_r - m) * inv_t : INFINITY);
+            l = (list_cross - list_sum * gap) / sum + ln_z - row_log(sum) - list_lift * (list_sum / sum);
+            if (REST && p_r > 0) l += p_r / sum * (z_r > 0 ? rest_log - row_log(z_r) - ((double)m_r - m) * inv_t : INFINITY);
         }
         loss[r] = used ? (nan ? NAN : (float)(w * temperature * temperature * l)) : 0.0f;
     }
@@ -214,7 +217,7 @@ __global__ __launch_bounds__(64 * W) void lsr_distill_team_kernel(
 #pragma unroll 1
             for (int i = 0; i < k; ++i) p += cls[i] == cls[j] ? teacher[i] : 0.0f;
         }
-        g[cls[j]] = (T)(float)(scale * (row_exp2(((double)student[j] - m) * unit) / z - p * down / sum));
+        g[cls[j]] = (T)(float)(scale * (row_exp2(((double)student[j] - m) * unit) / z - p / sum));
     }
 }
 
