@@ -14,7 +14,7 @@
 // Long rows, a team of W wavefronts per row (lsr_rows.h).  Wavefront 0 handles the list while the row is on its way.  The
 // listed classes are marked in a bit map, and where there is an outcome for the rest they are blanked in the registers, so
 // that maximum, sum and gradient run over the others alone.  The gradient of the listed classes is written over afterwards.
-// One read and one write of the row: 4096 x 131072 takes 516 us, 4.2 TB/s, a copy of that size 4.75.
+// One read and one write of the row: 4096 x 131072 takes 517 us, 4.2 TB/s, a copy of that size 4.75.
 template <int DT, int W, int N, bool REST, bool GRAD>
 __global__ __launch_bounds__(64 * W) void lsr_distill_team_kernel(
     const typename row_type<DT>::type* __restrict__ scores, int n_classes, int64_t row_stride,
@@ -228,7 +228,7 @@ __global__ __launch_bounds__(64 * W) void lsr_distill_team_kernel(
 // one logarithm instruction sequence for Z, S and the rest together, a lane each.
 // HELD: entries of the list that a lane keeps in registers (k <= 4 HELD), 0 to read them again in each of the three loops.
 // The sums into that table are atomics of one wavefront, so that their order is fixed.  2.2 M x 58 with k = 8, the rest and the
-// gradient takes 307 us, 3.9 TB/s.
+// gradient takes 308 us, 3.9 TB/s.
 template <int DT, int E, int HELD, bool REST, bool GRAD>
 __global__ __launch_bounds__(LSR_ROW_THREADS) void lsr_distill_quad_kernel(
     const typename row_type<DT>::type* __restrict__ scores, int64_t n_rows, int n_classes, int64_t row_stride,

@@ -102,7 +102,8 @@ __device__ __forceinline__ uint64_t list_head(const uint64_t* entry, const uint6
 }
 
 // A row in many passes over memory, by radix selection with weights: for rows that the fast form below does not take (an
-// infinite score, a cut that falls among thousands of scores that are alike).
+// infinite score, a cut that falls among thousands of scores that are alike or, by top_p, too near to a score's edge for 32
+// bits; a small top_k that is near or above the number of groups with a score).
 template <int DT, int W>
 __device__ __forceinline__ void sample_by_radix(const typename row_type<DT>::type* x, int n_classes, float best, double t,
                                                 int top_k, double top_p, double min_p, float u, const sample_args& a,
@@ -192,14 +193,14 @@ __device__ __forceinline__ void sample_by_radix(const typename row_type<DT>::typ
 //
 // Among the first entries of a row: a top_k of at most LSR_MAX_TOP, a min_p that few entries reach, a top_p that a short
 // head seems to hold.  They are collected and put in order as lsr_top_scores does it, weighed, cut, and the uniform number is
-// looked up in the order of their classes.  1 x 32768 with top_k 50 takes 9.5 us, 256 x 131072 25 us (reading them alone 18):
+// looked up in the order of their classes.  1 x 32768 with top_k 50 takes 9.9 us, 256 x 131072 26 us (reading them alone 18):
 // a chain of dependent passes and barriers in one workgroup.  A radix selection in the list instead of comparing its
 // entries took 22 us against 15 for one row.
 //
 // Otherwise every class is weighed, from memory: rows are not kept in registers, which 64-bit weights need.  A cut by order is
 // found from a histogram over the distance to the best score, and the entries of the bin in which it falls.  The weights of
 // what is kept are summed per step of the row, and the step, the run and the class that the uniform number falls on are
-// looked up.  Bound by the 64-bit exponentials of one compute unit per row: 96 x 50001 takes 23 us, with a top_p 41.
+// looked up.  Bound by the 64-bit exponentials of one compute unit per row: 96 x 50001 takes 25 us, with a top_p 47.
 template <int DT, int W>
 __global__ __launch_bounds__(64 * W) void lsr_sample_team_kernel(const typename row_type<DT>::type* __restrict__ scores,
                                                                  int n_classes, int64_t row_stride,
@@ -677,7 +678,7 @@ static void lsr_sample_team(hipStream_t stream, const void* scores_d, int64_t n_
 // Short rows (at most LSR_QUAD_CLASSES classes), a quad per row.  ORDER: some row is cut by its order.  The weights fall
 // with the scores, so a sorted copy of them, without the classes, says which weight is the last one that is kept and how
 // many entries of that weight; where not all of those are, they are taken one by one.  The sums are 64-bit floating ones in
-// a fixed order.  Bound by vector instructions: 2.2 M x 58 with a top_p takes 391 us for 1 664 of them per 16 rows,
+// a fixed order.  Bound by vector instructions: 2.2 M x 58 with a top_p takes 393 us for 1 664 of them per 16 rows,
 // five times what reading the rows takes; sorting score and class together instead of the weights was slower.
 template <int DT, int E, bool ORDER>
 __global__ __launch_bounds__(LSR_ROW_THREADS) void lsr_sample_quad_kernel(const typename row_type<DT>::type* __restrict__ scores,

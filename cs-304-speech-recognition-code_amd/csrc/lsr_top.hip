@@ -17,7 +17,8 @@ int lsr_check_rows(lsr_ctx* ctx, const char* name, const void* scores_d, int dty
 }
 
 // The lowest of the row's first `want` entries by radix selection, eight bits at a time from a histogram of the entries
-// that still match; what the group bound cannot narrow down (tens of thousands of equal scores) comes here.
+// that still match; what the group bound cannot narrow down comes here: more scores above it than the list takes, where
+// `want` is near or above the number of groups with a score, or a few groups hold thousands of the best scores.
 template <int DT, int W>
 __device__ __forceinline__ uint64_t top_radix(const typename row_type<DT>::type* x, int n_classes, int want, int* hist,
                                               uint64_t* shared) {
@@ -47,8 +48,9 @@ __device__ __forceinline__ uint64_t top_radix(const typename row_type<DT>::type*
 
 // Long rows, a team of W wavefronts per row (lsr_rows.h).  ON: workgroups of 16 wavefronts with kept rows fill their compute
 // unit alone; there are as many of them as compute units, and each requests its next row while it collects from this one
-// (2048 x 131072, k = 64, with the rest: 151 us, 3.6 TB/s, 12 % less than with a workgroup per row).  The registers that this takes are missing for the
-// sorting of longer lists, so that it is for k <= 64, whose lists have about 80 entries.
+// (2048 x 131072, k = 64, with the rest: 152 us, 3.5 TB/s, 12 % less than with a workgroup per row), although 26 registers
+// per lane spill in this form.  What it takes is missing for the sorting of longer lists, so that it is for k <= 64, whose
+// lists have about 80 entries.
 template <int DT, int W, int N, bool ON, bool REST>
 __global__ __launch_bounds__(64 * W) void lsr_top_team_kernel(const typename row_type<DT>::type* __restrict__ scores,
                                                               int64_t n_rows, int n_classes, int64_t row_stride, int k,

@@ -221,6 +221,7 @@ def test_rows_are_not_overwritten_under_a_side_stream(digits):
     torch.cuda.synchronize()
 
 
+@pytest.mark.filterwarnings("ignore:The CUDA Graph is empty")
 def test_capturing_the_engines_calls(digits):
     """On the engine's own stream state scores and their targets can be captured together; under another one the capture is
     refused, not left without them."""
