@@ -273,6 +273,11 @@ class Engine:
             self._stream = stream
             self._stream_handle = stream.cuda_stream
 
+    def _capturing(self) -> bool:
+        """Whether the current stream of the engine's device, which need not be the current device, is being captured."""
+        with self.torch.cuda.device(self.device):
+            return self.torch.cuda.is_current_stream_capturing()
+
     @contextlib.contextmanager
     def in_order(self):
         """Engine calls inside come after what torch's current stream has queued and before what it queues next (the two
@@ -282,7 +287,7 @@ class Engine:
             yield
             return
         current = self.torch.cuda.current_stream(self.device)
-        if self.torch.cuda.is_current_stream_capturing():
+        if self._capturing():
             raise NativeError("the engine's calls can only be captured on the engine's own stream (Engine.use_stream)")
         self._stream.wait_stream(current)
         try:
@@ -304,7 +309,7 @@ class Engine:
                     rc = fn(ctx, *args)
                 else:
                     stream = cuda.current_stream(self.device)
-                    if not cuda.is_current_stream_capturing():
+                    if not self._capturing():
                         stream.wait_stream(self._stream)
                     self._check(self.lib.lsr_set_stream(ctx, c_void_p(handle)), ctx)
                     try:
