@@ -47,7 +47,7 @@ def test_a_call_on_a_side_stream_leaves_the_engines_stream_alone(digits):
         return 0
 
     with torch.cuda.stream(side):
-        torch.cuda._sleep(A_WHILE)
+        torch.cuda._sleep(5 * A_WHILE)                    # well beyond what the other thread needs
         eng.on_current_stream(inside)
     torch.cuda.synchronize()
     assert out == [(True, False)]                         # the scores were there while the side stream was still busy
